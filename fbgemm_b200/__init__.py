@@ -10,6 +10,8 @@ Layers, bottom up:
 * ``embedding.py`` the reference's generator API in Python (host mirror)
 * ``tbe.py``       the table-batched operator above the generators (pooled and
                    sequence form, the pruning lookups that run before it)
+* ``paged.py``     a key-value cache in pages: slot maps, rotary positions and
+                   the rows' way in, single-token attention
 * ``workloads.py`` seeded synthetic inputs of the benchmark configurations
 * ``sharding.py``  table-wise sharding over the GPUs of one box
 

@@ -15,7 +15,12 @@ from . import build as _build
 STATUS_SLOTS = 1024
 HOST_LANES = 16
 USER_SLOTS = STATUS_SLOTS - HOST_LANES - 1
+STATUS_BAD_INDEX = 1
+STATUS_SIZE_MISMATCH = 3
 STATUS_PEER_TIMEOUT = 5
+STATUS_NO_PAGES = 6
+STATUS_BAD_PAGE = 7
+PAGED_MAX_BATCH = 16384
 IPC_HANDLE_BYTES = 64
 NOALLOC_MAX_BAGS = 1 << 20
 MAX_PEERS = 8
@@ -80,13 +85,46 @@ class PeerSync(C.Structure):
     ]
 
 
+class PagedCache(C.Structure):
+    """``fbgemm_b200_paged_cache``."""
+
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("num_pages", C.c_int64),
+        ("page_stride", C.c_int64),
+        ("slot_stride", C.c_int64),
+        ("head_stride", C.c_int64),
+        ("page_size", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("in_dtype", C.c_int32),
+        ("bit_rate", C.c_int32),
+    ]
+
+
+class Rotary(C.Structure):
+    """``fbgemm_b200_rotary``."""
+
+    _fields_ = [
+        ("cos_sin", C.c_void_p),
+        ("max_pos", C.c_int64),
+        ("rot_dim", C.c_int32),
+        ("interleaved", C.c_int32),
+        ("axes", C.c_int32),
+        ("section_end", C.c_int32 * 4),
+    ]
+
+
 class Fbgemmb200Error(RuntimeError):
     pass
 
 
 _p = C.c_void_p
 _i64 = C.c_int64
+_i32 = C.c_int32
 _cfgp = C.POINTER(SpmdmConfig)
+_cachep = C.POINTER(PagedCache)
 
 # name -> (restype, argtypes); exactly the symbols the header declares.
 SIGNATURES = {
@@ -145,6 +183,14 @@ SIGNATURES = {
                                            C.c_int, _p]),
     "fbgemm_b200_multi_host_release": (C.c_int, [_p, C.c_int64, _p]),
     "fbgemm_b200_multi_host_destroy": (None, [_p]),
+    "fbgemm_b200_paged_cache_check": (C.c_int, [_cachep]),
+    "fbgemm_b200_paged_slots": (C.c_int, [_p, _i32, _p, _p, _p, _i32, _i64, _p, _i32, _p, _i32, _i32, _p, _p, _p, _p, _p, _p,
+                                          C.c_int, _p]),
+    "fbgemm_b200_rotary_append": (C.c_int, [_p, _cachep, _i64, _i32, _i32, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p,
+                                            _p, _p, _i64, C.POINTER(Rotary), C.c_int, _p]),
+    "fbgemm_b200_paged_attention_workspace": (_i64, [_p, _cachep, _i32, _i32]),
+    "fbgemm_b200_paged_attention": (C.c_int, [_p, _cachep, _i32, _i32, _i32, _p, _i64, _i64, _p, _i32, _i64, _p, C.c_float,
+                                              _i32, _p, _p, _p, _i64, C.c_int, _p]),
     "fbgemm_b200_float_to_fused_8bit_rowwise": (C.c_int, [_p, _i64, C.c_int32, _p, _p]),
     "fbgemm_b200_float_to_fused_nbit_rowwise": (C.c_int, [C.c_int32, _p, _i64, C.c_int32, _p, _p]),
 }

@@ -9,6 +9,23 @@
 
 namespace fbgemm_b200 {
 
+int64_t sm_count() {
+  constexpr int kDevices = 64;
+  static std::atomic<int> counts[kDevices];
+  int device = 0, n = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kDevices) {
+    return 148;
+  }
+  n = counts[device].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) {
+      return 148;
+    }
+    counts[device].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
 namespace {
 
 struct VariantInfo {
@@ -83,24 +100,6 @@ int form_of(const BagTable& t) {
       t.index_size > 0x7fffff00LL;
   const bool options = t.flags & (kSbFirst | kNoBag | kPositional | kLengths);
   return wide ? bag::kWide : t.flags & kPruned ? bag::kMapped : options || t.data_size == 0 ? bag::kFull : bag::kLean;
-}
-
-// The current device's SMs.
-int64_t sm_count() {
-  constexpr int kDevices = 64;
-  static std::atomic<int> counts[kDevices];
-  int device = 0, n = 0;
-  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kDevices) {
-    return 148;
-  }
-  n = counts[device].load(std::memory_order_relaxed);
-  if (n == 0) {
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) {
-      return 148;
-    }
-    counts[device].store(n, std::memory_order_relaxed);
-  }
-  return n;
 }
 
 // Warps that are resident on `sms` SMs at a time, and blocks of the deep form.

@@ -309,6 +309,9 @@ int build_lookup_params(
     int64_t bags_per_peer,
     SpmdmParams* params);
 
+// The current device's SMs.
+int64_t sm_count();
+
 // Process-wide count of kernels launched by this library.
 extern std::atomic<uint64_t> g_launch_count;
 

@@ -44,6 +44,25 @@ static int address_of(PyObject* x, void** p) {
   return *p == NULL && PyErr_Occurred() ? -1 : 0;
 }
 
+/* Addresses of tensors whose strides the caller has looked at. */
+static int pointers(PyObject* const* args, int first, int n, void** p) {
+  for (int i = 0; i < n; ++i) {
+    p[i] = NULL;
+    if (args[first + i] != Py_None) {
+      PyObject* a = PyObject_CallMethodNoArgs(args[first + i], s_data_ptr);
+      if (!a) {
+        return -1;
+      }
+      p[i] = PyLong_AsVoidPtr(a);
+      Py_DECREF(a);
+      if (p[i] == NULL && PyErr_Occurred()) {
+        return -1;
+      }
+    }
+  }
+  return 0;
+}
+
 static int addresses(PyObject* const* args, int first, int n, void** p) {
   for (int i = 0; i < n; ++i) {
     if (address_of(args[first + i], &p[i])) {
@@ -177,6 +196,64 @@ static PyObject* sequence_lookup(PyObject* self, PyObject* const* args, Py_ssize
       (int32_t)out[0], out[1], (int32_t)out[2], (int32_t)out[3], (int32_t)out[4], (int32_t)out[5], stream));
 }
 
+/* paged_slots(ctx, batch, lengths, new_tokens, tables, width, table_stride, free_pages, free_capacity, num_free, page_size,
+ * capacity, slots, positions, requests, offsets, lengths_out, num_free_out, slot, stream) */
+static PyObject* paged_slots(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  (void)self;
+  void *ctx, *in[3], *pages[1], *num[1], *out[6], *stream;
+  int64_t batch, table[2], capacity, size[2], slot;
+  if (arity(n, 20) || handles(args, 0, 1, &ctx) || integers(args, 1, 1, &batch) || pointers(args, 2, 3, in) ||
+      integers(args, 5, 2, table) || pointers(args, 7, 1, pages) || integers(args, 8, 1, &capacity) ||
+      pointers(args, 9, 1, num) || integers(args, 10, 2, size) || pointers(args, 12, 6, out) ||
+      integers(args, 18, 1, &slot) || handles(args, 19, 1, &stream)) {
+    return NULL;
+  }
+  WITHOUT_LOCK(fbgemm_b200_paged_slots(ctx, (int32_t)batch, in[0], in[1], in[2], (int32_t)table[0], table[1], pages[0],
+                                       (int32_t)capacity, num[0], (int32_t)size[0], (int32_t)size[1], out[0], out[1], out[2],
+                                       out[3], out[4], out[5], (int)slot, stream));
+}
+
+/* rotary_append(ctx, cache, tokens, q_heads, dtype, q, token and head stride, k, its strides, v, its strides, q_out, slots,
+ * positions, positions_stride, cos_sin, max_pos, rot_dim, interleaved, axes, 4 section ends, slot, stream) */
+static PyObject* rotary_append(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  (void)self;
+  void *h[2], *x[3], *to[3], *angles, *stream;
+  int64_t size[3], strides[6], positions_stride, r[8], slot;
+  if (arity(n, 29) || handles(args, 0, 2, h) || integers(args, 2, 3, size) || pointers(args, 5, 1, &x[0]) ||
+      integers(args, 6, 2, &strides[0]) || pointers(args, 8, 1, &x[1]) || integers(args, 9, 2, &strides[2]) ||
+      pointers(args, 11, 1, &x[2]) || integers(args, 12, 2, &strides[4]) || pointers(args, 14, 3, to) ||
+      integers(args, 17, 1, &positions_stride) || pointers(args, 18, 1, &angles) || integers(args, 19, 8, r) ||
+      integers(args, 27, 1, &slot) || handles(args, 28, 1, &stream)) {
+    return NULL;
+  }
+  fbgemm_b200_rotary rotary = {angles, r[0], (int32_t)r[1], (int32_t)r[2], (int32_t)r[3],
+                               {(int32_t)r[4], (int32_t)r[5], (int32_t)r[6], (int32_t)r[7]}};
+  WITHOUT_LOCK(fbgemm_b200_rotary_append(h[0], h[1], size[0], (int32_t)size[1], (int32_t)size[2], x[0], strides[0], strides[1],
+                                         x[1], strides[2], strides[3], x[2], strides[4], strides[5], to[0], to[1], to[2],
+                                         positions_stride, angles ? &rotary : NULL, (int)slot, stream));
+}
+
+/* paged_attention(ctx, cache, batch, q_heads, dtype, q, token and head stride, tables, width, table_stride, lengths, scale,
+ * window, out, lse, workspace, workspace_bytes, slot, stream) */
+static PyObject* paged_attention(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  (void)self;
+  void *h[2], *q, *table, *lengths, *out[3], *stream;
+  int64_t size[3], strides[2], width[2], window, bytes, slot;
+  if (arity(n, 20) || handles(args, 0, 2, h) || integers(args, 2, 3, size) || pointers(args, 5, 1, &q) ||
+      integers(args, 6, 2, strides) || pointers(args, 8, 1, &table) || integers(args, 9, 2, width) ||
+      pointers(args, 11, 1, &lengths) || integers(args, 13, 1, &window) || pointers(args, 14, 3, out) ||
+      integers(args, 17, 1, &bytes) || integers(args, 18, 1, &slot) || handles(args, 19, 1, &stream)) {
+    return NULL;
+  }
+  const double scale = PyFloat_AsDouble(args[12]);
+  if (scale == -1.0 && PyErr_Occurred()) {
+    return NULL;
+  }
+  WITHOUT_LOCK(fbgemm_b200_paged_attention(h[0], h[1], (int32_t)size[0], (int32_t)size[1], (int32_t)size[2], q, strides[0],
+                                           strides[1], table, (int32_t)width[0], width[1], lengths, (float)scale,
+                                           (int32_t)window, out[0], out[1], out[2], bytes, (int)slot, stream));
+}
+
 static PyMethodDef methods[] = {
     {"spmdm_launch", (PyCFunction)(void (*)(void))spmdm_launch, METH_FASTCALL, "fbgemm_b200_spmdm_launch"},
     {"spmdm", (PyCFunction)(void (*)(void))spmdm, METH_FASTCALL, "fbgemm_b200_spmdm"},
@@ -184,6 +261,9 @@ static PyMethodDef methods[] = {
     {"quantize", (PyCFunction)(void (*)(void))quantize, METH_FASTCALL, "fbgemm_b200_float_to_fused_*_rowwise"},
     {"pruned_lookup", (PyCFunction)(void (*)(void))pruned_lookup, METH_FASTCALL, "fbgemm_b200_pruned_*_lookup"},
     {"sequence_lookup", (PyCFunction)(void (*)(void))sequence_lookup, METH_FASTCALL, "fbgemm_b200_sequence_lookup*"},
+    {"paged_slots", (PyCFunction)(void (*)(void))paged_slots, METH_FASTCALL, "fbgemm_b200_paged_slots"},
+    {"rotary_append", (PyCFunction)(void (*)(void))rotary_append, METH_FASTCALL, "fbgemm_b200_rotary_append"},
+    {"paged_attention", (PyCFunction)(void (*)(void))paged_attention, METH_FASTCALL, "fbgemm_b200_paged_attention"},
     {NULL, NULL, 0, NULL}};
 
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native_calls", NULL, -1, methods, NULL, NULL, NULL, NULL};

@@ -1,0 +1,937 @@
+// Attention of one new token per request over a paged cache:
+//   o = sum_t p_t v_t,  p = softmax_t(scale q.k_t),  t over the rows that the token sees,
+// for rows of 16-bit values or fused 8- and 4-bit rows (codes, scale s_t and bias b_t), where
+//   q.k_t = s_t (q.c_t) + b_t sum(q)   and   o = sum_t (p_t s_t) c_t + sum_t p_t b_t
+// so that the codes themselves are multiplied and a row's scale and bias cost one operation per score.
+//
+// Bound by memory: a cached row is read once and used for the `group` query heads that share it, 2 operations per byte
+// and head.  That is too much for the fp32 units (8 heads on 4-bit rows: 200 TFLOP/s at the memory's rate) and far too
+// little for 128-row tiles of the large tensor instructions, whose M the few heads would fill to a sixteenth.  So the
+// rows are M and the heads N of m16n8k16: S^T = K Q^T takes 16 rows and 8 heads, O^T = V^T P^T 16 columns and 8 heads,
+// nothing is padded at 8 heads.  The order of a contraction's terms is free, so each lane loads 16 bytes of its rows
+// straight from memory into the registers it feeds the products from; nothing goes through shared memory, and each row
+// may lie anywhere: pages, strides and ends of requests cost an address and a predicate per row.  V's pairs of rows are
+// interleaved in registers; P^T is turned to the second product's layout by movmatrix.
+//
+// One pass with a running maximum and sum per head in fp32 (in registers, per warp).  A warp's next K tile is on its
+// way while it works on V, and the next V while it works on K.  Weights are rounded to 16 bits for the second product:
+// bf16 beside bf16 rows; fp16 (scaled by 2^14, weights down to 2^-28 of the largest keep all 11 bits) otherwise, with
+// the quantized rows' scales taken relative to the largest power of two seen so far.  A weight's rounding is at most
+// half a step of the output's own type, and averages out over the rows.
+//
+// Work is split over the chip by paged_cache.h's rule.  A worker is a block of 4 warps that take the tiles of its units
+// in turn and join their results in shared memory; an item that several workers share is left as partial results, and a
+// second launch (paged_attention_join) adds them up in a fixed order.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "internal.h"
+#include "paged_cache.h"
+
+namespace fbgemm_b200 {
+namespace paged {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr float kWeightShift = 14.f;  // weights are 2^14 times as large as in the formula
+constexpr float kUnshift = 1.f / 16384.f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr unsigned kAll = 0xffffffffu;
+
+// ---- instructions -----------------------------------------------------------------------------------------------------
+
+template <bool BF16>
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+  if constexpr (BF16) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  } else {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+}
+
+// An 8 x 8 matrix of 16-bit values, row i in lanes 4i .. 4i + 3, to its transpose.
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+__device__ __forceinline__ float exp2_of(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// a in the low half.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack(float a, float b) {
+  uint32_t r;
+  if constexpr (BF16) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  } else {
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  }
+  return r;
+}
+
+// N words of a row; read once, so past the first cache.  WIDE: the address is a multiple of 4 N.
+template <int N, bool WIDE>
+__device__ __forceinline__ void load_words(uint32_t* r, const uint8_t* p) {
+  if constexpr (WIDE && N == 4) {
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "l"(p));
+  } else if constexpr (WIDE && N == 2) {
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(r[i]) : "l"(p + 4 * i));
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t half2_add(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t half2_fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+
+// Codes to fp16 without the conversion unit: 1024 + c has c in its lowest bits.  Codes are taken about the middle of
+// their range (c - 128, c - 8), which the bias makes up for: smaller products, smaller roundings.
+__device__ __forceinline__ uint32_t codes8(uint32_t two_bytes_of, uint32_t selector) {
+  return half2_add(__byte_perm(two_bytes_of, 0x64646464u, selector), 0xe480e480u);  // - 1152
+}
+__device__ __forceinline__ uint32_t codes4_low(uint32_t w) {   // nibbles 0 and 4
+  return half2_add((w & 0x000f000fu) | 0x64006400u, 0xe408e408u);  // - 1032
+}
+__device__ __forceinline__ uint32_t codes4_high(uint32_t w) {  // nibbles 1 and 5: 1024 + 16 c
+  return half2_fma((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);  // / 16 - 72
+}
+
+// ---- what a kernel variant is -----------------------------------------------------------------------------------------
+
+// BITS of a cached value, DP columns (dim rounded up to 64, 128 or 256), NT tiles of 8 query heads.
+template <int BITS_, int DP_, int NT_>
+struct Shape {
+  static constexpr int BITS = BITS_, DP = DP_, NT = NT_;
+  static constexpr int kRowWords = DP * BITS / 32;                       // of a row's columns
+  static constexpr int kTileWords = kRowWords / 2;                       // a lane's share of 16 rows
+  static constexpr int PARTS = kTileWords > 32 ? 2 : 1;                  // columns a tile is loaded in
+  static constexpr int SUB = kTileWords >= 32 ? 1 : kTileWords >= 16 ? 2 : 4;  // 16-row steps of a tile
+  static constexpr int ROWS = 16 * SUB;                                  // of a warp's tile
+  static constexpr int UNIT = kWarps * ROWS;
+  static constexpr int SLOTS = (ROWS + 31) / 32;                         // rows whose address a lane keeps
+  static constexpr int KW = kRowWords / 4 < 4 ? kRowWords / 4 : 4;       // words of a K chunk: a lane of four has every 4th
+  static constexpr int KC = kRowWords / 4 / KW / PARTS;                  // K chunks of a lane and part
+  static constexpr int VW = kRowWords / 8 < 4 ? kRowWords / 8 : 4;       // the same for V: a lane of eight
+  static constexpr int VC = kRowWords / 8 / VW / PARTS;
+  static constexpr int BUF = SUB * 2 * KC * KW;                          // = SUB * 4 * VC * VW
+  static constexpr int KSTEPS = DP / 16;
+  static constexpr int MT = DP / 16;                                     // 16-column tiles of the output
+  static constexpr int kPerWord = 32 / BITS;
+  static_assert(BUF == SUB * 4 * VC * VW && BUF <= 32, "a buffer holds either");
+  static constexpr int kHeads = 8 * NT;
+  static constexpr int kPartFloats = kHeads * (DP + 2);
+  // Registers: rows on their way (2 BUF), output (4 NT MT), queries (2 NT KSTEPS).
+  static constexpr int kBlocks = 2 * BUF + 4 * NT * MT + 2 * NT * KSTEPS <= 112 ? 3 : 2;
+};
+
+template <int BITS>
+struct ScaleBias {
+  float scale, bias;
+};
+
+// Scale and bias behind a row's codes.
+template <int BITS, bool WIDE>
+__device__ __forceinline__ ScaleBias<BITS> load_scale_bias(const uint8_t* p, bool there) {
+  ScaleBias<BITS> r{0.f, 0.f};
+  if (there) {
+    if constexpr (BITS == 8) {
+      uint32_t w[2];
+      load_words<2, WIDE>(w, p);
+      r.scale = __uint_as_float(w[0]);
+      r.bias = __fmaf_rn(128.f, r.scale, __uint_as_float(w[1]));
+    } else {
+      uint32_t w;
+      load_words<1, WIDE>(&w, p);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+      r.scale = f.x;
+      r.bias = __fmaf_rn(8.f, r.scale, f.y);
+    }
+  }
+  return r;
+}
+
+// ---- the kernel -------------------------------------------------------------------------------------------------------
+
+template <typename S, bool BF16, bool WIDE>
+__global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(const PagedAttentionParams p) {
+  constexpr int BITS = S::BITS, NT = S::NT, SUB = S::SUB, PARTS = S::PARTS;
+  constexpr bool kMmaBf16 = BITS == 16 && BF16;
+  constexpr int kWords16 = S::KW;  // words of a K chunk
+  __shared__ float sm_o[kWarps][S::kHeads][S::DP];
+  __shared__ float sm_m[kWarps][S::kHeads], sm_l[kWarps][S::kHeads];
+  __shared__ int64_t sm_sums[kWarps];
+  __shared__ int32_t sm_request;
+  __shared__ int64_t sm_unit;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const int per_request = p.kv_heads * p.head_tiles;
+
+  // -- this worker's units, and the request that the first of them belongs to
+  const int chunk = (p.batch + kThreads - 1) / kThreads;
+  const int b0 = min(tid * chunk, p.batch), b1 = min(b0 + chunk, p.batch);
+  int64_t sum = 0;
+  for (int b = b0; b < b1; ++b) {
+    sum += (int64_t)units_of(span_of(p.lengths[b], p.window, p.most_rows), S::UNIT) * per_request;
+  }
+  int64_t before = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t up = __shfl_up_sync(kAll, before, d);
+    before += lane >= d ? up : 0;
+  }
+  if (lane == 31) {
+    sm_sums[warp] = before;
+  }
+  __syncthreads();
+  before -= sum;
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    before += w < warp ? sm_sums[w] : 0;
+    total += sm_sums[w];
+  }
+  const int64_t per = units_per_worker(total, gridDim.x);
+  const int64_t first_unit = (int64_t)blockIdx.x * per, last_unit = min(first_unit + per, total);
+  if (first_unit >= total) {
+    if (tid == 0 && p.open) {
+      p.open[blockIdx.x] = make_int4(0, 0, 0, 0);
+    }
+    return;
+  }
+  if (first_unit >= before && first_unit < before + sum) {
+    for (int b = b0; b < b1; ++b) {
+      const int64_t n = (int64_t)units_of(span_of(p.lengths[b], p.window, p.most_rows), S::UNIT) * per_request;
+      if (first_unit < before + n) {
+        sm_request = b;
+        sm_unit = first_unit - before;
+        break;
+      }
+      before += n;
+    }
+  }
+  __syncthreads();
+  int request = sm_request;
+  int64_t unit_in_request = sm_unit;
+  int64_t unit_at = first_unit;
+  int4 opened = make_int4(0, 0, 0, 0);
+
+  // -- item after item: a request, a cached head and a tile of its query heads
+  while (unit_at < last_unit) {
+    const int32_t length = p.lengths[request];
+    const RowSpan span = span_of(length, p.window, p.most_rows);
+    const int32_t units = units_of(span, S::UNIT);
+    const int item = (int)(unit_in_request / units);
+    const int u0 = (int)(unit_in_request - (int64_t)item * units);
+    const int u1 = (int)min((int64_t)units, u0 + (last_unit - unit_at));
+    const int kv_head = item / p.head_tiles, first_head = (item - kv_head * p.head_tiles) * S::kHeads;
+    const int heads = min(p.group - first_head, S::kHeads);  // of this tile
+    const int q_head0 = kv_head * p.group + first_head;
+    if ((length < 0 || length > p.most_rows) && tid == 0 && item == 0 && u0 == 0 &&
+        atomicCAS(p.status, 0, FBGEMM_B200_STATUS_SIZE_MISMATCH) == 0) {
+      p.status[1] = request;
+      p.status[2] = 0;
+      p.status[3] = length;
+    }
+
+    // -- queries as the products take them: head g of a tile in lanes 4g .. 4g + 3, columns in the order of K's words
+    uint32_t qf[NT][S::KSTEPS][2];
+    float factor[NT][2], q_sum[NT][2];  // heads 2c and 2c + 1
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const bool there = 8 * n + g < heads;
+      const uint8_t* q = p.q + request * p.q_token + (q_head0 + 8 * n + (there ? g : 0)) * p.q_head;
+      constexpr int kQuads = S::kPerWord * kWords16 / 8;  // 16-byte pieces of q per chunk
+      float scale_head = 1.f, sum_head = 0.f;
+      uint32_t w[PARTS * S::KC][kQuads * 4];
+#pragma unroll
+      for (int i = 0; i < PARTS * S::KC; ++i) {
+#pragma unroll
+        for (int j = 0; j < kQuads; ++j) {
+          const int column = (4 * i + c) * (8 * kQuads) + 8 * j;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (there && column < p.dim) {
+            v = *reinterpret_cast<const uint4*>(q + 2 * column);
+          }
+          w[i][4 * j] = v.x;
+          w[i][4 * j + 1] = v.y;
+          w[i][4 * j + 2] = v.z;
+          w[i][4 * j + 3] = v.w;
+        }
+      }
+      if constexpr (BITS != 16) {
+        // Beside fp16 codes the queries are fp16 too; bf16 ones may lie outside its range, so each head is moved by a power of two.
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < PARTS * S::KC; ++i) {
+#pragma unroll
+          for (int j = 0; j < kQuads * 4; ++j) {
+            const float2 f = BF16 ? make_float2(__uint_as_float(w[i][j] << 16), __uint_as_float(w[i][j] & 0xffff0000u))
+                                  : __half22float2(*reinterpret_cast<const __half2*>(&w[i][j]));
+            most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        }
+        most = fmaxf(most, __shfl_xor_sync(kAll, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(kAll, most, 2));
+        const int e = (int)(__float_as_uint(most) >> 23);  // 127 + exponent
+        int move = e == 0 || e == 255 ? 0 : 137 - e;       // the largest comes to lie in [2^10, 2^11)
+        move = min(move, 126);
+        const float up = __uint_as_float((uint32_t)(127 + move) << 23);
+        scale_head = __uint_as_float((uint32_t)(127 - move) << 23);
+#pragma unroll
+        for (int i = 0; i < PARTS * S::KC; ++i) {
+#pragma unroll
+          for (int j = 0; j < kQuads * 4; ++j) {
+            const float2 f = BF16 ? make_float2(__uint_as_float(w[i][j] << 16), __uint_as_float(w[i][j] & 0xffff0000u))
+                                  : __half22float2(*reinterpret_cast<const __half2*>(&w[i][j]));
+            const float x = __fmul_rn(f.x, up), y = __fmul_rn(f.y, up);
+            sum_head += x + y;
+            w[i][j] = pack<false>(x, y);
+          }
+        }
+        sum_head += __shfl_xor_sync(kAll, sum_head, 1);
+        sum_head += __shfl_xor_sync(kAll, sum_head, 2);
+      }
+#pragma unroll
+      for (int i = 0; i < PARTS * S::KC; ++i) {
+        if constexpr (BITS == 4) {
+#pragma unroll
+          for (int j = 0; j < kWords16; ++j) {  // a word of codes: columns (0,4), (1,5) and (2,6), (3,7)
+            const uint32_t w0 = w[i][4 * j], w1 = w[i][4 * j + 1], w2 = w[i][4 * j + 2], w3 = w[i][4 * j + 3];
+            const int k = 2 * (i * kWords16 + j);
+            qf[n][k][0] = __byte_perm(w0, w2, 0x5410);
+            qf[n][k][1] = __byte_perm(w0, w2, 0x7632);
+            qf[n][k + 1][0] = __byte_perm(w1, w3, 0x5410);
+            qf[n][k + 1][1] = __byte_perm(w1, w3, 0x7632);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kQuads * 2; ++j) {
+            qf[n][i * kQuads * 2 + j][0] = w[i][2 * j];
+            qf[n][i * kQuads * 2 + j][1] = w[i][2 * j + 1];
+          }
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        factor[n][x] = __fmul_rn(__shfl_sync(kAll, scale_head, 4 * (2 * c + x)), p.scale_log2);
+        q_sum[n][x] = __shfl_sync(kAll, sum_head, 4 * (2 * c + x));
+      }
+    }
+
+    float o[NT][S::MT][4];
+    float m[NT][2], l[NT][2], bias_sum[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < S::MT; ++i) {
+        o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+      }
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = bias_sum[n][0] = bias_sum[n][1] = 0.f;
+    }
+    int exponent = 1;  // 127 + the exponent that V's scales are taken relative to
+
+    const uint8_t* const k_rows = p.k + kv_head * p.head_stride;
+    const uint8_t* const v_rows = p.v + kv_head * p.head_stride;
+    const int32_t* const table = p.tables + request * p.table_stride;
+
+    // Tile i of this warp: rows first + ((u0 + i) * kWarps + warp) * ROWS onwards.
+    const int tiles = u1 - u0;
+    auto row_of = [&](int i, int s) {
+      return (int64_t)span.first + ((int64_t)(u0 + i) * kWarps + warp) * S::ROWS + lane + 32 * s;
+    };
+    auto read_page = [&](int i, int s) -> int32_t {
+      const int64_t row = row_of(i, s);
+      return i < tiles && row < span.end && lane + 32 * s < S::ROWS ? __ldg(table + (row >> p.page_shift)) : -2;
+    };
+    // Byte offset of the row, -1: none (behind the last, or its page does not exist).
+    auto offset_of = [&](int i, int s, int32_t page) -> int64_t {
+      if (page == -2) {
+        return row_of(i, s) < span.end && i < tiles && lane + 32 * s < S::ROWS ? -3 : -1;
+      }
+      return page < 0 || page >= p.num_pages
+                 ? -3
+                 : page * p.page_stride + (row_of(i, s) & ((1 << p.page_shift) - 1)) * p.slot_stride;
+    };
+    auto checked = [&](int i, int s, int32_t page) -> int64_t {
+      const int64_t off = offset_of(i, s, page);
+      if (off == -3) {
+        if (atomicCAS(p.status, 0, FBGEMM_B200_STATUS_BAD_PAGE) == 0) {
+          p.status[1] = request;
+          p.status[2] = (int32_t)row_of(i, s);
+          p.status[3] = page;
+        }
+        return -1;
+      }
+      return off;
+    };
+
+    uint32_t bufs[2][S::BUF];
+    int64_t now[S::SLOTS], next[S::SLOTS];
+    int32_t pages[S::SLOTS];
+    ScaleBias<BITS> k_sb[S::SLOTS], v_sb[S::SLOTS];
+
+    auto load_k = [&](uint32_t (&buf)[S::BUF], const int64_t (&off)[S::SLOTS], int part) {
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int64_t at = __shfl_sync(kAll, off[s / 2], (16 * s + 8 * r + g) & 31);
+          const uint8_t* row = k_rows + at;
+#pragma unroll
+          for (int i = 0; i < S::KC; ++i) {
+            uint32_t* w = &buf[((s * 2 + r) * S::KC + i) * S::KW];
+            const int ch = 4 * (part * S::KC + i) + c;
+            if (at >= 0 && ch * (S::KW * S::kPerWord) < p.dim) {
+              load_words<S::KW, WIDE>(w, row + ch * (4 * S::KW));
+            } else {
+#pragma unroll
+              for (int j = 0; j < S::KW; ++j) {
+                w[j] = 0;
+              }
+            }
+          }
+        }
+      }
+      if constexpr (BITS != 16) {
+        if (part == 0) {
+#pragma unroll
+          for (int s = 0; s < S::SLOTS; ++s) {
+            k_sb[s] = load_scale_bias<BITS, WIDE>(k_rows + off[s] + p.dim * BITS / 8, off[s] >= 0);
+          }
+        }
+      }
+    };
+    auto load_v = [&](uint32_t (&buf)[S::BUF], const int64_t (&off)[S::SLOTS], int part) {
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {  // rows 2c, 2c + 1, 2c + 8, 2c + 9
+          const int64_t at = __shfl_sync(kAll, off[s / 2], (16 * s + 2 * c + (r & 1) + 8 * (r >> 1)) & 31);
+          const uint8_t* row = v_rows + at;
+#pragma unroll
+          for (int i = 0; i < S::VC; ++i) {
+            uint32_t* w = &buf[((s * 4 + r) * S::VC + i) * S::VW];
+            const int ch = 8 * (part * S::VC + i) + g;
+            if (at >= 0 && ch * (S::VW * S::kPerWord) < p.dim) {
+              load_words<S::VW, WIDE>(w, row + ch * (4 * S::VW));
+            } else {
+#pragma unroll
+              for (int j = 0; j < S::VW; ++j) {
+                w[j] = 0;
+              }
+            }
+          }
+        }
+      }
+      if constexpr (BITS != 16) {
+        if (part == 0) {
+#pragma unroll
+          for (int s = 0; s < S::SLOTS; ++s) {
+            v_sb[s] = load_scale_bias<BITS, WIDE>(v_rows + off[s] + p.dim * BITS / 8, off[s] >= 0);
+          }
+        }
+      }
+    };
+
+#pragma unroll
+    for (int s = 0; s < S::SLOTS; ++s) {
+      pages[s] = read_page(0, s);
+      next[s] = 0;
+    }
+    int32_t pages1[S::SLOTS];
+#pragma unroll
+    for (int s = 0; s < S::SLOTS; ++s) {
+      pages1[s] = read_page(1, s);
+      now[s] = checked(0, s, pages[s]);
+    }
+    load_k(bufs[0], now, 0);
+    if constexpr (PARTS == 2) {
+      load_k(bufs[1], now, 1);
+    } else {
+      load_v(bufs[1], now, 0);
+    }
+#pragma unroll
+    for (int s = 0; s < S::SLOTS; ++s) {
+      next[s] = checked(1, s, pages1[s]);
+      pages[s] = read_page(2, s);
+    }
+
+    for (int i = 0; i < tiles; ++i) {
+      // -- scores
+      float sc[NT][SUB][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+          sc[n][s][0] = sc[n][s][1] = sc[n][s][2] = sc[n][s][3] = 0.f;
+        }
+      }
+      auto score = [&](const uint32_t (&buf)[S::BUF], int part) {
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+#pragma unroll
+          for (int ch = 0; ch < S::KC; ++ch) {
+            const uint32_t* r0 = &buf[(s * 2 * S::KC + ch) * S::KW];
+            const uint32_t* r1 = &buf[((s * 2 + 1) * S::KC + ch) * S::KW];
+            const int k0 = (part * S::KC + ch) * S::KW * S::kPerWord / 4;  // products of this chunk: 4 columns of a lane each
+            if constexpr (BITS == 16) {
+#pragma unroll
+              for (int j = 0; j < S::KW / 2; ++j) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                  mma<kMmaBf16>(sc[n][s], r0[2 * j], r1[2 * j], r0[2 * j + 1], r1[2 * j + 1], qf[n][k0 + j][0],
+                                qf[n][k0 + j][1]);
+                }
+              }
+            } else if constexpr (BITS == 8) {
+#pragma unroll
+              for (int j = 0; j < S::KW; ++j) {
+                const uint32_t a0 = codes8(r0[j], 0x4140), a2 = codes8(r0[j], 0x4342);
+                const uint32_t a1 = codes8(r1[j], 0x4140), a3 = codes8(r1[j], 0x4342);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                  mma<false>(sc[n][s], a0, a1, a2, a3, qf[n][k0 + j][0], qf[n][k0 + j][1]);
+                }
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < S::KW; ++j) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const uint32_t x0 = r0[j] >> (8 * h), x1 = r1[j] >> (8 * h);
+                  const uint32_t a0 = codes4_low(x0), a2 = codes4_high(x0), a1 = codes4_low(x1), a3 = codes4_high(x1);
+#pragma unroll
+                  for (int n = 0; n < NT; ++n) {
+                    mma<false>(sc[n][s], a0, a1, a2, a3, qf[n][k0 + 2 * j + h][0], qf[n][k0 + 2 * j + h][1]);
+                  }
+                }
+              }
+            }
+          }
+        }
+      };
+      score(bufs[0], 0);
+      ScaleBias<BITS> k_now[S::SLOTS];
+#pragma unroll
+      for (int s = 0; s < S::SLOTS; ++s) {
+        k_now[s] = k_sb[s];
+      }
+      if constexpr (PARTS == 2) {
+        load_v(bufs[0], now, 0);
+        score(bufs[1], 1);
+        load_v(bufs[1], now, 1);
+      } else {
+        load_k(bufs[0], next, 0);
+      }
+
+      // -- weights
+      float top[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        top[n][0] = top[n][1] = -INFINITY;
+      }
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int from = (16 * s + 8 * r + g) & 31;
+          const bool there = __shfl_sync(kAll, (int)(now[s / 2] >> 32), from) >= 0;
+          float ks = 1.f, kb = 0.f;
+          if constexpr (BITS != 16) {
+            ks = __shfl_sync(kAll, k_now[s / 2].scale, from);
+            kb = __shfl_sync(kAll, k_now[s / 2].bias, from);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              float v = sc[n][s][2 * r + x];
+              if constexpr (BITS != 16) {
+                v = __fmaf_rn(ks, v, __fmul_rn(kb, q_sum[n][x]));
+              }
+              v = there ? __fmul_rn(v, factor[n][x]) : -INFINITY;
+              sc[n][s][2 * r + x] = v;
+              top[n][x] = fmaxf(top[n][x], v);
+            }
+          }
+        }
+      }
+      float base[NT][2], fade[NT][2];
+      bool faded = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float t = top[n][x];
+          t = fmaxf(t, __shfl_xor_sync(kAll, t, 4));
+          t = fmaxf(t, __shfl_xor_sync(kAll, t, 8));
+          t = fmaxf(t, __shfl_xor_sync(kAll, t, 16));
+          t = fmaxf(t, m[n][x]);
+          const float b = t == -INFINITY ? 0.f : t;  // nothing seen yet: every weight becomes 0
+          fade[n][x] = m[n][x] == t ? 1.f : exp2_of(m[n][x] - b);
+          faded |= m[n][x] != t;
+          // (a largest score of +inf: inf - inf, so that the row is NaN as in the formula)
+          base[n][x] = b - kWeightShift;
+          m[n][x] = t;
+        }
+      }
+      float fade_scale = 1.f, v_unit = 1.f;
+      if constexpr (BITS != 16) {
+        unsigned most = 0;
+#pragma unroll
+        for (int s = 0; s < S::SLOTS; ++s) {
+          most = max(most, (__float_as_uint(v_sb[s].scale) >> 23) & 0xff);
+        }
+        most = __reduce_max_sync(kAll, most);
+        most = min(max(most, 1u), 253u);
+        if ((int)most > exponent) {
+          const int down = (int)most - exponent;
+          fade_scale = down > 126 ? 0.f : __uint_as_float((uint32_t)(127 - down) << 23);
+          exponent = (int)most;
+          faded = true;
+        }
+        v_unit = __uint_as_float((uint32_t)(254 - exponent) << 23);
+      }
+      if (__any_sync(kAll, faded)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            l[n][x] = __fmul_rn(l[n][x], fade[n][x]);
+            bias_sum[n][x] = __fmul_rn(bias_sum[n][x], fade[n][x]);
+            const float f = __fmul_rn(fade[n][x], fade_scale);
+#pragma unroll
+            for (int t = 0; t < S::MT; ++t) {
+              o[n][t][x] = __fmul_rn(o[n][t][x], f);
+              o[n][t][2 + x] = __fmul_rn(o[n][t][2 + x], f);
+            }
+          }
+        }
+      }
+      uint32_t wt[NT][SUB][2];
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int from = (16 * s + 8 * r + g) & 31;
+          float vs = 1.f, vb = 0.f;
+          if constexpr (BITS != 16) {
+            vs = __fmul_rn(__shfl_sync(kAll, v_sb[s / 2].scale, from), v_unit);
+            vb = __shfl_sync(kAll, v_sb[s / 2].bias, from);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float e[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              e[x] = exp2_of(sc[n][s][2 * r + x] - base[n][x]);
+              l[n][x] += e[x];
+              if constexpr (BITS != 16) {
+                bias_sum[n][x] = __fmaf_rn(e[x], vb, bias_sum[n][x]);
+                e[x] = __fmul_rn(e[x], vs);
+              }
+            }
+            wt[n][s][r] = transposed(pack<kMmaBf16>(e[0], e[1]));
+          }
+        }
+      }
+
+      // -- the weighted sum
+      auto weigh = [&](const uint32_t (&buf)[S::BUF], int part) {
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+#pragma unroll
+          for (int ch = 0; ch < S::VC; ++ch) {
+            const uint32_t* r[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              r[j] = &buf[((s * 4 + j) * S::VC + ch) * S::VW];
+            }
+            const int t0 = (part * S::VC + ch) * S::VW * S::kPerWord / 2;  // 16-column tiles: 2 columns of a lane each
+#pragma unroll
+            for (int j = 0; j < S::VW; ++j) {
+              if constexpr (BITS == 16) {
+                const uint32_t a0 = __byte_perm(r[0][j], r[1][j], 0x5410), a1 = __byte_perm(r[0][j], r[1][j], 0x7632);
+                const uint32_t a2 = __byte_perm(r[2][j], r[3][j], 0x5410), a3 = __byte_perm(r[2][j], r[3][j], 0x7632);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                  mma<kMmaBf16>(o[n][t0 + j], a0, a1, a2, a3, wt[n][s][0], wt[n][s][1]);
+                }
+              } else if constexpr (BITS == 8) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const uint32_t x = __byte_perm(r[0][j], r[1][j], h ? 0x7362 : 0x5140);
+                  const uint32_t y = __byte_perm(r[2][j], r[3][j], h ? 0x7362 : 0x5140);
+                  const uint32_t a0 = codes8(x, 0x4140), a1 = codes8(x, 0x4342);
+                  const uint32_t a2 = codes8(y, 0x4140), a3 = codes8(y, 0x4342);
+#pragma unroll
+                  for (int n = 0; n < NT; ++n) {
+                    mma<false>(o[n][t0 + 2 * j + h], a0, a1, a2, a3, wt[n][s][0], wt[n][s][1]);
+                  }
+                }
+              } else {
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {  // codes 2h and 2h + 1 of the word
+                  const uint32_t x = __byte_perm(r[0][j], r[1][j], h < 2 ? 0x5410 : 0x7632) >> (8 * (h & 1));
+                  const uint32_t y = __byte_perm(r[2][j], r[3][j], h < 2 ? 0x5410 : 0x7632) >> (8 * (h & 1));
+                  const uint32_t a0 = codes4_low(x), a1 = codes4_high(x), a2 = codes4_low(y), a3 = codes4_high(y);
+#pragma unroll
+                  for (int n = 0; n < NT; ++n) {
+                    mma<false>(o[n][t0 + 4 * j + h], a0, a1, a2, a3, wt[n][s][0], wt[n][s][1]);
+                  }
+                }
+              }
+            }
+          }
+        }
+      };
+      if constexpr (PARTS == 2) {
+        weigh(bufs[0], 0);
+        load_k(bufs[0], next, 0);
+        weigh(bufs[1], 1);
+        load_k(bufs[1], next, 1);
+      } else {
+        weigh(bufs[1], 0);
+        load_v(bufs[1], next, 0);
+      }
+#pragma unroll
+      for (int s = 0; s < S::SLOTS; ++s) {
+        now[s] = next[s];
+        next[s] = checked(i + 2, s, pages[s]);
+        pages[s] = read_page(i + 3, s);
+      }
+    }
+
+    // -- the warps' results together
+    const float unit = BITS == 16 ? 1.f : __uint_as_float((uint32_t)exponent << 23);
+    __syncthreads();  // (the item before has been read)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int h = 8 * n + 2 * c + x;
+        float sum_l = l[n][x], sum_b = bias_sum[n][x];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          sum_l += __shfl_xor_sync(kAll, sum_l, d);
+          if constexpr (BITS != 16) {
+            sum_b += __shfl_xor_sync(kAll, sum_b, d);
+          }
+        }
+        if (g == 0) {
+          sm_m[warp][h] = m[n][x];
+          sm_l[warp][h] = sum_l;
+        }
+        constexpr int kPer = S::VW * S::kPerWord;  // columns of a lane's V chunk
+#pragma unroll
+        for (int t = 0; t < S::MT; ++t) {
+          const int ch = t / (kPer / 2), j = t % (kPer / 2);
+          float2 v = make_float2(o[n][t][x], o[n][t][2 + x]);
+          if constexpr (BITS != 16) {
+            v.x = __fmaf_rn(v.x, unit, sum_b);
+            v.y = __fmaf_rn(v.y, unit, sum_b);
+          }
+          *reinterpret_cast<float2*>(&sm_o[warp][h][(8 * ch + g) * kPer + 2 * j]) = v;
+        }
+      }
+    }
+    __syncthreads();
+    const bool whole = u0 == 0 && u1 == units;
+    float* const part = whole ? nullptr : p.parts + (2 * (int64_t)blockIdx.x + (u0 == 0)) * S::kPartFloats;
+    for (int at = tid; at < heads * (S::DP / 4); at += kThreads) {
+      const int h = at / (S::DP / 4), column = at % (S::DP / 4) * 4;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        top = fmaxf(top, sm_m[w][h]);
+      }
+      const float base = top == -INFINITY ? 0.f : top;
+      float sum_l = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = exp2_of(sm_m[w][h] - base);
+        const float4 x = *reinterpret_cast<const float4*>(&sm_o[w][h][column]);
+        sum_l = __fmaf_rn(f, sm_l[w][h], sum_l);
+        v.x = __fmaf_rn(f, x.x, v.x);
+        v.y = __fmaf_rn(f, x.y, v.y);
+        v.z = __fmaf_rn(f, x.z, v.z);
+        v.w = __fmaf_rn(f, x.w, v.w);
+      }
+      if (whole) {
+        const float inv = span.end > span.first ? __fdiv_rn(1.f, sum_l) : 0.f;  // no row at all: zeros
+        const int64_t row = (int64_t)request * p.kv_heads * p.group + q_head0 + h;
+        if (column < p.dim) {
+          const uint2 r = make_uint2(pack<BF16>(__fmul_rn(v.x, inv), __fmul_rn(v.y, inv)),
+                                     pack<BF16>(__fmul_rn(v.z, inv), __fmul_rn(v.w, inv)));
+          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + (row * p.dim + column) * 2) = r;
+        }
+        if (column == 0 && p.lse) {
+          p.lse[row] = span.end > span.first ? __fmaf_rn(base, kLn2, logf(__fmul_rn(sum_l, kUnshift))) : -INFINITY;
+        }
+      } else {
+        *reinterpret_cast<float4*>(part + 2 * S::kHeads + h * S::DP + column) = v;
+        if (column == 0) {
+          part[h] = top;
+          part[S::kHeads + h] = sum_l;
+        }
+      }
+    }
+    if (u0 == 0 && u1 < units) {  // others end what this worker began: it names them
+      const int64_t end = unit_at + units;
+      opened = make_int4((int)((end - 1) / per - blockIdx.x), request, item, 0);
+    }
+    unit_at += u1 - u0;
+    unit_in_request += u1 - u0;
+    if (unit_in_request == (int64_t)units * per_request) {
+      ++request;
+      unit_in_request = 0;
+    }
+  }
+  if (tid == 0 && p.open) {
+    p.open[blockIdx.x] = opened;
+  }
+}
+
+// One block per worker and query head of a tile: the item that the worker began, if others end it.
+template <typename S, bool BF16>
+__global__ void __launch_bounds__(kThreads) paged_attention_join(const PagedAttentionParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ float sm_o[kWarps][S::DP];
+  __shared__ float sm_l[kWarps];
+  __shared__ float sm_m[kWarps];
+  const int4 opened = p.open[blockIdx.x];
+  const int kv_head = opened.z / p.head_tiles, first_head = (opened.z - kv_head * p.head_tiles) * S::kHeads;
+  const int h = blockIdx.y;
+  if (opened.x == 0 || h >= p.group - first_head) {
+    return;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = opened.x + 1;
+  auto part_of = [&](int i) {  // what the worker began, then what the next ones ended
+    return p.parts + (2 * ((int64_t)blockIdx.x + i) + (i == 0)) * S::kPartFloats;
+  };
+  float top = -INFINITY;
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    top = fmaxf(top, part_of(i)[h]);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    top = fmaxf(top, __shfl_xor_sync(kAll, top, d));
+  }
+  if (lane == 0) {
+    sm_m[warp] = top;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    top = fmaxf(top, sm_m[w]);
+  }
+  const float base = top == -INFINITY ? 0.f : top;
+  constexpr int kCols = S::DP / 32;
+  float v[kCols], sum_l = 0.f;
+#pragma unroll
+  for (int j = 0; j < kCols; ++j) {
+    v[j] = 0.f;
+  }
+#pragma unroll 4
+  for (int i = warp; i < n; i += kWarps) {
+    const float* part = part_of(i);
+    const float f = exp2_of(part[h] - base);
+    sum_l = __fmaf_rn(f, part[S::kHeads + h], sum_l);
+#pragma unroll
+    for (int j = 0; j < kCols; j += 2) {
+      const float2 x = *reinterpret_cast<const float2*>(part + 2 * S::kHeads + h * S::DP + 32 * j + 2 * lane);
+      v[j] = __fmaf_rn(f, x.x, v[j]);
+      v[j + 1] = __fmaf_rn(f, x.y, v[j + 1]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kCols; j += 2) {
+    *reinterpret_cast<float2*>(&sm_o[warp][32 * j + 2 * lane]) = make_float2(v[j], v[j + 1]);
+  }
+  if (lane == 0) {
+    sm_l[warp] = sum_l;
+  }
+  __syncthreads();
+  sum_l = sm_l[0] + sm_l[1] + sm_l[2] + sm_l[3];
+  const int64_t row = (int64_t)opened.y * p.kv_heads * p.group + kv_head * p.group + first_head + h;
+  const float inv = __fdiv_rn(1.f, sum_l);
+  for (int column = 2 * threadIdx.x; column < p.dim; column += 2 * kThreads) {
+    float a = 0.f, b = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      a += sm_o[w][column];
+      b += sm_o[w][column + 1];
+    }
+    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.out) + (row * p.dim + column) * 2) =
+        pack<BF16>(__fmul_rn(a, inv), __fmul_rn(b, inv));
+  }
+  if (threadIdx.x == 0 && p.lse) {
+    p.lse[row] = __fmaf_rn(base, kLn2, logf(__fmul_rn(sum_l, kUnshift)));
+  }
+}
+
+// ---- launches ---------------------------------------------------------------------------------------------------------
+
+template <typename S>
+PagedAttentionPlan plan_of(int group, int64_t sms) {
+  PagedAttentionPlan r;
+  r.unit = S::UNIT;
+  r.tile_heads = S::kHeads;
+  r.head_tiles = (group + S::kHeads - 1) / S::kHeads;
+  r.workers = (int32_t)(sms * S::kBlocks);
+  r.part_floats = S::kPartFloats;
+  return r;
+}
+
+template <typename S, bool BF16, bool WIDE>
+cudaError_t launch_of(const PagedAttentionPlan& plan, const PagedAttentionParams& p, bool split, cudaStream_t stream) {
+  paged_attention_kernel<S, BF16, WIDE><<<(unsigned)plan.workers, kThreads, 0, stream>>>(p);
+  g_launch_count.fetch_add(1, std::memory_order_relaxed);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || !split) {
+    return e;
+  }
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)plan.workers, (unsigned)(p.group < S::kHeads ? p.group : S::kHeads));
+  config.blockDim = dim3(kThreads);
+  config.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its blocks wait for the first launch themselves
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  e = cudaLaunchKernelEx(&config, paged_attention_join<S, BF16>, p);
+  g_launch_count.fetch_add(1, std::memory_order_relaxed);
+  return e;
+}
+
+}  // namespace paged
+}  // namespace fbgemm_b200

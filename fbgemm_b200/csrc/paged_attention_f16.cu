@@ -1,0 +1,6 @@
+// paged_attention.cuh for rows of fp16 values.
+#include "paged_attention_variants.cuh"
+
+namespace fbgemm_b200 {
+FBGEMM_B200_PAGED_16(paged_attention_f16, false)
+}  // namespace fbgemm_b200

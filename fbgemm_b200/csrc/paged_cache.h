@@ -1,0 +1,126 @@
+// The paged key-value cache: what its kernels share (paged_slots_kernels.cu, rotary_append_kernels.cu,
+// paged_attention.cuh) and the rule by which the attention is split.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+#include "fbgemm_b200/embedding_c_api.h"
+
+namespace fbgemm_b200 {
+
+#ifdef __CUDACC__
+#define FBGEMM_B200_HD __host__ __device__ __forceinline__
+#else
+#define FBGEMM_B200_HD inline
+#endif
+
+// ---- how the attention is split (also compiled on the host by its test) -----------------------------------------------
+//
+// A request's rows are cut into units of `unit` rows, the last one short; every (request, cached head, head tile) has
+// units_of() of them, at least one, so that a request without rows is somebody's too.  All units stand in one line,
+// request after request, head after head, and each worker (a block) takes the same number of neighbours: the chip is
+// filled whatever the lengths are, long requests are split, short ones share a worker.
+
+// Rows [first, end) that a request's new token sees: `length` rows in the cache, the last `window` of them (0: all).
+struct RowSpan {
+  int32_t first, end;
+};
+FBGEMM_B200_HD RowSpan span_of(int32_t length, int32_t window, int64_t most) {
+  int64_t end = length < 0 ? 0 : length;
+  end = end > most ? most : end;
+  const int64_t first = window > 0 && end > window ? end - window : 0;
+  return RowSpan{(int32_t)first, (int32_t)end};
+}
+
+FBGEMM_B200_HD int32_t units_of(RowSpan s, int32_t unit) {
+  const int32_t n = (int32_t)(((int64_t)s.end - s.first + unit - 1) / unit);
+  return n > 0 ? n : 1;
+}
+
+// Units per worker: as even as whole units allow.
+FBGEMM_B200_HD int64_t units_per_worker(int64_t total, int64_t workers) {
+  const int64_t per = (total + workers - 1) / workers;
+  return per > 0 ? per : 1;
+}
+
+// ---- kernel parameters ------------------------------------------------------------------------------------------------
+
+struct PagedSlotsParams {
+  const int32_t* lengths;
+  const int32_t* fresh;      // new tokens of each request
+  int32_t* tables;
+  int64_t table_stride;      // elements between requests
+  const int32_t* free_pages;
+  const int32_t* num_free;
+  int64_t* slots;
+  int32_t* positions;
+  int32_t* requests;
+  int32_t* offsets;
+  int32_t* lengths_out;
+  int32_t* num_free_out;
+  int32_t* status;
+  int32_t batch, width, free_capacity, page_shift, capacity;
+};
+cudaError_t launch_paged_slots(const PagedSlotsParams& p, cudaStream_t stream);
+
+struct RotaryAppendParams {
+  const void *q, *k, *v;                       // 16-bit types, 16-byte aligned rows
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;  // bytes
+  void* q_out;                                 // [tokens, heads, dim], null: q is not rotated
+  const int64_t* slots;
+  const int32_t* positions;                    // [axes, tokens], null: nothing is rotated
+  int64_t positions_stride;                    // elements between axes
+  const float* cos_sin;                        // [max_pos, rot]: cosines, sines
+  int64_t max_pos;
+  uint8_t *k_cache, *v_cache;
+  int64_t page_stride, slot_stride, head_stride, num_slots;   // bytes; rows in all pages
+  int32_t* status;
+  int64_t tokens;
+  int32_t heads, kv_heads, dim, rot, page_shift, axes;
+  int32_t section_end[4];                      // pairs [section_end[a - 1], section_end[a]) turn by axis a
+  int32_t interleaved, bf16, bits;             // bits: 16, 8 or 4
+};
+cudaError_t launch_rotary_append(const RotaryAppendParams& p, cudaStream_t stream);
+
+struct PagedAttentionParams {
+  const uint8_t *k, *v;
+  int64_t page_stride, slot_stride, head_stride;  // bytes
+  const uint8_t* q;
+  int64_t q_token, q_head;                        // bytes
+  const int32_t* tables;
+  int64_t table_stride;
+  const int32_t* lengths;
+  void* out;                                      // [batch, heads, dim]
+  float* lse;                                     // [batch, heads] or null
+  float* parts;                                   // partial results, two per worker
+  int4* open;                                     // per worker: the item that it began and others end
+  int32_t* status;
+  int64_t most_rows;                              // rows that a block table names
+  float scale_log2;                               // softmax scale * log2(e)
+  int32_t num_pages, page_shift, batch, kv_heads, group, head_tiles, dim, window, workers;
+};
+
+// Which kernel a cache takes (paged_attention_kernels.cu).
+struct PagedAttentionShape {
+  int32_t bits;       // 16, 8, 4
+  bool bf16;          // of q, the output and 16-bit rows
+  int32_t dim;
+  int32_t group;      // query heads per cached head
+  bool wide;          // rows 16-byte aligned
+};
+struct PagedAttentionPlan {
+  int32_t unit;        // rows per unit
+  int32_t tile_heads;  // query heads of a tile
+  int32_t head_tiles;
+  int32_t workers;
+  size_t part_floats;  // of one partial result
+};
+PagedAttentionPlan plan_paged_attention(const PagedAttentionShape& s, int64_t sms);
+// `split`: an item may be shared by workers, whose results are then joined by a second launch.
+cudaError_t launch_paged_attention(const PagedAttentionShape& s, const PagedAttentionPlan& plan, const PagedAttentionParams& p,
+                                   bool split, cudaStream_t stream);
+
+}  // namespace fbgemm_b200

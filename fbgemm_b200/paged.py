@@ -1,0 +1,321 @@
+"""A serving step over a key-value cache in pages, on the GPU.
+
+The K and V rows of many requests lie in pages of a cache: 16-bit rows, or the
+fused 8- and 4-bit rows that the row-wise quantizers build and the lookups
+read.  A request's pages are named by its row of a block table.  One step is
+
+    step = paged_slots(lengths, new_tokens, block_tables, free_pages, num_free, page_size, capacity)
+    q = rotary_append(cache, q, k, v, step.slots, step.positions, cos_sin)      # in every layer
+    out = paged_attention(cache, q, block_tables, step.lengths)                 # one new token per request
+
+``paged_slots`` gives out pages and slots from the requests' lengths (beside
+the scan that turns bag lengths into offsets), ``rotary_append`` turns queries
+and keys and stores the new rows (beside the quantizers), ``paged_attention``
+gathers, dequantizes and pools each request's rows with the weights of a
+softmax (beside the pooled lookups).  The reference's operators of this kind are
+fbgemm_gpu/experimental/gen_ai/src/kv_cache; layouts and arithmetic are this
+library's own.
+
+All calls are asynchronous on torch's current stream of the tensors' device,
+allocate through torch only, and may be captured into a CUDA graph.  What they
+find wrong in the tensors' contents shows in status slot ``slot``
+(``fbgemm_b200.status_read``).
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple
+
+import torch
+
+from . import embedding as E
+
+_DTYPE = {torch.float16: 1, torch.bfloat16: 2}      # FBGEMM_B200_OUT_F16, _BF16
+_IN_DTYPE = {torch.float16: 2, torch.bfloat16: 3}   # FBGEMM_B200_IN_F16, _BF16
+
+
+def row_bytes(head_dim: int, bit_rate: int | None) -> int:
+    """Bytes of one cached row: 16-bit values, or codes with fp32 (8-bit rows) or fp16 (4-bit rows) scale and bias."""
+    if bit_rate is None:
+        return 2 * head_dim
+    if bit_rate not in (8, 4):
+        raise ValueError("bit_rate must be 8, 4 or None (16-bit rows)")
+    return head_dim + 8 if bit_rate == 8 else head_dim // 2 + 4
+
+
+class PagedKVCache:
+    """The K and V rows of one layer: ``k`` and ``v`` of shape [pages, page_size,
+    kv_heads, row], laid out alike and in any order of memory with whole rows.
+    ``bit_rate`` None: rows of head_dim float16 or bfloat16 values, 16-byte
+    aligned.  8 or 4: uint8, fused quantized rows, 4-byte aligned (a multiple of
+    16 bytes apart they are read fastest).  Holds the tensors, not a copy."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, bit_rate: int | None = None):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError("k and v are [pages, page_size, kv_heads, row], of one shape and type")
+        if bit_rate is None:
+            if k.dtype not in _DTYPE:
+                raise TypeError("16-bit rows are float16 or bfloat16 (quantized rows: uint8 and a bit_rate)")
+            head_dim = k.shape[3]
+        else:
+            if k.dtype != torch.uint8:
+                raise TypeError("quantized rows are uint8")
+            head_dim = k.shape[3] - 8 if bit_rate == 8 else (k.shape[3] - 4) * 2
+            row_bytes(max(head_dim, 0), bit_rate)
+        strides = [k.stride(i) if k.shape[i] > 1 else 0 for i in range(4)]
+        if strides != [v.stride(i) if v.shape[i] > 1 else 0 for i in range(4)] or strides[3] > 1:
+            raise ValueError("k and v are laid out alike, their rows without gaps")
+        if k.get_device() != v.get_device():
+            raise ValueError("k and v lie on one device")
+        self._k, self._v = k, v
+        self.bit_rate = bit_rate
+        self.dtype = k.dtype if bit_rate is None else None
+        self.num_pages, self.page_size, self.kv_heads = k.shape[:3]
+        self.head_dim = head_dim
+        self.device = k.device
+        size = k.element_size()
+        self._struct = E._capi.PagedCache(
+            k=k.data_ptr(), v=v.data_ptr(), num_pages=self.num_pages, page_stride=strides[0] * size,
+            slot_stride=strides[1] * size, head_stride=strides[2] * size, page_size=self.page_size, kv_heads=self.kv_heads,
+            head_dim=head_dim, in_dtype=0 if bit_rate else _IN_DTYPE[k.dtype], bit_rate=bit_rate or 0)
+        self._address = C.addressof(self._struct)
+        self._workspace = {}   # (query heads, type) -> bytes
+        E._capi.check(E._capi.lib().fbgemm_b200_paged_cache_check(C.byref(self._struct)), "PagedKVCache")
+
+    @classmethod
+    def allocate(cls, num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=torch.bfloat16,
+                 bit_rate: int | None = None, device="cuda", row_alignment: int = 16) -> "PagedKVCache":
+        """A cleared cache.  A head's rows of a page follow one another, as one request reads them; quantized rows are
+        padded to ``row_alignment`` bytes."""
+        n = row_bytes(head_dim, bit_rate)
+        if bit_rate is None:
+            shape, dtype = (num_pages, kv_heads, page_size, head_dim), dtype
+            rows = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(2)]
+        else:
+            pitch = (n + row_alignment - 1) // row_alignment * row_alignment
+            shape = (num_pages, kv_heads, page_size, pitch)
+            rows = [torch.zeros(shape, dtype=torch.uint8, device=device)[..., :n] for _ in range(2)]
+        return cls(*(x.permute(0, 2, 1, 3) for x in rows), bit_rate=bit_rate)
+
+    @property
+    def k(self) -> torch.Tensor:
+        return self._k
+
+    @property
+    def v(self) -> torch.Tensor:
+        return self._v
+
+    def __reduce__(self):   # a copy describes its own tensors
+        return PagedKVCache, (self._k, self._v, self.bit_rate)
+
+    def _workspace_bytes(self, heads: int, dtype) -> int:
+        n = self._workspace.get((heads, dtype))
+        if n is None:
+            rc = E._capi.lib().fbgemm_b200_paged_attention_workspace(
+                E._handle_of(self._k.get_device()), C.byref(self._struct), heads, _DTYPE[dtype])
+            n = self._workspace[heads, dtype] = E._capi.check(rc, "fbgemm_b200_paged_attention_workspace")
+        return n
+
+
+def _on(device: int, **tensors) -> None:
+    for name, x in tensors.items():
+        if x is not None and x.get_device() != device:
+            raise ValueError(f"{name} lies on {x.device}, not with the other tensors")
+    if device < 0:
+        raise ValueError("the tensors have to lie on a CUDA device")
+
+
+def _vector(x: torch.Tensor, dtype, n: int, name: str) -> None:
+    if x.dtype != dtype:
+        raise TypeError(f"{name} is {dtype}, got {x.dtype}")
+    if x.dim() != 1 or x.shape[0] != n or not x.is_contiguous():
+        raise ValueError(f"{name} is a contiguous vector of {n}")
+
+
+def _tables(x: torch.Tensor, batch: int) -> int:
+    """The table's row stride."""
+    if x.dtype != torch.int32:
+        raise TypeError(f"block_tables is torch.int32, got {x.dtype}")
+    if x.dim() != 2 or x.shape[0] != batch:
+        raise ValueError(f"block_tables is [{batch}, pages of a request]")
+    rows, columns = x.stride()
+    if columns != 1 and x.shape[1] > 1:
+        raise ValueError("block_tables has its columns side by side")
+    return rows if batch > 1 else max(rows, x.shape[1])
+
+
+class PagedSlots(NamedTuple):
+    """What ``paged_slots`` returns, all on the device."""
+    slots: torch.Tensor       # int64 [capacity]: page * page_size + place in the page; -1 behind the last row
+    positions: torch.Tensor   # int32 [capacity]: the row's place in its request; 0 behind the last row
+    requests: torch.Tensor    # int32 [capacity]: whose row it is; -1 behind the last row
+    offsets: torch.Tensor     # int32 [batch + 1]: each request's first row
+    lengths: torch.Tensor     # int32 [batch]: lengths + new_tokens
+    num_free: torch.Tensor    # int32 [1]: pages left
+
+
+def paged_slots(lengths: torch.Tensor, new_tokens: torch.Tensor, block_tables: torch.Tensor, free_pages: torch.Tensor,
+                num_free: torch.Tensor, page_size: int, capacity: int, slot: int = 0) -> PagedSlots:
+    """Room for ``new_tokens[b]`` more rows in each request that holds
+    ``lengths[b]`` (int32; negative counts are 0).
+
+    Pages that the new rows need come from the top of the stack
+    ``free_pages[:num_free]``, requests in order, and are entered into
+    ``block_tables`` (int32 [batch, pages], in place; no other entry changes).
+    The maps have ``capacity`` rows: the new rows, request after request, and
+    padding behind them.  A last page that is not full is continued, so it must
+    not be shared with another request.
+
+    All or nothing: if pages, table columns or capacity run out, no page and no
+    slot is given out (``slots`` all -1, lengths and num_free as they were) and
+    the status record is {6, first request that does not fit, its new length,
+    num_free}.  Give the outputs' ``lengths`` and ``num_free`` to the next step;
+    they are not the inputs' memory."""
+    batch = lengths.shape[0]
+    _vector(lengths, torch.int32, batch, "lengths")
+    _vector(new_tokens, torch.int32, batch, "new_tokens")
+    _vector(num_free, torch.int32, 1, "num_free")
+    _vector(free_pages, torch.int32, free_pages.numel(), "free_pages")
+    stride = _tables(block_tables, batch)
+    device = lengths.get_device()
+    _on(device, new_tokens=new_tokens, block_tables=block_tables, free_pages=free_pages, num_free=num_free)
+    slots = torch.empty(capacity, dtype=torch.int64, device=lengths.device)
+    rest = torch.empty(2 * capacity + 2 * batch + 2, dtype=torch.int32, device=lengths.device)
+    positions, requests, offsets, lengths_out, num_free_out = rest.split_with_sizes([capacity, capacity, batch + 1, batch, 1])
+    rc = E._capi.native().paged_slots(
+        E._handle_of(device), batch, lengths, new_tokens, block_tables, block_tables.shape[1], stride, free_pages,
+        free_pages.shape[0], num_free, page_size, capacity, slots, positions, requests, offsets, lengths_out, num_free_out,
+        slot, E._current_stream(device))
+    E._capi.check(rc, "fbgemm_b200_paged_slots")
+    return PagedSlots(slots, positions, requests, offsets, lengths_out, num_free_out)
+
+
+def _heads(x: torch.Tensor, tokens: int, heads: int, dim: int, dtype, name: str):
+    """Token and head stride of [tokens, heads, dim]."""
+    if x.dtype != dtype:
+        raise TypeError(f"{name} is {dtype}, got {x.dtype}")
+    if x.dim() != 3 or x.shape[0] != tokens or x.shape[1] != heads or x.shape[2] != dim:
+        raise ValueError(f"{name} is [{tokens}, {heads}, {dim}], got {list(x.shape)}")
+    t, h, c = x.stride()
+    if c != 1:
+        raise ValueError(f"{name} has a head's values side by side")
+    return t if tokens > 1 else 0, h if heads > 1 else 0
+
+
+def _activation_type(cache: PagedKVCache, dtype, name: str) -> None:
+    if dtype not in _DTYPE or (cache.dtype is not None and dtype != cache.dtype):
+        raise TypeError(f"{name} is {cache.dtype or 'float16 or bfloat16'}, got {dtype}")
+
+
+def rotary_append(cache: PagedKVCache, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
+                  positions: torch.Tensor | None = None, cos_sin: torch.Tensor | None = None, *, sections=None,
+                  interleaved: bool = False, q_out: torch.Tensor | None = None, slot: int = 0) -> torch.Tensor | None:
+    """Turns the heads of ``q`` [tokens, heads, head_dim] and ``k`` [tokens,
+    kv_heads, head_dim] by their positions, stores ``k`` and ``v`` in rows
+    ``slots`` (int64 [tokens], distinct; -1: not stored) of the cache, and returns
+    the turned ``q`` (None if ``q`` is).
+
+    ``cos_sin``: float32 [max_pos, rot_dim], a position's rot_dim / 2 cosines and
+    then its sines; the first rot_dim columns of a head (a multiple of 16) turn,
+    in pairs half of rot_dim apart, or next to each other if ``interleaved``.
+    None: nothing is turned, ``q`` is copied.  ``positions``: int32 [tokens], or [axes,
+    tokens] with ``sections``, the number of pairs of each axis in turn (time,
+    height, width).  The arithmetic is fp32 with one rounding: to 16 bits, or to
+    the codes, scale and bias that ``FloatToFused...Quantized...`` give for the
+    same fp32 row, byte for byte.
+
+    A position outside the table leaves its token's query unturned and its rows
+    unstored (status {1, token, 0, position}); a slot outside the cache stores
+    nothing (status {7, token, 0, slot})."""
+    _activation_type(cache, k.dtype, "k")
+    tokens, dim = k.shape[0], cache.head_dim
+    ks = _heads(k, tokens, cache.kv_heads, dim, k.dtype, "k")
+    vs = _heads(v, tokens, cache.kv_heads, dim, k.dtype, "v")
+    _vector(slots, torch.int64, tokens, "slots")
+    device = cache._k.get_device()
+    heads, qs = 0, (0, 0)
+    if q is not None:
+        heads = q.shape[1] if q.dim() == 3 else 0
+        qs = _heads(q, tokens, heads, dim, k.dtype, "q")
+        if q_out is None:
+            q_out = torch.empty((tokens, heads, dim), dtype=k.dtype, device=q.device)
+        elif q_out.dtype != k.dtype or q_out.shape != q.shape or not q_out.is_contiguous():
+            raise ValueError("q_out is a contiguous tensor of q's shape and type")
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    max_pos, rot, axes, stride, ends = 0, 0, 0, 0, (0, 0, 0, 0)
+    if cos_sin is not None:
+        if positions is None:
+            raise ValueError("cos_sin goes with positions")
+        if cos_sin.dtype != torch.float32 or positions.dtype != torch.int32:
+            raise TypeError("cos_sin is float32, positions are int32")
+        if cos_sin.dim() != 2 or not cos_sin.is_contiguous():
+            raise ValueError("cos_sin is [max_pos, rot_dim], contiguous")
+        max_pos, rot = cos_sin.shape
+        if sections is None:
+            _vector(positions, torch.int32, tokens, "positions")
+            axes, ends = 1, (rot // 2, 0, 0, 0)
+        else:
+            axes = len(sections)
+            if not 1 <= axes <= 4 or min(sections) < 0 or sum(sections) * 2 != rot:
+                raise ValueError("sections are the pairs of 1 to 4 axes, rot_dim / 2 in all")
+            if positions.shape != (axes, tokens) or (positions.stride(1) != 1 and tokens > 1):
+                raise ValueError("with sections, positions is [axes, tokens]")
+            stride = positions.stride(0)
+            total, ends = 0, []
+            for n in sections:
+                total += n
+                ends.append(total)
+            ends += [0] * (4 - axes)
+    elif positions is not None or sections is not None:
+        raise ValueError("positions and sections go with cos_sin")
+    _on(device, q=q, k=k, v=v, slots=slots, positions=positions, cos_sin=cos_sin, q_out=q_out)
+    rc = E._capi.native().rotary_append(
+        E._handle_of(device), cache._address, tokens, heads, _DTYPE[k.dtype], q, *qs, k, *ks, v, *vs, q_out, slots, positions,
+        stride, cos_sin, max_pos, rot, int(interleaved), axes, *ends, slot, E._current_stream(device))
+    E._capi.check(rc, "fbgemm_b200_rotary_append")
+    return q_out
+
+
+def paged_attention(cache: PagedKVCache, q: torch.Tensor, block_tables: torch.Tensor, lengths: torch.Tensor,
+                    scale: float | None = None, window: int = 0, out: torch.Tensor | None = None, return_lse: bool = False,
+                    slot: int = 0):
+    """Attention of one new token per request over its rows of the cache.
+
+    ``q``: [batch, heads, head_dim] float16 or bfloat16 (a 16-bit cache's type),
+    ``heads`` a multiple of the cache's, query head h reading cached head
+    h // (heads / kv_heads).  ``block_tables``: int32 [batch, pages], row t of
+    request b in page ``block_tables[b, t // page_size]``.  ``lengths``: int32
+    [batch], rows of each request with the new token's own.  ``scale``: of the
+    scores, head_dim ** -0.5 by default.  ``window``: rows that a token sees, the
+    last ones (0: all).  Returns [batch, heads, head_dim] in q's type, and with
+    ``return_lse`` the float32 [batch, heads] logarithms of the sums of
+    exp(scale * q.k), by which results over parts of the rows are joined.  A
+    request without rows gets zeros and -inf.
+
+    Scores, sums and the output are fp32 until the output's one rounding; the
+    weights enter the sum over rows as 16-bit numbers.  A page outside the cache
+    is left out (status {7, request, row, page}); a length that is negative or
+    beyond the table is brought within it (status {3, request, 0, length})."""
+    if q.dim() != 3:
+        raise ValueError("q is [batch, heads, head_dim]")
+    batch, heads, dim = q.shape
+    dtype = q.dtype
+    _activation_type(cache, dtype, "q")
+    qs = _heads(q, batch, heads, cache.head_dim, dtype, "q")
+    stride = _tables(block_tables, batch)
+    _vector(lengths, torch.int32, batch, "lengths")
+    device = q.get_device()
+    _on(device, block_tables=block_tables, lengths=lengths, cache=cache._k, out=out)
+    if out is None:
+        out = torch.empty((batch, heads, dim), dtype=dtype, device=q.device)
+    elif out.dtype != dtype or out.shape != q.shape or not out.is_contiguous():
+        raise ValueError("out is a contiguous tensor of q's shape and type")
+    lse = torch.empty((batch, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    n = cache._workspace_bytes(heads, dtype)
+    workspace = torch.empty(n, dtype=torch.uint8, device=q.device)   # the call's own: calls on several streams, captured ones too, share nothing
+    rc = E._capi.native().paged_attention(
+        E._handle_of(device), cache._address, batch, heads, _DTYPE[dtype], q, *qs, block_tables, block_tables.shape[1], stride,
+        lengths, dim ** -0.5 if scale is None else scale, window, out, lse, workspace, n, slot, E._current_stream(device))
+    E._capi.check(rc, "fbgemm_b200_paged_attention")
+    return (out, lse) if return_lse else out

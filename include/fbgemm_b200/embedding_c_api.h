@@ -70,6 +70,8 @@ extern "C" {
 #define FBGEMM_B200_STATUS_SIZE_MISMATCH 3 /* sum of lengths != index_size   */
 #define FBGEMM_B200_STATUS_TABLE_FULL 4 /* hash-map insert found no free slot */
 #define FBGEMM_B200_STATUS_PEER_TIMEOUT 5 /* a peer's counter did not arrive in time */
+#define FBGEMM_B200_STATUS_NO_PAGES 6   /* free pages, table columns or map capacity ran out */
+#define FBGEMM_B200_STATUS_BAD_PAGE 7   /* a page or slot outside the cache */
 
 /* Number of status slots a context owns (see fbgemm_b200_spmdm_launch). */
 #define FBGEMM_B200_STATUS_SLOTS 1024
@@ -852,6 +854,175 @@ FBGEMM_B200_API int fbgemm_b200_float_to_fused_nbit_rowwise(
     int64_t rows,
     int32_t cols,
     uint8_t* output,
+    void* stream);
+
+/* ---- key-value cache in pages -------------------------------------------- */
+
+/*
+ * The serving step of a language model over rows like those of the lookups: K
+ * and V rows of many requests in pages, block tables and slot maps from the
+ * requests' lengths, rotary positions with the rows' way into the cache, and
+ * the attention of one new token per request.  The reference has operators of
+ * this kind in its generative part (fbgemm_gpu/experimental/gen_ai/src/kv_cache);
+ * layouts and arithmetic here are this library's own.
+ *
+ * Row (page, slot, head) of K starts at k + page * page_stride + slot *
+ * slot_stride + head * head_stride, and the same offset from v is V's.  Rows
+ * hold head_dim values: FBGEMM_B200_IN_F16 / _IN_BF16, or (_IN_QUANTIZED) what
+ * the row-wise quantizers of this header give: 8-bit codes, fp32 scale and
+ * bias, or 4-bit codes, fp16 scale and bias.
+ */
+typedef struct fbgemm_b200_paged_cache {
+  void* k;
+  void* v;
+  int64_t num_pages;
+  int64_t page_stride; /* bytes; 16-bit rows: multiples of 16, as k and v are; */
+  int64_t slot_stride; /* quantized rows: multiples of 4 (of 16 is fastest)    */
+  int64_t head_stride;
+  int32_t page_size;   /* rows per page, a power of two, 65536 at most         */
+  int32_t kv_heads;
+  int32_t head_dim;    /* multiple of 16 (4-bit rows: of 32), 256 at most      */
+  int32_t in_dtype;    /* FBGEMM_B200_IN_QUANTIZED, _F16 or _BF16              */
+  int32_t bit_rate;    /* quantized rows: 8 or 4                               */
+} fbgemm_b200_paged_cache;
+
+/* Returns 0 or FBGEMM_B200_EINVAL. */
+FBGEMM_B200_API int fbgemm_b200_paged_cache_check(const fbgemm_b200_paged_cache* cache);
+
+/*
+ * Gives `new_tokens[b]` more rows to each of `batch` requests that hold
+ * `lengths[b]` (negative counts are 0): fresh pages come from the top of the
+ * stack free_pages[0 .. *num_free) (free_capacity entries), requests in order,
+ * and are entered into `block_tables` (`width` columns, rows table_stride
+ * elements apart); no other entry is written.  Maps of `capacity` rows: the
+ * new rows, request after request, then padding: slots (page * page_size +
+ * place in the page; padding -1), positions in the request (0), requests (-1).
+ * offsets[batch + 1] are the requests' first rows in the maps, lengths_out the
+ * new lengths, num_free_out the new height of the stack.  A row that goes to a
+ * page whose entry is negative gets slot -1.
+ * If the stack, the table's columns or the capacity run out, nothing is given
+ * out: slots and requests are all -1, positions and offsets 0, lengths_out =
+ * lengths, num_free_out = num_free, block_tables unchanged, and the record
+ * {NO_PAGES, first request that does not fit, its new length, num_free} is in
+ * status slot `slot`.  batch <= FBGEMM_B200_PAGED_MAX_BATCH, width * page_size
+ * < 2^31.  Inputs and outputs do not overlap.  One launch, nothing allocated.
+ */
+#define FBGEMM_B200_PAGED_MAX_BATCH 16384
+FBGEMM_B200_API int fbgemm_b200_paged_slots(
+    fbgemm_b200_ctx* ctx,
+    int32_t batch,
+    const int32_t* lengths,
+    const int32_t* new_tokens,
+    int32_t* block_tables,
+    int32_t width,
+    int64_t table_stride,
+    const int32_t* free_pages,
+    int32_t free_capacity,
+    const int32_t* num_free,
+    int32_t page_size,
+    int32_t capacity,
+    int64_t* slots,
+    int32_t* positions,
+    int32_t* requests,
+    int32_t* offsets,
+    int32_t* lengths_out,
+    int32_t* num_free_out,
+    int slot,
+    void* stream);
+
+/* How rotary_append turns heads.  Pairs are (i, i + rot_dim / 2), or (2 i, 2 i + 1) if interleaved, of the first rot_dim
+ * columns (a multiple of 16); the others stay.  Pair i < section_end[0] turns by the position on axis 0, i <
+ * section_end[1] on axis 1 and so on; section_end[axes - 1] = rot_dim / 2.  cos_sin: [max_pos][rot_dim], the cosines of
+ * the rot_dim / 2 angles of a position and then their sines. */
+typedef struct fbgemm_b200_rotary {
+  const float* cos_sin;
+  int64_t max_pos;
+  int32_t rot_dim;
+  int32_t interleaved;
+  int32_t axes; /* 1 .. 4 */
+  int32_t section_end[4];
+} fbgemm_b200_rotary;
+
+/*
+ * For each of `tokens` tokens: q_out[token][q_heads][head_dim] = its query
+ * heads turned (q_out NULL: none), and its key heads, turned, and value heads
+ * to row slots[token] of the cache (-1: not stored), from fp32 with one
+ * rounding: to the cache's 16-bit type, or to the bytes that the row-wise
+ * quantizers give for the same fp32 row.  q, k and v are dtype
+ * (FBGEMM_B200_OUT_F16 or _BF16, a 16-bit cache's own), [token][head][head_dim]
+ * with strides in elements that are multiples of 8, 16-byte aligned.
+ * positions: [axes][tokens], axes positions_stride elements apart.  rotary NULL: nothing
+ * is turned.  A position outside [0, max_pos) leaves its token's queries
+ * unturned and its rows unstored and is recorded (BAD_INDEX, token, 0,
+ * position); so is a slot outside the cache (BAD_PAGE, token, 0, slot).
+ * Slots of one call are distinct: a row that two tokens name may get parts of
+ * either.  One launch, nothing allocated.
+ */
+FBGEMM_B200_API int fbgemm_b200_rotary_append(
+    fbgemm_b200_ctx* ctx,
+    const fbgemm_b200_paged_cache* cache,
+    int64_t tokens,
+    int32_t q_heads,
+    int32_t dtype,
+    const void* q,
+    int64_t q_token_stride,
+    int64_t q_head_stride,
+    const void* k,
+    int64_t k_token_stride,
+    int64_t k_head_stride,
+    const void* v,
+    int64_t v_token_stride,
+    int64_t v_head_stride,
+    void* q_out,
+    const int64_t* slots,
+    const int32_t* positions,
+    int64_t positions_stride,
+    const fbgemm_b200_rotary* rotary,
+    int slot,
+    void* stream);
+
+/* Bytes of workspace (16-byte aligned, device memory, contents irrelevant before and after) of one paged_attention call
+ * with `q_heads` query heads; calls that overlap on the GPU need one each.  Negative: an error code. */
+FBGEMM_B200_API int64_t fbgemm_b200_paged_attention_workspace(
+    fbgemm_b200_ctx* ctx,
+    const fbgemm_b200_paged_cache* cache,
+    int32_t q_heads,
+    int32_t dtype);
+
+/*
+ * out[b][h] = sum over rows t of softmax_t(scale * q[b][h] . k_t) v_t with the
+ * rows that request b's newest token sees: [max(0, n - window), n), n =
+ * lengths[b] (window 0: all), row t at page block_tables[b][t / page_size].
+ * Query head h reads cached head h / (q_heads / kv_heads).  lse (or NULL):
+ * [batch][q_heads], the logarithm of the sum of exp(scale * q . k_t).  A
+ * request without rows gets zeros and -inf.  What lies in rows that are not
+ * seen does not matter.  q and out are dtype (FBGEMM_B200_OUT_F16 or _BF16, a
+ * 16-bit cache's own); q strides in elements are multiples of 8.
+ * A page outside the cache is recorded (BAD_PAGE, request, row, page) and its
+ * rows are left out; a negative length, or one beyond the table, is recorded
+ * (SIZE_MISMATCH, request, 0, length) and brought within it.  width *
+ * page_size < 2^31.  At most two launches, nothing allocated.
+ */
+FBGEMM_B200_API int fbgemm_b200_paged_attention(
+    fbgemm_b200_ctx* ctx,
+    const fbgemm_b200_paged_cache* cache,
+    int32_t batch,
+    int32_t q_heads,
+    int32_t dtype,
+    const void* q,
+    int64_t q_token_stride,
+    int64_t q_head_stride,
+    const int32_t* block_tables,
+    int32_t width,
+    int64_t table_stride,
+    const int32_t* lengths,
+    float scale,
+    int32_t window,
+    void* out,
+    float* lse,
+    void* workspace,
+    int64_t workspace_bytes,
+    int slot,
     void* stream);
 
 #ifdef __cplusplus

@@ -1,0 +1,66 @@
+// How paged attention is split over workers: every unit of every request belongs to one worker, and the worker that
+// begins an item names as many followers as there are.
+#include <cstdint>
+#include <cstdio>
+#include <vector>
+
+#include "paged_cache.h"
+
+using namespace fbgemm_b200;
+
+static int failures = 0;
+#define CHECK(x)                                         \
+  do {                                                   \
+    if (!(x)) {                                          \
+      std::printf("%s:%d: %s\n", __FILE__, __LINE__, #x); \
+      ++failures;                                        \
+    }                                                    \
+  } while (0)
+
+int main() {
+  // rows that a token sees
+  CHECK(span_of(0, 0, 100).first == 0 && span_of(0, 0, 100).end == 0);
+  CHECK(span_of(-3, 5, 100).first == 0 && span_of(-3, 5, 100).end == 0);
+  CHECK(span_of(7, 0, 100).first == 0 && span_of(7, 0, 100).end == 7);
+  CHECK(span_of(7, 7, 100).first == 0 && span_of(7, 6, 100).first == 1);
+  CHECK(span_of(2147483647, 0, 2147483647).end == 2147483647);
+  CHECK(span_of(2147483647, 10, 2147483647).first == 2147483637);
+  CHECK(span_of(101, 0, 100).end == 100);
+  // units
+  CHECK(units_of(span_of(0, 0, 9), 64) == 1 && units_of(span_of(1, 0, 9), 64) == 1);
+  CHECK(units_of(span_of(64, 0, 999), 64) == 1 && units_of(span_of(65, 0, 999), 64) == 2);
+  CHECK(units_of(span_of(2147483647, 0, 2147483647), 64) == 33554432);
+  CHECK(units_per_worker(0, 444) == 1 && units_per_worker(444, 444) == 1 && units_per_worker(445, 444) == 2);
+
+  const std::vector<std::vector<int32_t>> batches = {
+      {1}, {0}, {131072}, {0, 0, 0}, {1, 64, 65, 0, 5000}, std::vector<int32_t>(1000, 77), {5, 100000, 3, 3, 70000, 0}};
+  for (const auto& lengths : batches) {
+    for (int heads : {1, 3, 8}) {
+      for (int64_t workers : {1, 7, 296, 444}) {
+        std::vector<int64_t> start;  // of each item, in units
+        std::vector<int32_t> units;
+        int64_t total = 0;
+        for (int32_t n : lengths) {
+          for (int h = 0; h < heads; ++h) {
+            start.push_back(total);
+            units.push_back(units_of(span_of(n, 0, 1 << 30), 64));
+            total += units.back();
+          }
+        }
+        const int64_t per = units_per_worker(total, workers);
+        CHECK(per * workers >= total);
+        for (size_t i = 0; i < start.size(); ++i) {
+          const int64_t first = start[i] / per, last = (start[i] + units[i] - 1) / per;
+          CHECK(last < workers);
+          // as the kernel names them: (end - 1) / per - the worker that begins
+          CHECK((start[i] + units[i] - 1) / per - first == last - first);
+          if (units[i] == 1) {
+            CHECK(first == last);  // an item of one unit needs no joining
+          }
+        }
+      }
+    }
+  }
+  std::printf(failures ? "%d failures\n" : "ok\n", failures);
+  return failures != 0;
+}
