@@ -98,7 +98,7 @@ PagedAttentionShape shape_of(const fbgemm_b200_paged_cache& c, int32_t q_heads, 
   s.bf16 = dtype == FBGEMM_B200_OUT_BF16;
   s.dim = c.head_dim;
   s.group = q_heads / c.kv_heads;
-  s.wide = aligned(c.k, 16) && aligned(c.v, 16) && (c.page_stride | c.slot_stride | c.head_stride) % 16 == 0;
+  s.fast = c.page_size >= 16 && aligned(c.k, 16) && aligned(c.v, 16) && (c.page_stride | c.slot_stride | c.head_stride) % 16 == 0;
   return s;
 }
 
@@ -342,7 +342,7 @@ int fbgemm_b200_paged_attention(
   const PagedAttentionPlan plan = plan_paged_attention(shape, sm_count());
   const int64_t most = (int64_t)width * cache->page_size;
   const int64_t span = window > 0 && window < most ? window : most;
-  const bool split = span > plan.unit;  // (items of one unit have one worker)
+  const bool split = span + (window > 0 ? 15 : 0) > plan.unit;  // (items of one unit have one worker)
   if (split && (!workspace || !aligned(workspace, 16) || workspace_bytes < workspace_bytes_of(plan))) {
     return refuse("paged_attention: workspace missing, unaligned or too small (fbgemm_b200_paged_attention_workspace)");
   }

@@ -1,23 +1,32 @@
 // Attention of one new token per request over a paged cache:
 //   o = sum_t p_t v_t,  p = softmax_t(scale q.k_t),  t over the rows that the token sees,
-// for rows of 16-bit values or fused 8- and 4-bit rows (codes, scale s_t and bias b_t), where
+// for rows of 16-bit values or fused 8- and 4-bit rows (codes c_t, scale s_t and bias b_t), where
 //   q.k_t = s_t (q.c_t) + b_t sum(q)   and   o = sum_t (p_t s_t) c_t + sum_t p_t b_t
-// so that the codes themselves are multiplied and a row's scale and bias cost one operation per score.
+// so that the codes themselves are multiplied and a row's scale and bias cost a few operations per score.
 //
 // Bound by memory: a cached row is read once and used for the `group` query heads that share it, 2 operations per byte
 // and head.  That is too much for the fp32 units (8 heads on 4-bit rows: 200 TFLOP/s at the memory's rate) and far too
 // little for 128-row tiles of the large tensor instructions, whose M the few heads would fill to a sixteenth.  So the
 // rows are M and the heads N of m16n8k16: S^T = K Q^T takes 16 rows and 8 heads, O^T = V^T P^T 16 columns and 8 heads,
 // nothing is padded at 8 heads.  The order of a contraction's terms is free, so each lane loads 16 bytes of its rows
-// straight from memory into the registers it feeds the products from; nothing goes through shared memory, and each row
-// may lie anywhere: pages, strides and ends of requests cost an address and a predicate per row.  V's pairs of rows are
-// interleaved in registers; P^T is turned to the second product's layout by movmatrix.
+// straight from memory into the registers it feeds the products from; nothing goes through shared memory.  V's pairs of
+// rows are interleaved in registers; P^T is turned to the second product's layout by movmatrix.
+//
+// What is left to count is instructions.  Pages of 16 rows and more hold all 16 rows of a step, which then share one
+// address (FAST); smaller pages and unaligned rows exchange an address per row.  Every row is loaded, also those that the
+// token does not see (of the same page, or of page 0 in place of one that does not exist): they are masked in the
+// tiles that have some.  Codes become fp16 by being put into its lowest 8 bits: subnormal numbers, c 2^-24 (4-bit codes in the
+// upper half of them, c 2^-20), which the products take exactly; the power of two is made up for once per score and
+// result.  (The products align a subnormal as if its first bit were set: 4-bit codes in the lowest 4 bits cost 6 bits of
+// the sums, and results that were off by 1e-3.)  A tile's largest score is looked for across lanes only if one exceeds
+// the running maximum by more than 2^kSlack.
 //
 // One pass with a running maximum and sum per head in fp32 (in registers, per warp).  A warp's next K tile is on its
 // way while it works on V, and the next V while it works on K.  Weights are rounded to 16 bits for the second product:
-// bf16 beside bf16 rows; fp16 (scaled by 2^14, weights down to 2^-28 of the largest keep all 11 bits) otherwise, with
-// the quantized rows' scales taken relative to the largest power of two seen so far.  A weight's rounding is at most
-// half a step of the output's own type, and averages out over the rows.
+// bf16 beside bf16 rows; fp16 (2^kShift times as large, so that weights down to 2^-24 of the largest keep all 11 bits)
+// otherwise, with the quantized rows' scales taken relative to the largest power of two seen so far.  A weight's
+// rounding is at most half a step of the output's own type, and averages out over the rows; codes are weighed about the
+// middle of their range (sum w (c - 128) = sum w c - 128 sum w, with the rounded w), which keeps it there.
 //
 // Work is split over the chip by paged_cache.h's rule.  A worker is a block of 4 warps that take the tiles of its units
 // in turn and join their results in shared memory; an item that several workers share is left as partial results, and a
@@ -35,8 +44,10 @@ namespace paged {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr float kWeightShift = 14.f;  // weights are 2^14 times as large as in the formula
-constexpr float kUnshift = 1.f / 16384.f;
+// Weights are 2^kShift times as large as in the formula and at most 2^kSlack above their reference: 2^14 at most, and with
+// a scale of less than 2 below 2^15.
+constexpr float kShift = 10.f, kSlack = 4.f;
+constexpr float kUnshift = 1.f / 1024.f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -81,114 +92,91 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
   return r;
 }
 
-// N words of a row; read once, so past the first cache.  WIDE: the address is a multiple of 4 N.
-template <int N, bool WIDE>
-__device__ __forceinline__ void load_words(uint32_t* r, const uint8_t* p) {
-  if constexpr (WIDE && N == 4) {
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "l"(p));
+// N words of a row, if `ok`, else r stays as it is.  WIDE: the address is a multiple of 4 N.  ONCE: nobody else reads them.
+template <int N, bool WIDE, bool ONCE>
+__device__ __forceinline__ void load_words(uint32_t* r, const uint8_t* p, bool ok) {
+  if constexpr (WIDE && N == 4 && ONCE) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.s32 p, %5, 0;\n@p ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n}"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3])
+                 : "l"(p), "r"((int)ok));
+  } else if constexpr (WIDE && N == 4) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.s32 p, %5, 0;\n@p ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];\n}"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3])
+                 : "l"(p), "r"((int)ok));
   } else if constexpr (WIDE && N == 2) {
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
+    asm volatile("{\n.reg .pred p;\nsetp.ne.s32 p, %3, 0;\n@p ld.global.nc.v2.u32 {%0,%1}, [%2];\n}"
+                 : "+r"(r[0]), "+r"(r[1])
+                 : "l"(p), "r"((int)ok));
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(r[i]) : "l"(p + 4 * i));
+      asm volatile("{\n.reg .pred p;\nsetp.ne.s32 p, %2, 0;\n@p ld.global.nc.u32 %0, [%1];\n}"
+                   : "+r"(r[i])
+                   : "l"(p + 4 * i), "r"((int)ok));
     }
   }
 }
 
-__device__ __forceinline__ uint32_t half2_add(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-__device__ __forceinline__ uint32_t half2_fma(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t r;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-  return r;
+// Nibbles i and i + 4 of a word as subnormal fp16.
+__device__ __forceinline__ uint32_t nibbles(uint32_t w, int i) {
+  return (i == 0 ? w << 4 : w >> (4 * i - 4)) & 0x00f000f0u;
 }
 
-// Codes to fp16 without the conversion unit: 1024 + c has c in its lowest bits.  Codes are taken about the middle of
-// their range (c - 128, c - 8), which the bias makes up for: smaller products, smaller roundings.
-__device__ __forceinline__ uint32_t codes8(uint32_t two_bytes_of, uint32_t selector) {
-  return half2_add(__byte_perm(two_bytes_of, 0x64646464u, selector), 0xe480e480u);  // - 1152
-}
-__device__ __forceinline__ uint32_t codes4_low(uint32_t w) {   // nibbles 0 and 4
-  return half2_add((w & 0x000f000fu) | 0x64006400u, 0xe408e408u);  // - 1032
-}
-__device__ __forceinline__ uint32_t codes4_high(uint32_t w) {  // nibbles 1 and 5: 1024 + 16 c
-  return half2_fma((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);  // / 16 - 72
+__device__ __forceinline__ float2 halves(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
 // ---- what a kernel variant is -----------------------------------------------------------------------------------------
 
-// BITS of a cached value, DP columns (dim rounded up to 64, 128 or 256), NT tiles of 8 query heads.
-template <int BITS_, int DP_, int NT_>
+// BITS of a cached value, DP columns (dim rounded up to 64, 128 or 256), NT tiles of 8 query heads in a warp, HW warps that
+// take further heads of the same rows.
+template <int BITS_, int DP_, int NT_, int HW_>
 struct Shape {
-  static constexpr int BITS = BITS_, DP = DP_, NT = NT_;
-  static constexpr int kRowWords = DP * BITS / 32;                       // of a row's columns
-  static constexpr int kTileWords = kRowWords / 2;                       // a lane's share of 16 rows
-  static constexpr int PARTS = kTileWords > 32 ? 2 : 1;                  // columns a tile is loaded in
-  static constexpr int SUB = kTileWords >= 32 ? 1 : kTileWords >= 16 ? 2 : 4;  // 16-row steps of a tile
-  static constexpr int ROWS = 16 * SUB;                                  // of a warp's tile
-  static constexpr int UNIT = kWarps * ROWS;
-  static constexpr int SLOTS = (ROWS + 31) / 32;                         // rows whose address a lane keeps
-  static constexpr int KW = kRowWords / 4 < 4 ? kRowWords / 4 : 4;       // words of a K chunk: a lane of four has every 4th
-  static constexpr int KC = kRowWords / 4 / KW / PARTS;                  // K chunks of a lane and part
-  static constexpr int VW = kRowWords / 8 < 4 ? kRowWords / 8 : 4;       // the same for V: a lane of eight
+  static constexpr int BITS = BITS_, DP = DP_, NT = NT_, HW = HW_;
+  static constexpr int kRowWords = DP * BITS / 32;                  // of a row's columns
+  static constexpr int kTileWords = kRowWords / 2;                  // a lane's share of 16 rows
+  static constexpr int PARTS = kTileWords > 32 ? 2 : 1;             // columns a tile is loaded in
+  static constexpr int SUB = kTileWords >= 32 ? 1 : 2;              // 16-row steps of a tile
+  static constexpr int ROWS = 16 * SUB;                             // of a warp's tile
+  static constexpr int kRowWarps = kWarps / HW;
+  static constexpr int UNIT = kRowWarps * ROWS;
+  static constexpr int KW = kRowWords / 4 < 4 ? kRowWords / 4 : 4;  // words of a K chunk: a lane of four has every 4th
+  static constexpr int KC = kRowWords / 4 / KW / PARTS;             // K chunks of a lane and part
+  static constexpr int VW = kRowWords / 8 < 4 ? kRowWords / 8 : 4;  // the same for V: a lane of eight
   static constexpr int VC = kRowWords / 8 / VW / PARTS;
-  static constexpr int BUF = SUB * 2 * KC * KW;                          // = SUB * 4 * VC * VW
+  static constexpr int BUF = SUB * 2 * KC * KW;                     // = SUB * 4 * VC * VW
   static constexpr int KSTEPS = DP / 16;
-  static constexpr int MT = DP / 16;                                     // 16-column tiles of the output
+  static constexpr int MT = DP / 16;                                // 16-column tiles of the output
   static constexpr int kPerWord = 32 / BITS;
   static_assert(BUF == SUB * 4 * VC * VW && BUF <= 32, "a buffer holds either");
-  static constexpr int kHeads = 8 * NT;
+  static constexpr int kWarpHeads = 8 * NT;
+  static constexpr int kHeads = kWarpHeads * HW;
   static constexpr int kPartFloats = kHeads * (DP + 2);
-  // Registers: rows on their way (2 BUF), output (4 NT MT), queries (2 NT KSTEPS).
-  static constexpr int kBlocks = 2 * BUF + 4 * NT * MT + 2 * NT * KSTEPS <= 112 ? 3 : 2;
+  static constexpr int kTail = BITS == 8 ? 2 : 1;                   // words of a row's scale and bias
+  // Registers: rows on their way (2 BUF), output (4 NT MT), queries (2 NT KSTEPS), and about 60 more.
+  static constexpr int kRegisters = 2 * BUF + 4 * NT * MT + 2 * NT * KSTEPS;
+  static constexpr int kBlocks = kRegisters <= 64 ? 4 : kRegisters <= 112 ? 3 : 2;
 };
-
-template <int BITS>
-struct ScaleBias {
-  float scale, bias;
-};
-
-// Scale and bias behind a row's codes.
-template <int BITS, bool WIDE>
-__device__ __forceinline__ ScaleBias<BITS> load_scale_bias(const uint8_t* p, bool there) {
-  ScaleBias<BITS> r{0.f, 0.f};
-  if (there) {
-    if constexpr (BITS == 8) {
-      uint32_t w[2];
-      load_words<2, WIDE>(w, p);
-      r.scale = __uint_as_float(w[0]);
-      r.bias = __fmaf_rn(128.f, r.scale, __uint_as_float(w[1]));
-    } else {
-      uint32_t w;
-      load_words<1, WIDE>(&w, p);
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-      r.scale = f.x;
-      r.bias = __fmaf_rn(8.f, r.scale, f.y);
-    }
-  }
-  return r;
-}
 
 // ---- the kernel -------------------------------------------------------------------------------------------------------
 
-template <typename S, bool BF16, bool WIDE>
+// FAST: pages of 16 rows or more, rows 16-byte aligned.
+template <typename S, bool BF16, bool FAST>
 __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(const PagedAttentionParams p) {
   constexpr int BITS = S::BITS, NT = S::NT, SUB = S::SUB, PARTS = S::PARTS;
-  constexpr bool kMmaBf16 = BITS == 16 && BF16;
-  constexpr int kWords16 = S::KW;  // words of a K chunk
-  __shared__ float sm_o[kWarps][S::kHeads][S::DP];
-  __shared__ float sm_m[kWarps][S::kHeads], sm_l[kWarps][S::kHeads];
+  constexpr bool kQuantized = BITS != 16;
+  constexpr bool kMmaBf16 = !kQuantized && BF16;
+  constexpr bool kOnce = S::HW == 1;
+  constexpr float kMiddle = BITS == 8 ? 128.f : 8.f;
+  constexpr float kCode = BITS == 4 ? 1.f / 1048576.f : 1.f / 16777216.f;  // what a code of 1 is to the products
+  __shared__ float sm_o[S::kRowWarps][S::kHeads][S::DP];
+  __shared__ float sm_m[S::kRowWarps][S::kHeads], sm_l[S::kRowWarps][S::kHeads];
   __shared__ int64_t sm_sums[kWarps];
   __shared__ int32_t sm_request;
   __shared__ int64_t sm_unit;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const int row_warp = warp / S::HW, head_warp = warp % S::HW;
   const int per_request = p.kv_heads * p.head_tiles;
 
   // -- this worker's units, and the request that the first of them belongs to
@@ -240,6 +228,19 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
   int64_t unit_at = first_unit;
   int4 opened = make_int4(0, 0, 0, 0);
 
+  // Where a lane's rows and columns lie: K rows g and g + 8 of a step, V rows 2c, 2c + 1, 2c + 8 and 2c + 9.
+  const int64_t k_lane = (FAST ? g * p.slot_stride : 0) + c * (4 * S::KW);
+  const int64_t v_lane = (FAST ? 2 * c * p.slot_stride : 0) + g * (4 * S::VW);
+  const int64_t tail = p.dim * BITS / 8 - c * (4 * S::KW);  // from k_lane's column to scale and bias
+  auto k_column = [&](int part, int i) { return (4 * (part * S::KC + i) + c) * (S::KW * S::kPerWord) < p.dim; };
+  auto v_column = [&](int part, int i) { return (8 * (part * S::VC + i) + g) * (S::VW * S::kPerWord) < p.dim; };
+
+  uint32_t bufs[2][S::BUF];
+#pragma unroll
+  for (int j = 0; j < S::BUF; ++j) {
+    bufs[0][j] = bufs[1][j] = 0;  // columns that no row has stay 0
+  }
+
   // -- item after item: a request, a cached head and a tile of its query heads
   while (unit_at < last_unit) {
     const int32_t length = p.lengths[request];
@@ -258,18 +259,95 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
       p.status[3] = length;
     }
 
-    // -- queries as the products take them: head g of a tile in lanes 4g .. 4g + 3, columns in the order of K's words
+    const uint8_t* const k_rows = p.k + kv_head * p.head_stride;
+    const uint8_t* const v_rows = p.v + kv_head * p.head_stride;
+    const int32_t* const table = p.tables + request * p.table_stride;
+
+    // Tile i of this warp: rows row0 + i * UNIT onwards.
+    const int64_t row0 = aligned_first(span) + ((int64_t)u0 * S::kRowWarps + row_warp) * S::ROWS;
+    const int tiles = (int)min((int64_t)(u1 - u0), row0 < span.end ? (span.end - row0 + S::UNIT - 1) / S::UNIT : 0);
+    // A lane looks after the address of a step's 16 rows (FAST), or of one row.
+    constexpr int kLeaders = FAST ? SUB : S::ROWS;
+    constexpr unsigned kLed = kLeaders == 32 ? kAll : (1u << (kLeaders & 31)) - 1;
+    auto row_of = [&](int i) { return row0 + (int64_t)i * S::UNIT + lane * (FAST ? 16 : 1); };
+    auto led = [&](int i) {
+      const int64_t row = row_of(i);
+      return i < tiles && lane < kLeaders && row < span.end && (FAST || row >= span.first);
+    };
+    auto read_page = [&](int i) { return led(i) ? __ldg(table + (row_of(i) >> p.page_shift)) : 0; };
+    // Byte offset of the row; one that does not exist stands for row 0 of page 0 (and a step's for the first 16).
+    auto offset_of = [&](int i, int32_t page, unsigned& ok) -> int64_t {
+      const bool exists = led(i);
+      const bool good = exists && page >= 0 && page < p.num_pages;
+      if (exists && !good && atomicCAS(p.status, 0, FBGEMM_B200_STATUS_BAD_PAGE) == 0) {
+        p.status[1] = request;
+        p.status[2] = (int32_t)row_of(i);
+        p.status[3] = page;
+      }
+      ok = __ballot_sync(kAll, good);
+      return good ? page * p.page_stride + (row_of(i) & ((1 << p.page_shift) - 1)) * p.slot_stride : 0;
+    };
+
+    uint32_t k_tail[SUB][2][S::kTail], v_tail[SUB][2][S::kTail];
+    auto load_k = [&](uint32_t (&buf)[S::BUF], int64_t off, int part) {
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) {
+        const uint8_t* step = FAST ? k_rows + __shfl_sync(kAll, off, s) + k_lane : nullptr;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint8_t* row = FAST ? step + (r ? 8 * p.slot_stride : 0) : k_rows + __shfl_sync(kAll, off, 16 * s + 8 * r + g) + k_lane;
+#pragma unroll
+          for (int i = 0; i < S::KC; ++i) {
+            load_words<S::KW, FAST || !kQuantized, kOnce>(&buf[((s * 2 + r) * S::KC + i) * S::KW],
+                                                          row + (part * S::KC + i) * (16 * S::KW), k_column(part, i));
+          }
+          if constexpr (kQuantized) {
+            load_words<S::kTail, FAST, false>(k_tail[s][r], row + tail, true);
+          }
+        }
+      }
+    };
+    auto load_v = [&](uint32_t (&buf)[S::BUF], int64_t off, int part) {
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) {
+        const int64_t first = FAST ? __shfl_sync(kAll, off, s) : 0;
+        const uint8_t* step = v_rows + first + v_lane;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint8_t* row = FAST ? step + (r == 0 ? 0 : r == 1 ? 1 : r == 2 ? 8 : 9) * p.slot_stride
+                                    : v_rows + __shfl_sync(kAll, off, 16 * s + 2 * c + (r & 1) + 8 * (r >> 1)) + v_lane;
+#pragma unroll
+          for (int i = 0; i < S::VC; ++i) {
+            load_words<S::VW, FAST || !kQuantized, kOnce>(&buf[((s * 4 + r) * S::VC + i) * S::VW],
+                                                          row + (part * S::VC + i) * (32 * S::VW), v_column(part, i));
+          }
+        }
+        if constexpr (kQuantized) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint8_t* row = FAST ? v_rows + first + k_lane + (r ? 8 * p.slot_stride : 0)
+                                      : v_rows + __shfl_sync(kAll, off, 16 * s + 8 * r + g) + k_lane;
+            load_words<S::kTail, FAST, false>(v_tail[s][r], row + tail, true);
+          }
+        }
+      }
+    };
+
+    // -- the first tiles' way, and the queries as the products take them: head g of a tile in lanes 4g .. 4g + 3, columns in
+    // the order of K's words
+    int32_t page_now = read_page(0), page_next = read_page(1);
     uint32_t qf[NT][S::KSTEPS][2];
     float factor[NT][2], q_sum[NT][2];  // heads 2c and 2c + 1
+    constexpr int kQuads = S::kPerWord * S::KW / 8;  // 16-byte pieces of q per chunk
+    constexpr int kChunks = PARTS * S::KC;
+    uint32_t q_words[NT][kChunks][kQuads * 4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const bool there = 8 * n + g < heads;
-      const uint8_t* q = p.q + request * p.q_token + (q_head0 + 8 * n + (there ? g : 0)) * p.q_head;
-      constexpr int kQuads = S::kPerWord * kWords16 / 8;  // 16-byte pieces of q per chunk
-      float scale_head = 1.f, sum_head = 0.f;
-      uint32_t w[PARTS * S::KC][kQuads * 4];
+      const int head = head_warp * S::kWarpHeads + 8 * n + g;
+      const bool there = head < heads;
+      const uint8_t* q = p.q + request * p.q_token + (q_head0 + (there ? head : 0)) * p.q_head;
 #pragma unroll
-      for (int i = 0; i < PARTS * S::KC; ++i) {
+      for (int i = 0; i < kChunks; ++i) {
 #pragma unroll
         for (int j = 0; j < kQuads; ++j) {
           const int column = (4 * i + c) * (8 * kQuads) + 8 * j;
@@ -277,21 +355,42 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
           if (there && column < p.dim) {
             v = *reinterpret_cast<const uint4*>(q + 2 * column);
           }
-          w[i][4 * j] = v.x;
-          w[i][4 * j + 1] = v.y;
-          w[i][4 * j + 2] = v.z;
-          w[i][4 * j + 3] = v.w;
+          q_words[n][i][4 * j] = v.x;
+          q_words[n][i][4 * j + 1] = v.y;
+          q_words[n][i][4 * j + 2] = v.z;
+          q_words[n][i][4 * j + 3] = v.w;
         }
       }
-      if constexpr (BITS != 16) {
-        // Beside fp16 codes the queries are fp16 too; bf16 ones may lie outside its range, so each head is moved by a power of two.
+    }
+    unsigned ok_now = 0, ok_next = 0;
+    int64_t now = offset_of(0, page_now, ok_now);
+    if (tiles > 0) {
+      load_k(bufs[0], now, 0);
+      if constexpr (PARTS == 2) {
+        load_k(bufs[1], now, 1);
+      } else {
+        load_v(bufs[1], now, 0);
+      }
+    }
+    int64_t next = offset_of(1, page_next, ok_next);
+    page_next = read_page(2);
+
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float scale_head = 1.f, sum_head = 0.f;
+      uint32_t(&w)[kChunks][kQuads * 4] = q_words[n];
+      if constexpr (kQuantized) {
+        // Beside fp16 codes the queries are fp16 too; bf16 ones may lie outside its range, so each head is moved by a power
+        // of two.
+        auto two = [&](uint32_t x) {
+          return BF16 ? make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)) : halves(x);
+        };
         float most = 0.f;
 #pragma unroll
-        for (int i = 0; i < PARTS * S::KC; ++i) {
+        for (int i = 0; i < kChunks; ++i) {
 #pragma unroll
           for (int j = 0; j < kQuads * 4; ++j) {
-            const float2 f = BF16 ? make_float2(__uint_as_float(w[i][j] << 16), __uint_as_float(w[i][j] & 0xffff0000u))
-                                  : __half22float2(*reinterpret_cast<const __half2*>(&w[i][j]));
+            const float2 f = two(w[i][j]);
             most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
           }
         }
@@ -303,11 +402,10 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
         const float up = __uint_as_float((uint32_t)(127 + move) << 23);
         scale_head = __uint_as_float((uint32_t)(127 - move) << 23);
 #pragma unroll
-        for (int i = 0; i < PARTS * S::KC; ++i) {
+        for (int i = 0; i < kChunks; ++i) {
 #pragma unroll
           for (int j = 0; j < kQuads * 4; ++j) {
-            const float2 f = BF16 ? make_float2(__uint_as_float(w[i][j] << 16), __uint_as_float(w[i][j] & 0xffff0000u))
-                                  : __half22float2(*reinterpret_cast<const __half2*>(&w[i][j]));
+            const float2 f = two(w[i][j]);
             const float x = __fmul_rn(f.x, up), y = __fmul_rn(f.y, up);
             sum_head += x + y;
             w[i][j] = pack<false>(x, y);
@@ -317,12 +415,12 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
         sum_head += __shfl_xor_sync(kAll, sum_head, 2);
       }
 #pragma unroll
-      for (int i = 0; i < PARTS * S::KC; ++i) {
+      for (int i = 0; i < kChunks; ++i) {
         if constexpr (BITS == 4) {
 #pragma unroll
-          for (int j = 0; j < kWords16; ++j) {  // a word of codes: columns (0,4), (1,5) and (2,6), (3,7)
+          for (int j = 0; j < S::KW; ++j) {  // a word of codes: columns (0,4), (1,5) and (2,6), (3,7)
             const uint32_t w0 = w[i][4 * j], w1 = w[i][4 * j + 1], w2 = w[i][4 * j + 2], w3 = w[i][4 * j + 3];
-            const int k = 2 * (i * kWords16 + j);
+            const int k = 2 * (i * S::KW + j);
             qf[n][k][0] = __byte_perm(w0, w2, 0x5410);
             qf[n][k][1] = __byte_perm(w0, w2, 0x7632);
             qf[n][k + 1][0] = __byte_perm(w1, w3, 0x5410);
@@ -338,149 +436,33 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
       }
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        factor[n][x] = __fmul_rn(__shfl_sync(kAll, scale_head, 4 * (2 * c + x)), p.scale_log2);
-        q_sum[n][x] = __shfl_sync(kAll, sum_head, 4 * (2 * c + x));
+        const int from = 4 * (2 * c + x);
+        factor[n][x] = __fmul_rn(__shfl_sync(kAll, scale_head, from), p.scale_log2);
+        if constexpr (kQuantized) {
+          factor[n][x] = __fmul_rn(factor[n][x], 1.f / kCode);
+          q_sum[n][x] = __fmul_rn(__shfl_sync(kAll, sum_head, from), kCode);
+        }
       }
     }
 
     float o[NT][S::MT][4];
-    float m[NT][2], l[NT][2], bias_sum[NT][2];
+    // m: what weights are relative to, base = m - kShift; l: their sum over this lane's rows; of the rounded weights
+    // w_sum, of the weights times the rows' biases bias_sum
+    float m[NT][2], base[NT][2], l[NT][2], w_sum[NT][2], bias_sum[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int i = 0; i < S::MT; ++i) {
         o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
       }
-      m[n][0] = m[n][1] = -INFINITY;
-      l[n][0] = l[n][1] = bias_sum[n][0] = bias_sum[n][1] = 0.f;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        m[n][x] = -INFINITY;
+        base[n][x] = -kShift;
+        l[n][x] = w_sum[n][x] = bias_sum[n][x] = 0.f;
+      }
     }
     int exponent = 1;  // 127 + the exponent that V's scales are taken relative to
-
-    const uint8_t* const k_rows = p.k + kv_head * p.head_stride;
-    const uint8_t* const v_rows = p.v + kv_head * p.head_stride;
-    const int32_t* const table = p.tables + request * p.table_stride;
-
-    // Tile i of this warp: rows first + ((u0 + i) * kWarps + warp) * ROWS onwards.
-    const int tiles = u1 - u0;
-    auto row_of = [&](int i, int s) {
-      return (int64_t)span.first + ((int64_t)(u0 + i) * kWarps + warp) * S::ROWS + lane + 32 * s;
-    };
-    auto read_page = [&](int i, int s) -> int32_t {
-      const int64_t row = row_of(i, s);
-      return i < tiles && row < span.end && lane + 32 * s < S::ROWS ? __ldg(table + (row >> p.page_shift)) : -2;
-    };
-    // Byte offset of the row, -1: none (behind the last, or its page does not exist).
-    auto offset_of = [&](int i, int s, int32_t page) -> int64_t {
-      if (page == -2) {
-        return row_of(i, s) < span.end && i < tiles && lane + 32 * s < S::ROWS ? -3 : -1;
-      }
-      return page < 0 || page >= p.num_pages
-                 ? -3
-                 : page * p.page_stride + (row_of(i, s) & ((1 << p.page_shift) - 1)) * p.slot_stride;
-    };
-    auto checked = [&](int i, int s, int32_t page) -> int64_t {
-      const int64_t off = offset_of(i, s, page);
-      if (off == -3) {
-        if (atomicCAS(p.status, 0, FBGEMM_B200_STATUS_BAD_PAGE) == 0) {
-          p.status[1] = request;
-          p.status[2] = (int32_t)row_of(i, s);
-          p.status[3] = page;
-        }
-        return -1;
-      }
-      return off;
-    };
-
-    uint32_t bufs[2][S::BUF];
-    int64_t now[S::SLOTS], next[S::SLOTS];
-    int32_t pages[S::SLOTS];
-    ScaleBias<BITS> k_sb[S::SLOTS], v_sb[S::SLOTS];
-
-    auto load_k = [&](uint32_t (&buf)[S::BUF], const int64_t (&off)[S::SLOTS], int part) {
-#pragma unroll
-      for (int s = 0; s < SUB; ++s) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int64_t at = __shfl_sync(kAll, off[s / 2], (16 * s + 8 * r + g) & 31);
-          const uint8_t* row = k_rows + at;
-#pragma unroll
-          for (int i = 0; i < S::KC; ++i) {
-            uint32_t* w = &buf[((s * 2 + r) * S::KC + i) * S::KW];
-            const int ch = 4 * (part * S::KC + i) + c;
-            if (at >= 0 && ch * (S::KW * S::kPerWord) < p.dim) {
-              load_words<S::KW, WIDE>(w, row + ch * (4 * S::KW));
-            } else {
-#pragma unroll
-              for (int j = 0; j < S::KW; ++j) {
-                w[j] = 0;
-              }
-            }
-          }
-        }
-      }
-      if constexpr (BITS != 16) {
-        if (part == 0) {
-#pragma unroll
-          for (int s = 0; s < S::SLOTS; ++s) {
-            k_sb[s] = load_scale_bias<BITS, WIDE>(k_rows + off[s] + p.dim * BITS / 8, off[s] >= 0);
-          }
-        }
-      }
-    };
-    auto load_v = [&](uint32_t (&buf)[S::BUF], const int64_t (&off)[S::SLOTS], int part) {
-#pragma unroll
-      for (int s = 0; s < SUB; ++s) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {  // rows 2c, 2c + 1, 2c + 8, 2c + 9
-          const int64_t at = __shfl_sync(kAll, off[s / 2], (16 * s + 2 * c + (r & 1) + 8 * (r >> 1)) & 31);
-          const uint8_t* row = v_rows + at;
-#pragma unroll
-          for (int i = 0; i < S::VC; ++i) {
-            uint32_t* w = &buf[((s * 4 + r) * S::VC + i) * S::VW];
-            const int ch = 8 * (part * S::VC + i) + g;
-            if (at >= 0 && ch * (S::VW * S::kPerWord) < p.dim) {
-              load_words<S::VW, WIDE>(w, row + ch * (4 * S::VW));
-            } else {
-#pragma unroll
-              for (int j = 0; j < S::VW; ++j) {
-                w[j] = 0;
-              }
-            }
-          }
-        }
-      }
-      if constexpr (BITS != 16) {
-        if (part == 0) {
-#pragma unroll
-          for (int s = 0; s < S::SLOTS; ++s) {
-            v_sb[s] = load_scale_bias<BITS, WIDE>(v_rows + off[s] + p.dim * BITS / 8, off[s] >= 0);
-          }
-        }
-      }
-    };
-
-#pragma unroll
-    for (int s = 0; s < S::SLOTS; ++s) {
-      pages[s] = read_page(0, s);
-      next[s] = 0;
-    }
-    int32_t pages1[S::SLOTS];
-#pragma unroll
-    for (int s = 0; s < S::SLOTS; ++s) {
-      pages1[s] = read_page(1, s);
-      now[s] = checked(0, s, pages[s]);
-    }
-    load_k(bufs[0], now, 0);
-    if constexpr (PARTS == 2) {
-      load_k(bufs[1], now, 1);
-    } else {
-      load_v(bufs[1], now, 0);
-    }
-#pragma unroll
-    for (int s = 0; s < S::SLOTS; ++s) {
-      next[s] = checked(1, s, pages1[s]);
-      pages[s] = read_page(2, s);
-    }
 
     for (int i = 0; i < tiles; ++i) {
       // -- scores
@@ -512,8 +494,8 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
             } else if constexpr (BITS == 8) {
 #pragma unroll
               for (int j = 0; j < S::KW; ++j) {
-                const uint32_t a0 = codes8(r0[j], 0x4140), a2 = codes8(r0[j], 0x4342);
-                const uint32_t a1 = codes8(r1[j], 0x4140), a3 = codes8(r1[j], 0x4342);
+                const uint32_t a0 = __byte_perm(r0[j], 0, 0x4140), a2 = __byte_perm(r0[j], 0, 0x4342);
+                const uint32_t a1 = __byte_perm(r1[j], 0, 0x4140), a3 = __byte_perm(r1[j], 0, 0x4342);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                   mma<false>(sc[n][s], a0, a1, a2, a3, qf[n][k0 + j][0], qf[n][k0 + j][1]);
@@ -524,8 +506,8 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
               for (int j = 0; j < S::KW; ++j) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                  const uint32_t x0 = r0[j] >> (8 * h), x1 = r1[j] >> (8 * h);
-                  const uint32_t a0 = codes4_low(x0), a2 = codes4_high(x0), a1 = codes4_low(x1), a3 = codes4_high(x1);
+                  const uint32_t a0 = nibbles(r0[j], 2 * h), a2 = nibbles(r0[j], 2 * h + 1);
+                  const uint32_t a1 = nibbles(r1[j], 2 * h), a3 = nibbles(r1[j], 2 * h + 1);
 #pragma unroll
                   for (int n = 0; n < NT; ++n) {
                     mma<false>(sc[n][s], a0, a1, a2, a3, qf[n][k0 + 2 * j + h][0], qf[n][k0 + 2 * j + h][1]);
@@ -537,114 +519,150 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
         }
       };
       score(bufs[0], 0);
-      ScaleBias<BITS> k_now[S::SLOTS];
+      float2 k_sb[SUB][2];
+      if constexpr (kQuantized) {
 #pragma unroll
-      for (int s = 0; s < S::SLOTS; ++s) {
-        k_now[s] = k_sb[s];
+        for (int s = 0; s < SUB; ++s) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            if constexpr (BITS == 8) {
+              k_sb[s][r] = make_float2(__uint_as_float(k_tail[s][r][0]), __uint_as_float(k_tail[s][r][S::kTail - 1]));
+            } else {
+              k_sb[s][r] = halves(k_tail[s][r][0]);
+            }
+          }
+        }
       }
       if constexpr (PARTS == 2) {
         load_v(bufs[0], now, 0);
         score(bufs[1], 1);
         load_v(bufs[1], now, 1);
-      } else {
+      } else if (i + 1 < tiles) {
         load_k(bufs[0], next, 0);
       }
 
-      // -- weights
-      float top[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        top[n][0] = top[n][1] = -INFINITY;
-      }
+      // -- rows that the token does not see
+      const int64_t row = row0 + (int64_t)i * S::UNIT;
+      const bool partial = row < span.first || row + S::ROWS > span.end || ok_now != kLed;
+      auto seen = [&](int at) {
+        return row + at >= span.first && row + at < span.end && ((ok_now >> (FAST ? at / 16 : at)) & 1);
+      };
 #pragma unroll
       for (int s = 0; s < SUB; ++s) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int from = (16 * s + 8 * r + g) & 31;
-          const bool there = __shfl_sync(kAll, (int)(now[s / 2] >> 32), from) >= 0;
-          float ks = 1.f, kb = 0.f;
-          if constexpr (BITS != 16) {
-            ks = __shfl_sync(kAll, k_now[s / 2].scale, from);
-            kb = __shfl_sync(kAll, k_now[s / 2].bias, from);
-          }
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              float v = sc[n][s][2 * r + x];
-              if constexpr (BITS != 16) {
-                v = __fmaf_rn(ks, v, __fmul_rn(kb, q_sum[n][x]));
+              float& v = sc[n][s][2 * r + x];
+              if constexpr (kQuantized) {
+                v = __fmaf_rn(k_sb[s][r].x, v, __fmul_rn(k_sb[s][r].y, q_sum[n][x]));
               }
-              v = there ? __fmul_rn(v, factor[n][x]) : -INFINITY;
-              sc[n][s][2 * r + x] = v;
-              top[n][x] = fmaxf(top[n][x], v);
+              v = __fmul_rn(v, factor[n][x]);
             }
           }
         }
       }
-      float base[NT][2], fade[NT][2];
-      bool faded = false;
+      if (partial) {
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const bool there = seen(16 * s + 8 * r + g);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              sc[n][s][2 * r] = there ? sc[n][s][2 * r] : -INFINITY;
+              sc[n][s][2 * r + 1] = there ? sc[n][s][2 * r + 1] : -INFINITY;
+            }
+            if constexpr (kQuantized) {
+#pragma unroll
+              for (int j = 0; j < S::kTail; ++j) {
+                v_tail[s][r][j] = there ? v_tail[s][r][j] : 0;
+              }
+            }
+          }
+        }
+      }
+
+      // -- weights
+      bool more = false;
+      float top[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          float t = top[n][x];
-          t = fmaxf(t, __shfl_xor_sync(kAll, t, 4));
-          t = fmaxf(t, __shfl_xor_sync(kAll, t, 8));
-          t = fmaxf(t, __shfl_xor_sync(kAll, t, 16));
-          t = fmaxf(t, m[n][x]);
-          const float b = t == -INFINITY ? 0.f : t;  // nothing seen yet: every weight becomes 0
-          fade[n][x] = m[n][x] == t ? 1.f : exp2_of(m[n][x] - b);
-          faded |= m[n][x] != t;
-          // (a largest score of +inf: inf - inf, so that the row is NaN as in the formula)
-          base[n][x] = b - kWeightShift;
-          m[n][x] = t;
-        }
-      }
-      float fade_scale = 1.f, v_unit = 1.f;
-      if constexpr (BITS != 16) {
-        unsigned most = 0;
+          top[n][x] = fmaxf(sc[n][0][x], sc[n][0][2 + x]);
 #pragma unroll
-        for (int s = 0; s < S::SLOTS; ++s) {
-          most = max(most, (__float_as_uint(v_sb[s].scale) >> 23) & 0xff);
+          for (int s = 1; s < SUB; ++s) {
+            top[n][x] = fmaxf(top[n][x], fmaxf(sc[n][s][x], sc[n][s][2 + x]));
+          }
+          more |= top[n][x] > m[n][x] + kSlack;
         }
-        most = __reduce_max_sync(kAll, most);
-        most = min(max(most, 1u), 253u);
-        if ((int)most > exponent) {
-          const int down = (int)most - exponent;
-          fade_scale = down > 126 ? 0.f : __uint_as_float((uint32_t)(127 - down) << 23);
-          exponent = (int)most;
-          faded = true;
-        }
-        v_unit = __uint_as_float((uint32_t)(254 - exponent) << 23);
       }
-      if (__any_sync(kAll, faded)) {
+      float2 v_sb[SUB][2];
+      unsigned largest = 0;
+      if constexpr (kQuantized) {
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            if constexpr (BITS == 8) {
+              v_sb[s][r] = make_float2(__uint_as_float(v_tail[s][r][0]), __uint_as_float(v_tail[s][r][S::kTail - 1]));
+            } else {
+              v_sb[s][r] = halves(v_tail[s][r][0]);
+            }
+            largest = max(largest, (__float_as_uint(v_sb[s][r].x) >> 23) & 0xff);
+          }
+        }
+        largest = min(largest, 253u);
+        more |= (int)largest > exponent;
+      }
+      if (__any_sync(kAll, more)) {
+        float fade_scale = 1.f;
+        if constexpr (kQuantized) {
+          const int to = (int)__reduce_max_sync(kAll, largest);
+          if (to > exponent) {
+            fade_scale = to - exponent > 126 ? 0.f : __uint_as_float((uint32_t)(127 - (to - exponent)) << 23);
+            exponent = to;
+          }
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            l[n][x] = __fmul_rn(l[n][x], fade[n][x]);
-            bias_sum[n][x] = __fmul_rn(bias_sum[n][x], fade[n][x]);
-            const float f = __fmul_rn(fade[n][x], fade_scale);
+            float t = top[n][x];
+            t = fmaxf(t, __shfl_xor_sync(kAll, t, 4));
+            t = fmaxf(t, __shfl_xor_sync(kAll, t, 8));
+            t = fmaxf(t, __shfl_xor_sync(kAll, t, 16));
+            t = fmaxf(t, m[n][x]);
+            const float b = t == -INFINITY ? 0.f : t;  // nothing seen yet: every weight is 0
+            // (a largest score of +inf: inf - inf, so that the row becomes NaN as in the formula)
+            const float fade = m[n][x] == t ? 1.f : exp2_of(m[n][x] - b);
+            m[n][x] = t;
+            base[n][x] = b - kShift;
+            l[n][x] = __fmul_rn(l[n][x], fade);
+            const float f = __fmul_rn(fade, fade_scale);
+            if constexpr (kQuantized) {
+              bias_sum[n][x] = __fmul_rn(bias_sum[n][x], fade);
+              w_sum[n][x] = __fmul_rn(w_sum[n][x], f);
+            }
 #pragma unroll
-            for (int t = 0; t < S::MT; ++t) {
-              o[n][t][x] = __fmul_rn(o[n][t][x], f);
-              o[n][t][2 + x] = __fmul_rn(o[n][t][2 + x], f);
+            for (int k = 0; k < S::MT; ++k) {
+              o[n][k][x] = __fmul_rn(o[n][k][x], f);
+              o[n][k][2 + x] = __fmul_rn(o[n][k][2 + x], f);
             }
           }
         }
       }
       uint32_t wt[NT][SUB][2];
+      const float v_unit = __uint_as_float((uint32_t)(254 - exponent) << 23);
 #pragma unroll
       for (int s = 0; s < SUB; ++s) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int from = (16 * s + 8 * r + g) & 31;
-          float vs = 1.f, vb = 0.f;
-          if constexpr (BITS != 16) {
-            vs = __fmul_rn(__shfl_sync(kAll, v_sb[s / 2].scale, from), v_unit);
-            vb = __shfl_sync(kAll, v_sb[s / 2].bias, from);
-          }
+          const float vs = kQuantized ? __fmul_rn(v_sb[s][r].x, v_unit) : 1.f;
+          const float vb = kQuantized ? __fmaf_rn(kMiddle, v_sb[s][r].x, v_sb[s][r].y) : 0.f;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             float e[2];
@@ -652,18 +670,38 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
             for (int x = 0; x < 2; ++x) {
               e[x] = exp2_of(sc[n][s][2 * r + x] - base[n][x]);
               l[n][x] += e[x];
-              if constexpr (BITS != 16) {
+              if constexpr (kQuantized) {
                 bias_sum[n][x] = __fmaf_rn(e[x], vb, bias_sum[n][x]);
                 e[x] = __fmul_rn(e[x], vs);
               }
             }
-            wt[n][s][r] = transposed(pack<kMmaBf16>(e[0], e[1]));
+            const uint32_t w = pack<kMmaBf16>(e[0], e[1]);
+            if constexpr (kQuantized) {
+              const float2 rounded = halves(w);
+              w_sum[n][0] += rounded.x;
+              w_sum[n][1] += rounded.y;
+            }
+            wt[n][s][r] = transposed(w);
           }
         }
       }
 
       // -- the weighted sum
-      auto weigh = [&](const uint32_t (&buf)[S::BUF], int part) {
+      auto weigh = [&](uint32_t (&buf)[S::BUF], int part) {
+        if (partial) {
+#pragma unroll
+          for (int s = 0; s < SUB; ++s) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const bool there = kQuantized || seen(16 * s + 2 * c + (r & 1) + 8 * (r >> 1));  // (codes are finite)
+#pragma unroll
+              for (int j = 0; j < S::VC * S::VW; ++j) {
+                uint32_t& w = buf[(s * 4 + r) * S::VC * S::VW + j];
+                w = there ? w : 0;
+              }
+            }
+          }
+        }
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
 #pragma unroll
@@ -688,8 +726,8 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
                 for (int h = 0; h < 2; ++h) {
                   const uint32_t x = __byte_perm(r[0][j], r[1][j], h ? 0x7362 : 0x5140);
                   const uint32_t y = __byte_perm(r[2][j], r[3][j], h ? 0x7362 : 0x5140);
-                  const uint32_t a0 = codes8(x, 0x4140), a1 = codes8(x, 0x4342);
-                  const uint32_t a2 = codes8(y, 0x4140), a3 = codes8(y, 0x4342);
+                  const uint32_t a0 = __byte_perm(x, 0, 0x4140), a1 = __byte_perm(x, 0, 0x4342);
+                  const uint32_t a2 = __byte_perm(y, 0, 0x4140), a3 = __byte_perm(y, 0, 0x4342);
 #pragma unroll
                   for (int n = 0; n < NT; ++n) {
                     mma<false>(o[n][t0 + 2 * j + h], a0, a1, a2, a3, wt[n][s][0], wt[n][s][1]);
@@ -698,9 +736,10 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
               } else {
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {  // codes 2h and 2h + 1 of the word
-                  const uint32_t x = __byte_perm(r[0][j], r[1][j], h < 2 ? 0x5410 : 0x7632) >> (8 * (h & 1));
-                  const uint32_t y = __byte_perm(r[2][j], r[3][j], h < 2 ? 0x5410 : 0x7632) >> (8 * (h & 1));
-                  const uint32_t a0 = codes4_low(x), a1 = codes4_high(x), a2 = codes4_low(y), a3 = codes4_high(y);
+                  const uint32_t x = __byte_perm(r[0][j], r[1][j], h < 2 ? 0x5410 : 0x7632);
+                  const uint32_t y = __byte_perm(r[2][j], r[3][j], h < 2 ? 0x5410 : 0x7632);
+                  const uint32_t a0 = nibbles(x, 2 * (h & 1)), a1 = nibbles(x, 2 * (h & 1) + 1);
+                  const uint32_t a2 = nibbles(y, 2 * (h & 1)), a3 = nibbles(y, 2 * (h & 1) + 1);
 #pragma unroll
                   for (int n = 0; n < NT; ++n) {
                     mma<false>(o[n][t0 + 4 * j + h], a0, a1, a2, a3, wt[n][s][0], wt[n][s][1]);
@@ -713,70 +752,78 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
       };
       if constexpr (PARTS == 2) {
         weigh(bufs[0], 0);
-        load_k(bufs[0], next, 0);
+        if (i + 1 < tiles) {
+          load_k(bufs[0], next, 0);
+        }
         weigh(bufs[1], 1);
-        load_k(bufs[1], next, 1);
+        if (i + 1 < tiles) {
+          load_k(bufs[1], next, 1);
+        }
       } else {
         weigh(bufs[1], 0);
-        load_v(bufs[1], next, 0);
+        if (i + 1 < tiles) {
+          load_v(bufs[1], next, 0);
+        }
       }
-#pragma unroll
-      for (int s = 0; s < S::SLOTS; ++s) {
-        now[s] = next[s];
-        next[s] = checked(i + 2, s, pages[s]);
-        pages[s] = read_page(i + 3, s);
-      }
+      now = next;
+      ok_now = ok_next;
+      next = offset_of(i + 2, page_next, ok_next);
+      page_next = read_page(i + 3);
     }
 
     // -- the warps' results together
-    const float unit = BITS == 16 ? 1.f : __uint_as_float((uint32_t)exponent << 23);
     __syncthreads();  // (the item before has been read)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const int h = 8 * n + 2 * c + x;
-        float sum_l = l[n][x], sum_b = bias_sum[n][x];
+        const int h = head_warp * S::kWarpHeads + 8 * n + 2 * c + x;
+        const float unit = kQuantized ? __uint_as_float((uint32_t)exponent << 23) : 1.f;
+        float sum_l = l[n][x], sum_b = 0.f;
+        if constexpr (kQuantized) {
+          sum_b = __fmaf_rn(__fmul_rn(w_sum[n][x], unit), -kMiddle, bias_sum[n][x]);
+        }
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) {
           sum_l += __shfl_xor_sync(kAll, sum_l, d);
-          if constexpr (BITS != 16) {
+          if constexpr (kQuantized) {
             sum_b += __shfl_xor_sync(kAll, sum_b, d);
           }
         }
         if (g == 0) {
-          sm_m[warp][h] = m[n][x];
-          sm_l[warp][h] = sum_l;
+          sm_m[row_warp][h] = m[n][x];
+          sm_l[row_warp][h] = sum_l;
         }
         constexpr int kPer = S::VW * S::kPerWord;  // columns of a lane's V chunk
 #pragma unroll
         for (int t = 0; t < S::MT; ++t) {
           const int ch = t / (kPer / 2), j = t % (kPer / 2);
           float2 v = make_float2(o[n][t][x], o[n][t][2 + x]);
-          if constexpr (BITS != 16) {
-            v.x = __fmaf_rn(v.x, unit, sum_b);
-            v.y = __fmaf_rn(v.y, unit, sum_b);
+          if constexpr (kQuantized) {
+            v.x = __fmaf_rn(__fmul_rn(v.x, 1.f / kCode), unit, sum_b);
+            v.y = __fmaf_rn(__fmul_rn(v.y, 1.f / kCode), unit, sum_b);
           }
-          *reinterpret_cast<float2*>(&sm_o[warp][h][(8 * ch + g) * kPer + 2 * j]) = v;
+          *reinterpret_cast<float2*>(&sm_o[row_warp][h][(8 * ch + g) * kPer + 2 * j]) = v;
         }
       }
     }
     __syncthreads();
     const bool whole = u0 == 0 && u1 == units;
+    const bool none = span.end == span.first;
     float* const part = whole ? nullptr : p.parts + (2 * (int64_t)blockIdx.x + (u0 == 0)) * S::kPartFloats;
     for (int at = tid; at < heads * (S::DP / 4); at += kThreads) {
       const int h = at / (S::DP / 4), column = at % (S::DP / 4) * 4;
       float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
+      for (int w = 0; w < S::kRowWarps; ++w) {
         top = fmaxf(top, sm_m[w][h]);
       }
-      const float base = top == -INFINITY ? 0.f : top;
+      const float from = top == -INFINITY ? 0.f : top;
       float sum_l = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float f = exp2_of(sm_m[w][h] - base);
+      for (int w = 0; w < S::kRowWarps; ++w) {
+        const float f = exp2_of(sm_m[w][h] - from);
         const float4 x = *reinterpret_cast<const float4*>(&sm_o[w][h][column]);
         sum_l = __fmaf_rn(f, sm_l[w][h], sum_l);
         v.x = __fmaf_rn(f, x.x, v.x);
@@ -785,7 +832,7 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
         v.w = __fmaf_rn(f, x.w, v.w);
       }
       if (whole) {
-        const float inv = span.end > span.first ? __fdiv_rn(1.f, sum_l) : 0.f;  // no row at all: zeros
+        const float inv = none ? 0.f : __fdiv_rn(1.f, sum_l);  // no row at all: zeros
         const int64_t row = (int64_t)request * p.kv_heads * p.group + q_head0 + h;
         if (column < p.dim) {
           const uint2 r = make_uint2(pack<BF16>(__fmul_rn(v.x, inv), __fmul_rn(v.y, inv)),
@@ -793,7 +840,7 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
           *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + (row * p.dim + column) * 2) = r;
         }
         if (column == 0 && p.lse) {
-          p.lse[row] = span.end > span.first ? __fmaf_rn(base, kLn2, logf(__fmul_rn(sum_l, kUnshift))) : -INFINITY;
+          p.lse[row] = none ? -INFINITY : __fmaf_rn(from, kLn2, logf(__fmul_rn(sum_l, kUnshift)));
         }
       } else {
         *reinterpret_cast<float4*>(part + 2 * S::kHeads + h * S::DP + column) = v;
@@ -911,9 +958,9 @@ PagedAttentionPlan plan_of(int group, int64_t sms) {
   return r;
 }
 
-template <typename S, bool BF16, bool WIDE>
+template <typename S, bool BF16, bool FAST>
 cudaError_t launch_of(const PagedAttentionPlan& plan, const PagedAttentionParams& p, bool split, cudaStream_t stream) {
-  paged_attention_kernel<S, BF16, WIDE><<<(unsigned)plan.workers, kThreads, 0, stream>>>(p);
+  paged_attention_kernel<S, BF16, FAST><<<(unsigned)plan.workers, kThreads, 0, stream>>>(p);
   g_launch_count.fetch_add(1, std::memory_order_relaxed);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || !split) {

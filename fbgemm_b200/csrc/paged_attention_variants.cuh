@@ -1,6 +1,7 @@
 // The variants of paged_attention.cuh by row width and query heads per cached head: rows of up to 64, 128 and 256
-// columns, tiles of 8 heads, and of 16 where the output of 16 fits the registers (up to 128 columns; 256 columns take
-// further heads as another item, which reads the rows again, mostly from L2).
+// columns; 8 heads in a warp, 16 where the output of 16 fits the registers (up to 128 columns), and twice as many in two
+// warps that read the same rows at about the same time, the second from the caches.  More heads than that are an item of
+// their own, which reads the rows again.
 #pragma once
 
 #include "paged_attention.cuh"
@@ -11,12 +12,12 @@ namespace paged {
 template <int BITS, typename F>
 auto with_shape(int dim, int group, F&& f) {
   if (dim > 128) {
-    return f(Shape<BITS, 256, 1>());
+    return group > 8 ? f(Shape<BITS, 256, 1, 2>()) : f(Shape<BITS, 256, 1, 1>());
   }
   if (dim > 64) {
-    return group > 8 ? f(Shape<BITS, 128, 2>()) : f(Shape<BITS, 128, 1>());
+    return group > 16 ? f(Shape<BITS, 128, 2, 2>()) : group > 8 ? f(Shape<BITS, 128, 2, 1>()) : f(Shape<BITS, 128, 1, 1>());
   }
-  return group > 8 ? f(Shape<BITS, 64, 2>()) : f(Shape<BITS, 64, 1>());
+  return group > 16 ? f(Shape<BITS, 64, 2, 2>()) : group > 8 ? f(Shape<BITS, 64, 2, 1>()) : f(Shape<BITS, 64, 1, 1>());
 }
 
 }  // namespace paged
@@ -42,7 +43,8 @@ cudaError_t paged_attention_4(const PagedAttentionShape&, int64_t, PagedAttentio
         *plan = paged::plan_of<S>(s.group, sms);                                                                             \
         return cudaSuccess;                                                                                                  \
       }                                                                                                                      \
-      return paged::launch_of<S, IS_BF16, true>(*plan, *p, split, stream);                                                   \
+      return s.fast ? paged::launch_of<S, IS_BF16, true>(*plan, *p, split, stream)                                           \
+                    : paged::launch_of<S, IS_BF16, false>(*plan, *p, split, stream);                                         \
     });                                                                                                                      \
   }
 
@@ -55,7 +57,7 @@ cudaError_t paged_attention_4(const PagedAttentionShape&, int64_t, PagedAttentio
         *plan = paged::plan_of<S>(s.group, sms);                                                                             \
         return cudaSuccess;                                                                                                  \
       }                                                                                                                      \
-      return s.wide ? (s.bf16 ? paged::launch_of<S, true, true>(*plan, *p, split, stream)                                    \
+      return s.fast ? (s.bf16 ? paged::launch_of<S, true, true>(*plan, *p, split, stream)                                    \
                               : paged::launch_of<S, false, true>(*plan, *p, split, stream))                                  \
                     : (s.bf16 ? paged::launch_of<S, true, false>(*plan, *p, split, stream)                                   \
                               : paged::launch_of<S, false, false>(*plan, *p, split, stream));                                \

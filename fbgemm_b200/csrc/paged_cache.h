@@ -35,8 +35,12 @@ FBGEMM_B200_HD RowSpan span_of(int32_t length, int32_t window, int64_t most) {
   return RowSpan{(int32_t)first, (int32_t)end};
 }
 
+// Units are counted from a multiple of 16 rows, so that 16 rows of a step lie in one page of 16 or more.
+FBGEMM_B200_HD int32_t aligned_first(RowSpan s) {
+  return s.first & ~15;
+}
 FBGEMM_B200_HD int32_t units_of(RowSpan s, int32_t unit) {
-  const int32_t n = (int32_t)(((int64_t)s.end - s.first + unit - 1) / unit);
+  const int32_t n = (int32_t)(((int64_t)s.end - aligned_first(s) + unit - 1) / unit);
   return n > 0 ? n : 1;
 }
 
@@ -109,7 +113,7 @@ struct PagedAttentionShape {
   bool bf16;          // of q, the output and 16-bit rows
   int32_t dim;
   int32_t group;      // query heads per cached head
-  bool wide;          // rows 16-byte aligned
+  bool fast;          // rows 16-byte aligned, 16 or more to a page
 };
 struct PagedAttentionPlan {
   int32_t unit;        // rows per unit

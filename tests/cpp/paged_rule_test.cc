@@ -29,6 +29,8 @@ int main() {
   // units
   CHECK(units_of(span_of(0, 0, 9), 64) == 1 && units_of(span_of(1, 0, 9), 64) == 1);
   CHECK(units_of(span_of(64, 0, 999), 64) == 1 && units_of(span_of(65, 0, 999), 64) == 2);
+  CHECK(aligned_first(span_of(100, 71, 999)) == 16 && units_of(span_of(100, 71, 999), 64) == 2);
+  CHECK(units_of(span_of(80, 64, 999), 64) == 1 && units_of(span_of(79, 64, 999), 64) == 2);
   CHECK(units_of(span_of(2147483647, 0, 2147483647), 64) == 33554432);
   CHECK(units_per_worker(0, 444) == 1 && units_per_worker(444, 444) == 1 && units_per_worker(445, 444) == 2);
 
