@@ -92,13 +92,17 @@ bool good_rows(const void* p, int64_t token, int64_t head) {
   return p && aligned(p, 16) && token % 8 == 0 && head % 8 == 0;
 }
 
+bool rows_aligned(const fbgemm_b200_paged_cache& c) {
+  return aligned(c.k, 16) && aligned(c.v, 16) && (c.page_stride | c.slot_stride | c.head_stride) % 16 == 0;
+}
+
 PagedAttentionShape shape_of(const fbgemm_b200_paged_cache& c, int32_t q_heads, int32_t dtype) {
   PagedAttentionShape s;
   s.bits = bits_of(c);
   s.bf16 = dtype == FBGEMM_B200_OUT_BF16;
   s.dim = c.head_dim;
   s.group = q_heads / c.kv_heads;
-  s.fast = c.page_size >= 16 && aligned(c.k, 16) && aligned(c.v, 16) && (c.page_stride | c.slot_stride | c.head_stride) % 16 == 0;
+  s.fast = c.page_size >= 16 && rows_aligned(c) && c.slot_stride < (1 << 27);
   return s;
 }
 
@@ -376,6 +380,7 @@ int fbgemm_b200_paged_attention(
   p.dim = cache->head_dim;
   p.window = window;
   p.workers = plan.workers;
+  p.aligned = rows_aligned(*cache);
   const cudaError_t e = launch_paged_attention(shape, plan, p, split, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? 0 : fail_cuda(e, "paged_attention launch");
 } catch (...) {

@@ -8,25 +8,28 @@
 // and head.  That is too much for the fp32 units (8 heads on 4-bit rows: 200 TFLOP/s at the memory's rate) and far too
 // little for 128-row tiles of the large tensor instructions, whose M the few heads would fill to a sixteenth.  So the
 // rows are M and the heads N of m16n8k16: S^T = K Q^T takes 16 rows and 8 heads, O^T = V^T P^T 16 columns and 8 heads,
-// nothing is padded at 8 heads.  The order of a contraction's terms is free, so each lane loads 16 bytes of its rows
-// straight from memory into the registers it feeds the products from; nothing goes through shared memory.  V's pairs of
-// rows are interleaved in registers; P^T is turned to the second product's layout by movmatrix.
+// nothing is padded at 8 heads.  P^T is turned to the second product's layout by movmatrix.
 //
-// What is left to count is instructions.  Pages of 16 rows and more hold all 16 rows of a step, which then share one
-// address (FAST); smaller pages and unaligned rows exchange an address per row.  Every row is loaded, also those that the
-// token does not see (of the same page, or of page 0 in place of one that does not exist): they are masked in the
-// tiles that have some.  Codes become fp16 by being put into its lowest 8 bits: subnormal numbers, c 2^-24 (4-bit codes in the
-// upper half of them, c 2^-20), which the products take exactly; the power of two is made up for once per score and
-// result.  (The products align a subnormal as if its first bit were set: 4-bit codes in the lowest 4 bits cost 6 bits of
-// the sums, and results that were off by 1e-3.)  A tile's largest score is looked for across lanes only if one exceeds
-// the running maximum by more than 2^kSlack.
+// At 44 GB/s per SM and a microsecond of latency about 44 KB have to be on their way to every SM all the time.  Each
+// warp has a ring of half tiles (16 or 32 rows of K, or of V) in shared memory that it fills by asynchronous copies of
+// its own, several ahead of the one it works on: 165 KB per SM at 128 columns.  (With the rows on their way to registers a
+// warp had two half tiles in flight at most: 97 us for 64 requests of up to 8192 16-bit rows, 92 for 128 of up to 4096 4-bit
+// rows.)  Rows lie an odd multiple of 16 bytes apart there, so that ldmatrix reads K without
+// conflicts, and turns V, for 16-bit values and for pairs of 8-bit and fours of 4-bit codes alike: a register holds the
+// same columns of two rows, and their codes become two fp16 numbers by a mask or a byte permutation that puts them into
+// the lowest bits: subnormal numbers, c 2^-24 (4-bit codes in the upper half of a byte, c 2^-20), which the products take
+// exactly.  The power of two is made up for once per score and result.  (The products align a subnormal as if its first
+// bit were set: 4-bit codes in the lowest 4 bits cost 6 bits of the sums, and results that were off by 1e-3.)
 //
-// One pass with a running maximum and sum per head in fp32 (in registers, per warp).  A warp's next K tile is on its
-// way while it works on V, and the next V while it works on K.  Weights are rounded to 16 bits for the second product:
-// bf16 beside bf16 rows; fp16 (2^kShift times as large, so that weights down to 2^-24 of the largest keep all 11 bits)
-// otherwise, with the quantized rows' scales taken relative to the largest power of two seen so far.  A weight's
-// rounding is at most half a step of the output's own type, and averages out over the rows; codes are weighed about the
-// middle of their range (sum w (c - 128) = sum w c - 128 sum w, with the rounded w), which keeps it there.
+// Pages of 16 rows and more hold all 16 rows of a step, which then share one address (FAST); smaller pages and unaligned
+// rows have an address each.  Rows that the token does not see arrive as zeros, and a tile that has some is masked.
+//
+// One pass with a running maximum and sum per head in fp32 (in registers, per warp).  A tile's largest score is looked
+// for across lanes only if one exceeds the running maximum by more than 2^kSlack.  Weights are rounded to 16 bits for
+// the second product: bf16 beside bf16 rows; fp16 (2^kShift times as large, so that weights down to 2^-24 of the largest
+// keep all 11 bits) otherwise, with the quantized rows' scales taken relative to the largest power of two seen so far.
+// A weight's rounding is at most half a step of the output's own type, and averages out over the rows; codes are weighed
+// about the middle of their range (sum w (c - 128) = sum w c - 128 sum w, with the rounded w), which keeps it there.
 //
 // Work is split over the chip by paged_cache.h's rule.  A worker is a block of 4 warps that take the tiles of its units
 // in turn and join their results in shared memory; an item that several workers share is left as partial results, and a
@@ -92,29 +95,26 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
   return r;
 }
 
-// N words of a row, if `ok`, else r stays as it is.  WIDE: the address is a multiple of 4 N.  ONCE: nobody else reads them.
-template <int N, bool WIDE, bool ONCE>
-__device__ __forceinline__ void load_words(uint32_t* r, const uint8_t* p, bool ok) {
-  if constexpr (WIDE && N == 4 && ONCE) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.s32 p, %5, 0;\n@p ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n}"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3])
-                 : "l"(p), "r"((int)ok));
-  } else if constexpr (WIDE && N == 4) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.s32 p, %5, 0;\n@p ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];\n}"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3])
-                 : "l"(p), "r"((int)ok));
-  } else if constexpr (WIDE && N == 2) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.s32 p, %3, 0;\n@p ld.global.nc.v2.u32 {%0,%1}, [%2];\n}"
-                 : "+r"(r[0]), "+r"(r[1])
-                 : "l"(p), "r"((int)ok));
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      asm volatile("{\n.reg .pred p;\nsetp.ne.s32 p, %2, 0;\n@p ld.global.nc.u32 %0, [%1];\n}"
-                   : "+r"(r[i])
-                   : "l"(p + 4 * i), "r"((int)ok));
-    }
-  }
+// Four 8 x 8 matrices of 16-bit values; lane 8 i + j has the address of row j of matrix i.
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void load_turned(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+
+// 16 or 4 bytes to shared memory, past the first cache where that is possible; `bytes` 0: zeros instead.
+__device__ __forceinline__ void copy16(uint32_t to, const uint8_t* from, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const uint8_t* from, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 
 // Nibbles i and i + 4 of a word as subnormal fp16.
@@ -133,29 +133,30 @@ __device__ __forceinline__ float2 halves(uint32_t w) {
 template <int BITS_, int DP_, int NT_, int HW_>
 struct Shape {
   static constexpr int BITS = BITS_, DP = DP_, NT = NT_, HW = HW_;
-  static constexpr int kRowWords = DP * BITS / 32;                  // of a row's columns
-  static constexpr int kTileWords = kRowWords / 2;                  // a lane's share of 16 rows
-  static constexpr int PARTS = kTileWords > 32 ? 2 : 1;             // columns a tile is loaded in
-  static constexpr int SUB = kTileWords >= 32 ? 1 : 2;              // 16-row steps of a tile
+  static constexpr int kTail = BITS == 8 ? 8 : BITS == 4 ? 4 : 0;   // bytes of a row's scale and bias
+  static constexpr int kPieces = (DP * BITS / 8 + kTail + 15) / 16; // 16-byte pieces of a row
+  static constexpr int PITCH = (kPieces | 1) * 16;                  // between rows in shared memory
+  static constexpr int kBlocks16 = DP * BITS / 128;                 // 16-byte blocks of a row's columns
+  static constexpr int SUB = PITCH > 144 ? 1 : 2;                   // 16-row steps of a tile
   static constexpr int ROWS = 16 * SUB;                             // of a warp's tile
+  static constexpr int SLOT = ROWS * PITCH;                         // bytes of a half tile
   static constexpr int kRowWarps = kWarps / HW;
   static constexpr int UNIT = kRowWarps * ROWS;
-  static constexpr int KW = kRowWords / 4 < 4 ? kRowWords / 4 : 4;  // words of a K chunk: a lane of four has every 4th
-  static constexpr int KC = kRowWords / 4 / KW / PARTS;             // K chunks of a lane and part
-  static constexpr int VW = kRowWords / 8 < 4 ? kRowWords / 8 : 4;  // the same for V: a lane of eight
-  static constexpr int VC = kRowWords / 8 / VW / PARTS;
-  static constexpr int BUF = SUB * 2 * KC * KW;                     // = SUB * 4 * VC * VW
   static constexpr int KSTEPS = DP / 16;
   static constexpr int MT = DP / 16;                                // 16-column tiles of the output
-  static constexpr int kPerWord = 32 / BITS;
-  static_assert(BUF == SUB * 4 * VC * VW && BUF <= 32, "a buffer holds either");
   static constexpr int kWarpHeads = 8 * NT;
   static constexpr int kHeads = kWarpHeads * HW;
   static constexpr int kPartFloats = kHeads * (DP + 2);
-  static constexpr int kTail = BITS == 8 ? 2 : 1;                   // words of a row's scale and bias
-  // Registers: rows on their way (2 BUF), output (4 NT MT), queries (2 NT KSTEPS), and about 60 more.
-  static constexpr int kRegisters = 2 * BUF + 4 * NT * MT + 2 * NT * KSTEPS;
-  static constexpr int kBlocks = kRegisters <= 64 ? 4 : kRegisters <= 112 ? 3 : 2;
+  // Blocks of an SM by registers (output 4 NT MT, queries 2 NT KSTEPS, scores, and about 70 more), and ring slots of a warp
+  // by shared memory.
+  static constexpr int kRegisters = 4 * NT * MT + 2 * NT * KSTEPS + 4 * NT * SUB;
+  static constexpr int kBlocks = kRegisters <= 90 ? 3 : 2;
+  static constexpr int kFit = 224 * 1024 / (kBlocks * kWarps * SLOT);
+  static constexpr int SLOTS = kFit > 6 ? 6 : kFit;
+  static constexpr int HP = DP + 4;                                 // floats between heads in the join of the warps
+  static constexpr int kRing = kWarps * SLOTS * SLOT, kJoin = kRowWarps * kHeads * HP * 4;
+  static constexpr int kShared = kRing > kJoin ? kRing : kJoin;
+  static_assert(SLOTS >= 3, "two half tiles on their way");
 };
 
 // ---- the kernel -------------------------------------------------------------------------------------------------------
@@ -163,17 +164,19 @@ struct Shape {
 // FAST: pages of 16 rows or more, rows 16-byte aligned.
 template <typename S, bool BF16, bool FAST>
 __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(const PagedAttentionParams p) {
-  constexpr int BITS = S::BITS, NT = S::NT, SUB = S::SUB, PARTS = S::PARTS;
+  constexpr int BITS = S::BITS, NT = S::NT, SUB = S::SUB;
   constexpr bool kQuantized = BITS != 16;
   constexpr bool kMmaBf16 = !kQuantized && BF16;
-  constexpr bool kOnce = S::HW == 1;
   constexpr float kMiddle = BITS == 8 ? 128.f : 8.f;
   constexpr float kCode = BITS == 4 ? 1.f / 1048576.f : 1.f / 16777216.f;  // what a code of 1 is to the products
-  __shared__ float sm_o[S::kRowWarps][S::kHeads][S::DP];
+  constexpr unsigned kFull = S::ROWS == 32 ? kAll : (1u << (S::ROWS & 31)) - 1;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ unsigned sm_seen[kWarps][S::SLOTS];  // rows of a half tile that the token sees
   __shared__ float sm_m[S::kRowWarps][S::kHeads], sm_l[S::kRowWarps][S::kHeads];
   __shared__ int64_t sm_sums[kWarps];
   __shared__ int32_t sm_request;
   __shared__ int64_t sm_unit;
+  float* const sm_o = reinterpret_cast<float*>(smem);  // [row warp][head][HP], in place of the rings
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int row_warp = warp / S::HW, head_warp = warp % S::HW;
@@ -195,6 +198,15 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
   if (lane == 31) {
     sm_sums[warp] = before;
   }
+  // (columns that no row has stay 0 in the rings)
+  uint8_t* const ring = smem + warp * (S::SLOTS * S::SLOT);
+  auto clear_ring = [&] {
+    for (int at = lane * 16; at < S::SLOTS * S::SLOT; at += 512) {
+      *reinterpret_cast<uint4*>(ring + at) = make_uint4(0, 0, 0, 0);
+    }
+    __syncwarp();
+  };
+  const bool padded = !kQuantized && p.dim < S::DP;
   __syncthreads();
   before -= sum;
   int64_t total = 0;
@@ -228,18 +240,14 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
   int64_t unit_at = first_unit;
   int4 opened = make_int4(0, 0, 0, 0);
 
-  // Where a lane's rows and columns lie: K rows g and g + 8 of a step, V rows 2c, 2c + 1, 2c + 8 and 2c + 9.
-  const int64_t k_lane = (FAST ? g * p.slot_stride : 0) + c * (4 * S::KW);
-  const int64_t v_lane = (FAST ? 2 * c * p.slot_stride : 0) + g * (4 * S::VW);
-  const int64_t tail = p.dim * BITS / 8 - c * (4 * S::KW);  // from k_lane's column to scale and bias
-  auto k_column = [&](int part, int i) { return (4 * (part * S::KC + i) + c) * (S::KW * S::kPerWord) < p.dim; };
-  auto v_column = [&](int part, int i) { return (8 * (part * S::VC + i) + g) * (S::VW * S::kPerWord) < p.dim; };
-
-  uint32_t bufs[2][S::BUF];
-#pragma unroll
-  for (int j = 0; j < S::BUF; ++j) {
-    bufs[0][j] = bufs[1][j] = 0;  // columns that no row has stay 0
-  }
+  const int row_bytes = p.dim * BITS / 8 + S::kTail;
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  const uint32_t ring_end = ring_at + S::SLOTS * S::SLOT;
+  // ldmatrix: K's matrices are rows 0 - 7 and 8 - 15 of a block of columns, then of the next; V's two blocks of rows 0 - 7,
+  // then of 8 - 15.
+  const uint32_t k_lane = ((lane & 7) + (lane & 8)) * S::PITCH + (lane >> 4) * 16;
+  const uint32_t v_lane = ((lane & 7) + ((lane >> 4) << 3)) * S::PITCH + ((lane >> 3) & 1) * 16;
+  const uint32_t tail_lane = g * S::PITCH + p.dim * BITS / 8;
 
   // -- item after item: a request, a cached head and a tile of its query heads
   while (unit_at < last_unit) {
@@ -268,15 +276,14 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
     const int tiles = (int)min((int64_t)(u1 - u0), row0 < span.end ? (span.end - row0 + S::UNIT - 1) / S::UNIT : 0);
     // A lane looks after the address of a step's 16 rows (FAST), or of one row.
     constexpr int kLeaders = FAST ? SUB : S::ROWS;
-    constexpr unsigned kLed = kLeaders == 32 ? kAll : (1u << (kLeaders & 31)) - 1;
     auto row_of = [&](int i) { return row0 + (int64_t)i * S::UNIT + lane * (FAST ? 16 : 1); };
     auto led = [&](int i) {
       const int64_t row = row_of(i);
       return i < tiles && lane < kLeaders && row < span.end && (FAST || row >= span.first);
     };
     auto read_page = [&](int i) { return led(i) ? __ldg(table + (row_of(i) >> p.page_shift)) : 0; };
-    // Byte offset of the row; one that does not exist stands for row 0 of page 0 (and a step's for the first 16).
-    auto offset_of = [&](int i, int32_t page, unsigned& ok) -> int64_t {
+    // Byte offset of the row (0 in place of one that does not exist) and the rows of the tile that the token sees.
+    auto offset_of = [&](int i, int32_t page, unsigned& seen) -> int64_t {
       const bool exists = led(i);
       const bool good = exists && page >= 0 && page < p.num_pages;
       if (exists && !good && atomicCAS(p.status, 0, FBGEMM_B200_STATUS_BAD_PAGE) == 0) {
@@ -284,101 +291,125 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
         p.status[2] = (int32_t)row_of(i);
         p.status[3] = page;
       }
-      ok = __ballot_sync(kAll, good);
+      seen = __ballot_sync(kAll, good);
+      if constexpr (FAST) {
+        const int64_t row = row0 + (int64_t)i * S::UNIT;
+        seen = (seen & 1 ? 0xffffu : 0u) | (SUB == 2 && (seen & 2) ? 0xffff0000u : 0u);
+        if (row < span.first) {  // (by less than 16)
+          seen &= ~0u << (span.first - row);
+        }
+        if (row + S::ROWS > span.end) {
+          seen &= span.end > row ? kFull >> (row + S::ROWS - span.end) : 0u;
+        }
+      }
       return good ? page * p.page_stride + (row_of(i) & ((1 << p.page_shift) - 1)) * p.slot_stride : 0;
     };
 
-    uint32_t k_tail[SUB][2][S::kTail], v_tail[SUB][2][S::kTail];
-    auto load_k = [&](uint32_t (&buf)[S::BUF], int64_t off, int part) {
+    // A half tile's rows on their way to `to`.
+    auto copy_rows = [&](uint32_t to, const uint8_t* rows, int64_t off, unsigned seen) {
+      if (FAST || p.aligned) {
+        const int pieces = (row_bytes + 15) / 16;
 #pragma unroll
-      for (int s = 0; s < SUB; ++s) {
-        const uint8_t* step = FAST ? k_rows + __shfl_sync(kAll, off, s) + k_lane : nullptr;
+        for (int s = 0; s < SUB; ++s) {
+          const uint8_t* step = FAST ? rows + __shfl_sync(kAll, off, s) : rows;
+          constexpr int kRounds = (16 * S::kPieces + 31) / 32;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const uint8_t* row = FAST ? step + (r ? 8 * p.slot_stride : 0) : k_rows + __shfl_sync(kAll, off, 16 * s + 8 * r + g) + k_lane;
-#pragma unroll
-          for (int i = 0; i < S::KC; ++i) {
-            load_words<S::KW, FAST || !kQuantized, kOnce>(&buf[((s * 2 + r) * S::KC + i) * S::KW],
-                                                          row + (part * S::KC + i) * (16 * S::KW), k_column(part, i));
-          }
-          if constexpr (kQuantized) {
-            load_words<S::kTail, FAST, false>(k_tail[s][r], row + tail, true);
-          }
-        }
-      }
-    };
-    auto load_v = [&](uint32_t (&buf)[S::BUF], int64_t off, int part) {
-#pragma unroll
-      for (int s = 0; s < SUB; ++s) {
-        const int64_t first = FAST ? __shfl_sync(kAll, off, s) : 0;
-        const uint8_t* step = v_rows + first + v_lane;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint8_t* row = FAST ? step + (r == 0 ? 0 : r == 1 ? 1 : r == 2 ? 8 : 9) * p.slot_stride
-                                    : v_rows + __shfl_sync(kAll, off, 16 * s + 2 * c + (r & 1) + 8 * (r >> 1)) + v_lane;
-#pragma unroll
-          for (int i = 0; i < S::VC; ++i) {
-            load_words<S::VW, FAST || !kQuantized, kOnce>(&buf[((s * 4 + r) * S::VC + i) * S::VW],
-                                                          row + (part * S::VC + i) * (32 * S::VW), v_column(part, i));
+          for (int j = 0; j < kRounds; ++j) {
+            const int at = lane + 32 * j, row = at / S::kPieces, piece = at - row * S::kPieces;
+            const int64_t row_off = FAST ? (int64_t)(uint32_t)(row * (uint32_t)p.slot_stride) : __shfl_sync(kAll, off, 16 * s + min(row, 15));
+            if (piece < pieces && (16 * S::kPieces % 32 == 0 || row < 16)) {
+              copy16(to + (16 * s + row) * S::PITCH + piece * 16, step + row_off + piece * 16,
+                     (seen >> (16 * s + row)) & 1 ? 16 : 0);
+            }
           }
         }
-        if constexpr (kQuantized) {
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const uint8_t* row = FAST ? v_rows + first + k_lane + (r ? 8 * p.slot_stride : 0)
-                                      : v_rows + __shfl_sync(kAll, off, 16 * s + 8 * r + g) + k_lane;
-            load_words<S::kTail, FAST, false>(v_tail[s][r], row + tail, true);
-          }
+      } else if (lane < S::ROWS) {
+        const uint32_t bytes = (seen >> lane) & 1 ? 4 : 0;
+        for (int at = 0; at < row_bytes; at += 4) {
+          copy4(to + lane * S::PITCH + at, rows + off + at, bytes);
         }
       }
     };
 
-    // -- the first tiles' way, and the queries as the products take them: head g of a tile in lanes 4g .. 4g + 3, columns in
-    // the order of K's words
-    int32_t page_now = read_page(0), page_next = read_page(1);
+    // -- half tile h: K (even) or V (odd) of tile h / 2, into slot h % SLOTS; SLOTS - 1 are on their way
+    int64_t off = 0;
+    unsigned seen = 0;
+    int32_t page_next = read_page(0), page_after = read_page(1);
+    int fill_tile = -1;
+    uint32_t fill_at = ring_at;
+    int fill_slot = 0;
+    auto fill = [&](bool is_v) {
+      if (!is_v) {
+        ++fill_tile;
+        off = offset_of(fill_tile, page_next, seen);
+        page_next = page_after;
+        page_after = read_page(fill_tile + 2);
+      }
+      if (fill_tile < tiles) {
+        copy_rows(fill_at, is_v ? v_rows : k_rows, off, seen);
+        if (lane == 0) {
+          sm_seen[warp][fill_slot] = seen;
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      fill_at += S::SLOT;
+      ++fill_slot;
+      if (fill_at == ring_end) {
+        fill_at = ring_at;
+        fill_slot = 0;
+      }
+    };
+    auto arrived = [&] {
+      asm volatile("cp.async.wait_group %0;" ::"n"(S::SLOTS - 2) : "memory");
+      __syncwarp();
+    };
+    if (padded) {
+      clear_ring();
+    }
+
+    // -- queries as the products take them: head g of a tile in lanes 4g .. 4g + 3, columns in the order of K's registers.
+    // Columns of 16 bits: 2c, 2c + 1 and 2c + 8, 2c + 9 of a step of 16.  8-bit codes: 4c .. 4c + 3 of a step.  4-bit codes:
+    // 8c .. 8c + 7 of two steps.
     uint32_t qf[NT][S::KSTEPS][2];
-    float factor[NT][2], q_sum[NT][2];  // heads 2c and 2c + 1
-    constexpr int kQuads = S::kPerWord * S::KW / 8;  // 16-byte pieces of q per chunk
-    constexpr int kChunks = PARTS * S::KC;
-    uint32_t q_words[NT][kChunks][kQuads * 4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int head = head_warp * S::kWarpHeads + 8 * n + g;
       const bool there = head < heads;
       const uint8_t* q = p.q + request * p.q_token + (q_head0 + (there ? head : 0)) * p.q_head;
+      if constexpr (BITS == 4) {
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-#pragma unroll
-        for (int j = 0; j < kQuads; ++j) {
-          const int column = (4 * i + c) * (8 * kQuads) + 8 * j;
+        for (int k = 0; k < S::KSTEPS; k += 2) {
+          const int column = 16 * k + 8 * c;
           uint4 v = make_uint4(0, 0, 0, 0);
           if (there && column < p.dim) {
             v = *reinterpret_cast<const uint4*>(q + 2 * column);
           }
-          q_words[n][i][4 * j] = v.x;
-          q_words[n][i][4 * j + 1] = v.y;
-          q_words[n][i][4 * j + 2] = v.z;
-          q_words[n][i][4 * j + 3] = v.w;
+          qf[n][k][0] = v.x;
+          qf[n][k][1] = v.y;
+          qf[n][k + 1][0] = v.z;
+          qf[n][k + 1][1] = v.w;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < S::KSTEPS; ++k) {
+          const int column = 16 * k + (BITS == 16 ? 2 : 4) * c;
+          qf[n][k][0] = qf[n][k][1] = 0;
+          if (there && 16 * k < p.dim) {
+            qf[n][k][0] = *reinterpret_cast<const uint32_t*>(q + 2 * column);
+            qf[n][k][1] = *reinterpret_cast<const uint32_t*>(q + 2 * column + (BITS == 16 ? 16 : 4));
+          }
         }
       }
     }
-    unsigned ok_now = 0, ok_next = 0;
-    int64_t now = offset_of(0, page_now, ok_now);
-    if (tiles > 0) {
-      load_k(bufs[0], now, 0);
-      if constexpr (PARTS == 2) {
-        load_k(bufs[1], now, 1);
-      } else {
-        load_v(bufs[1], now, 0);
-      }
+#pragma unroll
+    for (int h = 0; h < S::SLOTS - 1; ++h) {
+      fill(h & 1);
     }
-    int64_t next = offset_of(1, page_next, ok_next);
-    page_next = read_page(2);
 
+    float factor[NT][2], q_sum[NT][2];  // heads 2c and 2c + 1
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float scale_head = 1.f, sum_head = 0.f;
-      uint32_t(&w)[kChunks][kQuads * 4] = q_words[n];
       if constexpr (kQuantized) {
         // Beside fp16 codes the queries are fp16 too; bf16 ones may lie outside its range, so each head is moved by a power
         // of two.
@@ -387,10 +418,10 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
         };
         float most = 0.f;
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
+        for (int k = 0; k < S::KSTEPS; ++k) {
 #pragma unroll
-          for (int j = 0; j < kQuads * 4; ++j) {
-            const float2 f = two(w[i][j]);
+          for (int j = 0; j < 2; ++j) {
+            const float2 f = two(qf[n][k][j]);
             most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
           }
         }
@@ -402,36 +433,26 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
         const float up = __uint_as_float((uint32_t)(127 + move) << 23);
         scale_head = __uint_as_float((uint32_t)(127 - move) << 23);
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
+        for (int k = 0; k < S::KSTEPS; ++k) {
 #pragma unroll
-          for (int j = 0; j < kQuads * 4; ++j) {
-            const float2 f = two(w[i][j]);
+          for (int j = 0; j < 2; ++j) {
+            const float2 f = two(qf[n][k][j]);
             const float x = __fmul_rn(f.x, up), y = __fmul_rn(f.y, up);
             sum_head += x + y;
-            w[i][j] = pack<false>(x, y);
+            qf[n][k][j] = pack<false>(x, y);
           }
         }
         sum_head += __shfl_xor_sync(kAll, sum_head, 1);
         sum_head += __shfl_xor_sync(kAll, sum_head, 2);
       }
+      if constexpr (BITS == 4) {
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        if constexpr (BITS == 4) {
-#pragma unroll
-          for (int j = 0; j < S::KW; ++j) {  // a word of codes: columns (0,4), (1,5) and (2,6), (3,7)
-            const uint32_t w0 = w[i][4 * j], w1 = w[i][4 * j + 1], w2 = w[i][4 * j + 2], w3 = w[i][4 * j + 3];
-            const int k = 2 * (i * S::KW + j);
-            qf[n][k][0] = __byte_perm(w0, w2, 0x5410);
-            qf[n][k][1] = __byte_perm(w0, w2, 0x7632);
-            qf[n][k + 1][0] = __byte_perm(w1, w3, 0x5410);
-            qf[n][k + 1][1] = __byte_perm(w1, w3, 0x7632);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < kQuads * 2; ++j) {
-            qf[n][i * kQuads * 2 + j][0] = w[i][2 * j];
-            qf[n][i * kQuads * 2 + j][1] = w[i][2 * j + 1];
-          }
+        for (int k = 0; k < S::KSTEPS; k += 2) {  // columns (0,4), (1,5) and (2,6), (3,7)
+          const uint32_t w0 = qf[n][k][0], w1 = qf[n][k][1], w2 = qf[n][k + 1][0], w3 = qf[n][k + 1][1];
+          qf[n][k][0] = __byte_perm(w0, w2, 0x5410);
+          qf[n][k][1] = __byte_perm(w0, w2, 0x7632);
+          qf[n][k + 1][0] = __byte_perm(w1, w3, 0x5410);
+          qf[n][k + 1][1] = __byte_perm(w1, w3, 0x7632);
         }
       }
 #pragma unroll
@@ -464,8 +485,33 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
     }
     int exponent = 1;  // 127 + the exponent that V's scales are taken relative to
 
+    uint32_t at = ring_at;
+    int slot = 0;
+    auto advance = [&] {
+      at += S::SLOT;
+      ++slot;
+      if (at == ring_end) {
+        at = ring_at;
+        slot = 0;
+      }
+    };
+    auto tail_of = [&](uint32_t half, int s, int r) {
+      const uint32_t from = half + tail_lane + (16 * s + 8 * r) * S::PITCH;
+      if constexpr (BITS == 8) {
+        float2 v;
+        asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(from) : "memory");
+        return v;
+      } else {
+        uint32_t w;
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(from) : "memory");
+        return halves(w);
+      }
+    };
+
     for (int i = 0; i < tiles; ++i) {
       // -- scores
+      arrived();
+      fill(S::SLOTS % 2 == 0);
       float sc[NT][SUB][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -474,118 +520,80 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
           sc[n][s][0] = sc[n][s][1] = sc[n][s][2] = sc[n][s][3] = 0.f;
         }
       }
-      auto score = [&](const uint32_t (&buf)[S::BUF], int part) {
 #pragma unroll
-        for (int s = 0; s < SUB; ++s) {
+      for (int s = 0; s < SUB; ++s) {
 #pragma unroll
-          for (int ch = 0; ch < S::KC; ++ch) {
-            const uint32_t* r0 = &buf[(s * 2 * S::KC + ch) * S::KW];
-            const uint32_t* r1 = &buf[((s * 2 + 1) * S::KC + ch) * S::KW];
-            const int k0 = (part * S::KC + ch) * S::KW * S::kPerWord / 4;  // products of this chunk: 4 columns of a lane each
-            if constexpr (BITS == 16) {
+        for (int b = 0; b < S::kBlocks16; b += 2) {
+          uint32_t r[4];
+          load_matrices(r, at + k_lane + 16 * s * S::PITCH + 16 * b);
+          if constexpr (BITS == 16) {
 #pragma unroll
-              for (int j = 0; j < S::KW / 2; ++j) {
+            for (int n = 0; n < NT; ++n) {
+              mma<kMmaBf16>(sc[n][s], r[0], r[1], r[2], r[3], qf[n][b / 2][0], qf[n][b / 2][1]);
+            }
+          } else {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                  mma<kMmaBf16>(sc[n][s], r0[2 * j], r1[2 * j], r0[2 * j + 1], r1[2 * j + 1], qf[n][k0 + j][0],
-                                qf[n][k0 + j][1]);
-                }
-              }
-            } else if constexpr (BITS == 8) {
-#pragma unroll
-              for (int j = 0; j < S::KW; ++j) {
-                const uint32_t a0 = __byte_perm(r0[j], 0, 0x4140), a2 = __byte_perm(r0[j], 0, 0x4342);
-                const uint32_t a1 = __byte_perm(r1[j], 0, 0x4140), a3 = __byte_perm(r1[j], 0, 0x4342);
+            for (int h = 0; h < 2; ++h) {  // r[2h]: block b + h of rows g, r[2h + 1]: of rows g + 8
+              if constexpr (BITS == 8) {
+                const uint32_t a0 = __byte_perm(r[2 * h], 0, 0x4140), a2 = __byte_perm(r[2 * h], 0, 0x4342);
+                const uint32_t a1 = __byte_perm(r[2 * h + 1], 0, 0x4140), a3 = __byte_perm(r[2 * h + 1], 0, 0x4342);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                  mma<false>(sc[n][s], a0, a1, a2, a3, qf[n][k0 + j][0], qf[n][k0 + j][1]);
+                  mma<false>(sc[n][s], a0, a1, a2, a3, qf[n][b + h][0], qf[n][b + h][1]);
                 }
-              }
-            } else {
+              } else {
 #pragma unroll
-              for (int j = 0; j < S::KW; ++j) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  const uint32_t a0 = nibbles(r0[j], 2 * h), a2 = nibbles(r0[j], 2 * h + 1);
-                  const uint32_t a1 = nibbles(r1[j], 2 * h), a3 = nibbles(r1[j], 2 * h + 1);
+                for (int j = 0; j < 2; ++j) {
+                  const uint32_t a0 = nibbles(r[2 * h], 2 * j), a2 = nibbles(r[2 * h], 2 * j + 1);
+                  const uint32_t a1 = nibbles(r[2 * h + 1], 2 * j), a3 = nibbles(r[2 * h + 1], 2 * j + 1);
 #pragma unroll
                   for (int n = 0; n < NT; ++n) {
-                    mma<false>(sc[n][s], a0, a1, a2, a3, qf[n][k0 + 2 * j + h][0], qf[n][k0 + 2 * j + h][1]);
+                    mma<false>(sc[n][s], a0, a1, a2, a3, qf[n][2 * (b + h) + j][0], qf[n][2 * (b + h) + j][1]);
                   }
                 }
               }
             }
           }
         }
-      };
-      score(bufs[0], 0);
-      float2 k_sb[SUB][2];
-      if constexpr (kQuantized) {
-#pragma unroll
-        for (int s = 0; s < SUB; ++s) {
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            if constexpr (BITS == 8) {
-              k_sb[s][r] = make_float2(__uint_as_float(k_tail[s][r][0]), __uint_as_float(k_tail[s][r][S::kTail - 1]));
-            } else {
-              k_sb[s][r] = halves(k_tail[s][r][0]);
-            }
-          }
-        }
       }
-      if constexpr (PARTS == 2) {
-        load_v(bufs[0], now, 0);
-        score(bufs[1], 1);
-        load_v(bufs[1], now, 1);
-      } else if (i + 1 < tiles) {
-        load_k(bufs[0], next, 0);
-      }
-
-      // -- rows that the token does not see
-      const int64_t row = row0 + (int64_t)i * S::UNIT;
-      const bool partial = row < span.first || row + S::ROWS > span.end || ok_now != kLed;
-      auto seen = [&](int at) {
-        return row + at >= span.first && row + at < span.end && ((ok_now >> (FAST ? at / 16 : at)) & 1);
-      };
 #pragma unroll
       for (int s = 0; s < SUB; ++s) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
+          const float2 sb = kQuantized ? tail_of(at, s, r) : make_float2(1.f, 0.f);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               float& v = sc[n][s][2 * r + x];
               if constexpr (kQuantized) {
-                v = __fmaf_rn(k_sb[s][r].x, v, __fmul_rn(k_sb[s][r].y, q_sum[n][x]));
+                v = __fmaf_rn(sb.x, v, __fmul_rn(sb.y, q_sum[n][x]));
               }
               v = __fmul_rn(v, factor[n][x]);
             }
           }
         }
       }
-      if (partial) {
+      const unsigned rows_seen = sm_seen[warp][slot];
+      if (rows_seen != kFull) {
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const bool there = seen(16 * s + 8 * r + g);
+            const bool there = (rows_seen >> (16 * s + 8 * r + g)) & 1;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               sc[n][s][2 * r] = there ? sc[n][s][2 * r] : -INFINITY;
               sc[n][s][2 * r + 1] = there ? sc[n][s][2 * r + 1] : -INFINITY;
             }
-            if constexpr (kQuantized) {
-#pragma unroll
-              for (int j = 0; j < S::kTail; ++j) {
-                v_tail[s][r][j] = there ? v_tail[s][r][j] : 0;
-              }
-            }
           }
         }
       }
+      advance();
 
       // -- weights
+      arrived();
+      fill(S::SLOTS % 2 != 0);
       bool more = false;
       float top[NT][2];
 #pragma unroll
@@ -607,11 +615,7 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
         for (int s = 0; s < SUB; ++s) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            if constexpr (BITS == 8) {
-              v_sb[s][r] = make_float2(__uint_as_float(v_tail[s][r][0]), __uint_as_float(v_tail[s][r][S::kTail - 1]));
-            } else {
-              v_sb[s][r] = halves(v_tail[s][r][0]);
-            }
+            v_sb[s][r] = tail_of(at, s, r);
             largest = max(largest, (__float_as_uint(v_sb[s][r].x) >> 23) & 0xff);
           }
         }
@@ -687,92 +691,48 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
       }
 
       // -- the weighted sum
-      auto weigh = [&](uint32_t (&buf)[S::BUF], int part) {
-        if (partial) {
 #pragma unroll
-          for (int s = 0; s < SUB; ++s) {
+      for (int s = 0; s < SUB; ++s) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const bool there = kQuantized || seen(16 * s + 2 * c + (r & 1) + 8 * (r >> 1));  // (codes are finite)
+        for (int b = 0; b < S::kBlocks16; b += 2) {
+          uint32_t r[4];
+          load_turned(r, at + v_lane + 16 * s * S::PITCH + 16 * b);
+          if constexpr (BITS == 16) {
 #pragma unroll
-              for (int j = 0; j < S::VC * S::VW; ++j) {
-                uint32_t& w = buf[(s * 4 + r) * S::VC * S::VW + j];
-                w = there ? w : 0;
-              }
+            for (int n = 0; n < NT; ++n) {
+              mma<kMmaBf16>(o[n][b / 2], r[0], r[1], r[2], r[3], wt[n][s][0], wt[n][s][1]);
             }
-          }
-        }
+          } else {
 #pragma unroll
-        for (int s = 0; s < SUB; ++s) {
-#pragma unroll
-          for (int ch = 0; ch < S::VC; ++ch) {
-            const uint32_t* r[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              r[j] = &buf[((s * 4 + j) * S::VC + ch) * S::VW];
-            }
-            const int t0 = (part * S::VC + ch) * S::VW * S::kPerWord / 2;  // 16-column tiles: 2 columns of a lane each
-#pragma unroll
-            for (int j = 0; j < S::VW; ++j) {
-              if constexpr (BITS == 16) {
-                const uint32_t a0 = __byte_perm(r[0][j], r[1][j], 0x5410), a1 = __byte_perm(r[0][j], r[1][j], 0x7632);
-                const uint32_t a2 = __byte_perm(r[2][j], r[3][j], 0x5410), a3 = __byte_perm(r[2][j], r[3][j], 0x7632);
+            for (int h = 0; h < 2; ++h) {  // r[h]: block b + h of rows 2c, 2c + 1, r[2 + h]: of rows 2c + 8, 2c + 9
+              if constexpr (BITS == 8) {
+                const uint32_t a0 = r[h] & 0x00ff00ffu, a1 = __byte_perm(r[h], 0, 0x4341);
+                const uint32_t a2 = r[2 + h] & 0x00ff00ffu, a3 = __byte_perm(r[2 + h], 0, 0x4341);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                  mma<kMmaBf16>(o[n][t0 + j], a0, a1, a2, a3, wt[n][s][0], wt[n][s][1]);
-                }
-              } else if constexpr (BITS == 8) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  const uint32_t x = __byte_perm(r[0][j], r[1][j], h ? 0x7362 : 0x5140);
-                  const uint32_t y = __byte_perm(r[2][j], r[3][j], h ? 0x7362 : 0x5140);
-                  const uint32_t a0 = __byte_perm(x, 0, 0x4140), a1 = __byte_perm(x, 0, 0x4342);
-                  const uint32_t a2 = __byte_perm(y, 0, 0x4140), a3 = __byte_perm(y, 0, 0x4342);
-#pragma unroll
-                  for (int n = 0; n < NT; ++n) {
-                    mma<false>(o[n][t0 + 2 * j + h], a0, a1, a2, a3, wt[n][s][0], wt[n][s][1]);
-                  }
+                  mma<false>(o[n][b + h], a0, a1, a2, a3, wt[n][s][0], wt[n][s][1]);
                 }
               } else {
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {  // codes 2h and 2h + 1 of the word
-                  const uint32_t x = __byte_perm(r[0][j], r[1][j], h < 2 ? 0x5410 : 0x7632);
-                  const uint32_t y = __byte_perm(r[2][j], r[3][j], h < 2 ? 0x5410 : 0x7632);
-                  const uint32_t a0 = nibbles(x, 2 * (h & 1)), a1 = nibbles(x, 2 * (h & 1) + 1);
-                  const uint32_t a2 = nibbles(y, 2 * (h & 1)), a3 = nibbles(y, 2 * (h & 1) + 1);
+                for (int j = 0; j < 2; ++j) {
+                  const uint32_t a0 = nibbles(r[h], 2 * j), a1 = nibbles(r[h], 2 * j + 1);
+                  const uint32_t a2 = nibbles(r[2 + h], 2 * j), a3 = nibbles(r[2 + h], 2 * j + 1);
 #pragma unroll
                   for (int n = 0; n < NT; ++n) {
-                    mma<false>(o[n][t0 + 4 * j + h], a0, a1, a2, a3, wt[n][s][0], wt[n][s][1]);
+                    mma<false>(o[n][2 * (b + h) + j], a0, a1, a2, a3, wt[n][s][0], wt[n][s][1]);
                   }
                 }
               }
             }
           }
         }
-      };
-      if constexpr (PARTS == 2) {
-        weigh(bufs[0], 0);
-        if (i + 1 < tiles) {
-          load_k(bufs[0], next, 0);
-        }
-        weigh(bufs[1], 1);
-        if (i + 1 < tiles) {
-          load_k(bufs[1], next, 1);
-        }
-      } else {
-        weigh(bufs[1], 0);
-        if (i + 1 < tiles) {
-          load_v(bufs[1], next, 0);
-        }
       }
-      now = next;
-      ok_now = ok_next;
-      next = offset_of(i + 2, page_next, ok_next);
-      page_next = read_page(i + 3);
+      advance();
     }
 
-    // -- the warps' results together
-    __syncthreads();  // (the item before has been read)
+    // -- the warps' results together, where the rings were
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -794,16 +754,18 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
           sm_m[row_warp][h] = m[n][x];
           sm_l[row_warp][h] = sum_l;
         }
-        constexpr int kPer = S::VW * S::kPerWord;  // columns of a lane's V chunk
+        float* const to = sm_o + (row_warp * S::kHeads + h) * S::HP;
 #pragma unroll
         for (int t = 0; t < S::MT; ++t) {
-          const int ch = t / (kPer / 2), j = t % (kPer / 2);
           float2 v = make_float2(o[n][t][x], o[n][t][2 + x]);
-          if constexpr (kQuantized) {
+          if constexpr (BITS == 16) {
+            to[16 * t + g] = v.x;
+            to[16 * t + 8 + g] = v.y;
+          } else {
             v.x = __fmaf_rn(__fmul_rn(v.x, 1.f / kCode), unit, sum_b);
             v.y = __fmaf_rn(__fmul_rn(v.y, 1.f / kCode), unit, sum_b);
+            *reinterpret_cast<float2*>(to + (BITS == 8 ? 16 * t + 2 * g : 32 * (t / 2) + 4 * g + 2 * (t % 2))) = v;
           }
-          *reinterpret_cast<float2*>(&sm_o[row_warp][h][(8 * ch + g) * kPer + 2 * j]) = v;
         }
       }
     }
@@ -824,7 +786,7 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
 #pragma unroll
       for (int w = 0; w < S::kRowWarps; ++w) {
         const float f = exp2_of(sm_m[w][h] - from);
-        const float4 x = *reinterpret_cast<const float4*>(&sm_o[w][h][column]);
+        const float4 x = *reinterpret_cast<const float4*>(sm_o + (w * S::kHeads + h) * S::HP + column);
         sum_l = __fmaf_rn(f, sm_l[w][h], sum_l);
         v.x = __fmaf_rn(f, x.x, v.x);
         v.y = __fmaf_rn(f, x.y, v.y);
@@ -860,6 +822,7 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
       ++request;
       unit_in_request = 0;
     }
+    __syncthreads();  // (the rings are filled again)
   }
   if (tid == 0 && p.open) {
     p.open[blockIdx.x] = opened;
@@ -958,11 +921,31 @@ PagedAttentionPlan plan_of(int group, int64_t sms) {
   return r;
 }
 
+// More than 48 KB of shared memory have to be asked for, once per kernel and device.
+template <typename Kernel>
+cudaError_t allow_shared(Kernel kernel, int bytes, std::atomic<uint64_t>& asked) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  const uint64_t bit = 1ull << (device & 63);
+  if (e == cudaSuccess && (device > 63 || !(asked.load(std::memory_order_relaxed) & bit))) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) {
+      asked.fetch_or(bit, std::memory_order_relaxed);
+    }
+  }
+  return e;
+}
+
 template <typename S, bool BF16, bool FAST>
 cudaError_t launch_of(const PagedAttentionPlan& plan, const PagedAttentionParams& p, bool split, cudaStream_t stream) {
-  paged_attention_kernel<S, BF16, FAST><<<(unsigned)plan.workers, kThreads, 0, stream>>>(p);
+  static std::atomic<uint64_t> asked{0};
+  cudaError_t e = allow_shared(paged_attention_kernel<S, BF16, FAST>, S::kShared, asked);
+  if (e != cudaSuccess) {
+    return e;
+  }
+  paged_attention_kernel<S, BF16, FAST><<<(unsigned)plan.workers, kThreads, S::kShared, stream>>>(p);
   g_launch_count.fetch_add(1, std::memory_order_relaxed);
-  cudaError_t e = cudaGetLastError();
+  e = cudaGetLastError();
   if (e != cudaSuccess || !split) {
     return e;
   }

@@ -105,6 +105,7 @@ struct PagedAttentionParams {
   int64_t most_rows;                              // rows that a block table names
   float scale_log2;                               // softmax scale * log2(e)
   int32_t num_pages, page_shift, batch, kv_heads, group, head_tiles, dim, window, workers;
+  bool aligned;                                   // rows are 16-byte aligned
 };
 
 // Which kernel a cache takes (paged_attention_kernels.cu).
@@ -113,7 +114,7 @@ struct PagedAttentionShape {
   bool bf16;          // of q, the output and 16-bit rows
   int32_t dim;
   int32_t group;      // query heads per cached head
-  bool fast;          // rows 16-byte aligned, 16 or more to a page
+  bool fast;          // rows 16-byte aligned, 16 or more to a page, 16 within 2 GB
 };
 struct PagedAttentionPlan {
   int32_t unit;        // rows per unit
