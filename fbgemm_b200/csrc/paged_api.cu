@@ -102,7 +102,8 @@ PagedAttentionShape shape_of(const fbgemm_b200_paged_cache& c, int32_t q_heads, 
   s.bf16 = dtype == FBGEMM_B200_OUT_BF16;
   s.dim = c.head_dim;
   s.group = q_heads / c.kv_heads;
-  s.fast = c.page_size >= 16 && rows_aligned(c) && c.slot_stride < (1 << 27);
+  s.fast = c.page_size >= 16 && rows_aligned(c) && c.page_stride < (1LL << 39) && c.slot_stride < (1LL << 39) &&
+      c.head_stride < (1LL << 39);
   return s;
 }
 

@@ -12,17 +12,19 @@
 //
 // At 44 GB/s per SM and a microsecond of latency about 44 KB have to be on their way to every SM all the time.  Each
 // warp has a ring of half tiles (16 or 32 rows of K, or of V) in shared memory that it fills by asynchronous copies of
-// its own, several ahead of the one it works on: 165 KB per SM at 128 columns.  (With the rows on their way to registers a
+// its own, several ahead of the one it works on: 147 KB per SM at 128 columns.  (With the rows on their way to registers a
 // warp had two half tiles in flight at most: 97 us for 64 requests of up to 8192 16-bit rows, 92 for 128 of up to 4096 4-bit
-// rows.)  Rows lie an odd multiple of 16 bytes apart there, so that ldmatrix reads K without
-// conflicts, and turns V, for 16-bit values and for pairs of 8-bit and fours of 4-bit codes alike: a register holds the
-// same columns of two rows, and their codes become two fp16 numbers by a mask or a byte permutation that puts them into
-// the lowest bits: subnormal numbers, c 2^-24 (4-bit codes in the upper half of a byte, c 2^-20), which the products take
-// exactly.  The power of two is made up for once per score and result.  (The products align a subnormal as if its first
-// bit were set: 4-bit codes in the lowest 4 bits cost 6 bits of the sums, and results that were off by 1e-3.)
+// rows.)  Pages of 16 rows and more hold all 16 rows of a step: one lane asks for a step by a tensor copy, whatever the strides (FAST;
+// copies of 16 bytes by all lanes cost half of all instructions, 102 us for one request of 131072 16-bit rows);
+// smaller pages and unaligned rows are copied in pieces of 16 or 4 bytes.  Rows that the token does not see are masked, in
+// the tiles that have some.
 //
-// Pages of 16 rows and more hold all 16 rows of a step, which then share one address (FAST); smaller pages and unaligned
-// rows have an address each.  Rows that the token does not see arrive as zeros, and a tile that has some is masked.
+// ldmatrix reads K without conflicts (16-bit rows are swizzled, quantized ones an odd multiple of 16 bytes apart), and
+// turns V, for 16-bit values and for pairs of 8-bit and fours of 4-bit codes alike: a register holds the same columns of
+// two rows, and their codes become two fp16 numbers by a mask or a byte permutation that puts them into the lowest
+// bits: subnormal numbers, c 2^-24 (4-bit codes in the upper half of a byte, c 2^-20), which the products take exactly.
+// The power of two is made up for once per score and result.  (The products align a subnormal as if its first bit were
+// set: 4-bit codes in the lowest 4 bits cost 6 bits of the sums, and results that were off by 1e-3.)
 //
 // One pass with a running maximum and sum per head in fp32 (in registers, per warp).  A tile's largest score is looked
 // for across lanes only if one exceeds the running maximum by more than 2^kSlack.  Weights are rounded to 16 bits for
@@ -36,6 +38,7 @@
 // second launch (paged_attention_join) adds them up in a fixed order.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -43,6 +46,13 @@
 #include "paged_cache.h"
 
 namespace fbgemm_b200 {
+
+// The rows at `rows` (K's or V's) as a tensor [page][slot][head][columns] for copies of 16 rows of a head: 16-bit columns in
+// swizzled boxes of 64, quantized rows as 4-byte words in boxes of `box`, whose end is filled with zeros
+// (paged_attention_dispatch.cu).
+cudaError_t encode_rows(CUtensorMap* map, const uint8_t* rows, const PagedAttentionParams& p, bool swizzled, int box, int bits,
+                        int tail_bytes);
+
 namespace paged {
 
 constexpr int kWarps = 4;
@@ -117,6 +127,37 @@ __device__ __forceinline__ void copy4(uint32_t to, const uint8_t* from, uint32_t
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 
+// ---- tensor copies ----------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ void barrier_init(uint32_t bar) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// Waits for a phase of the barrier, for a second or so at most; false: it did not come.
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
+  for (int i = 0; i < (1 << 24); ++i) {
+    uint32_t done;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(done)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+    if (done) {
+      return true;
+    }
+  }
+  return false;
+}
+__device__ __forceinline__ void copy_box(uint32_t to, const CUtensorMap* map, int column, int head, int slot, int page,
+                                         uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          to),
+      "l"(map), "r"(column), "r"(head), "r"(slot), "r"(page), "r"(bar)
+      : "memory");
+}
+
 // Nibbles i and i + 4 of a word as subnormal fp16.
 __device__ __forceinline__ uint32_t nibbles(uint32_t w, int i) {
   return (i == 0 ? w << 4 : w >> (4 * i - 4)) & 0x00f000f0u;
@@ -135,11 +176,15 @@ struct Shape {
   static constexpr int BITS = BITS_, DP = DP_, NT = NT_, HW = HW_;
   static constexpr int kTail = BITS == 8 ? 8 : BITS == 4 ? 4 : 0;   // bytes of a row's scale and bias
   static constexpr int kPieces = (DP * BITS / 8 + kTail + 15) / 16; // 16-byte pieces of a row
-  static constexpr int PITCH = (kPieces | 1) * 16;                  // between rows in shared memory
+  static constexpr int PITCH = (kPieces | 1) * 16;                  // between rows in shared memory (not swizzled ones)
   static constexpr int kBlocks16 = DP * BITS / 128;                 // 16-byte blocks of a row's columns
   static constexpr int SUB = PITCH > 144 ? 1 : 2;                   // 16-row steps of a tile
   static constexpr int ROWS = 16 * SUB;                             // of a warp's tile
+  static constexpr bool kSwizzled = BITS == 16;                     // by tensor copies: boxes of 16 rows of 128 bytes
+  static constexpr int kBoxes = kSwizzled ? DP / 64 : 1;            // of a step
+  static constexpr int kBoxBytes = 16 * (kSwizzled ? 128 : PITCH);
   static constexpr int SLOT = ROWS * PITCH;                         // bytes of a half tile
+  static constexpr int SLOT_FAST = SUB * kBoxes * kBoxBytes;
   static constexpr int kRowWarps = kWarps / HW;
   static constexpr int UNIT = kRowWarps * ROWS;
   static constexpr int KSTEPS = DP / 16;
@@ -151,26 +196,33 @@ struct Shape {
   // by shared memory.
   static constexpr int kRegisters = 4 * NT * MT + 2 * NT * KSTEPS + 4 * NT * SUB;
   static constexpr int kBlocks = kRegisters <= 90 ? 3 : 2;
-  static constexpr int kFit = 224 * 1024 / (kBlocks * kWarps * SLOT);
+  static constexpr int kFit = 222 * 1024 / (kBlocks * kWarps * SLOT);
   static constexpr int SLOTS = kFit > 6 ? 6 : kFit;
   static constexpr int HP = DP + 4;                                 // floats between heads in the join of the warps
-  static constexpr int kRing = kWarps * SLOTS * SLOT, kJoin = kRowWarps * kHeads * HP * 4;
-  static constexpr int kShared = kRing > kJoin ? kRing : kJoin;
+  static constexpr int kJoin = kRowWarps * kHeads * HP * 4;
+  static constexpr int kRing = kWarps * SLOTS * SLOT;               // (as large as the ring of tensor copies with its alignment)
+  static constexpr int kShared = (kRing > kJoin ? kRing : kJoin) + 1024;
+  static_assert(SLOT >= SLOT_FAST, "one size for both");
   static_assert(SLOTS >= 3, "two half tiles on their way");
 };
 
 // ---- the kernel -------------------------------------------------------------------------------------------------------
 
-// FAST: pages of 16 rows or more, rows 16-byte aligned.
+// FAST: pages of 16 rows or more, rows 16-byte aligned, by tensor copies.
 template <typename S, bool BF16, bool FAST>
-__global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(const PagedAttentionParams p) {
+__global__ void __launch_bounds__(kThreads, S::kBlocks)
+paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUtensorMap k_map,
+                       const __grid_constant__ CUtensorMap v_map) {
   constexpr int BITS = S::BITS, NT = S::NT, SUB = S::SUB;
   constexpr bool kQuantized = BITS != 16;
   constexpr bool kMmaBf16 = !kQuantized && BF16;
   constexpr float kMiddle = BITS == 8 ? 128.f : 8.f;
   constexpr float kCode = BITS == 4 ? 1.f / 1048576.f : 1.f / 16777216.f;  // what a code of 1 is to the products
   constexpr unsigned kFull = S::ROWS == 32 ? kAll : (1u << (S::ROWS & 31)) - 1;
-  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int kSlot = FAST ? S::SLOT_FAST : S::SLOT;
+  extern __shared__ __align__(1024) uint8_t smem_start[];
+  uint8_t* const smem = smem_start + (-(uint32_t)__cvta_generic_to_shared(smem_start) & 1023);  // swizzled boxes: 1024 bytes
+  __shared__ uint64_t sm_bars[kWarps][S::SLOTS];
   __shared__ unsigned sm_seen[kWarps][S::SLOTS];  // rows of a half tile that the token sees
   __shared__ float sm_m[S::kRowWarps][S::kHeads], sm_l[S::kRowWarps][S::kHeads];
   __shared__ int64_t sm_sums[kWarps];
@@ -198,15 +250,12 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
   if (lane == 31) {
     sm_sums[warp] = before;
   }
-  // (columns that no row has stay 0 in the rings)
-  uint8_t* const ring = smem + warp * (S::SLOTS * S::SLOT);
-  auto clear_ring = [&] {
-    for (int at = lane * 16; at < S::SLOTS * S::SLOT; at += 512) {
-      *reinterpret_cast<uint4*>(ring + at) = make_uint4(0, 0, 0, 0);
-    }
-    __syncwarp();
-  };
-  const bool padded = !kQuantized && p.dim < S::DP;
+  uint8_t* const ring = smem + warp * (S::SLOTS * kSlot);
+  const uint32_t bars = (uint32_t)__cvta_generic_to_shared(&sm_bars[warp][0]);
+  if (FAST && lane < S::SLOTS) {
+    barrier_init(bars + 8 * lane);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   __syncthreads();
   before -= sum;
   int64_t total = 0;
@@ -242,12 +291,27 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
 
   const int row_bytes = p.dim * BITS / 8 + S::kTail;
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-  const uint32_t ring_end = ring_at + S::SLOTS * S::SLOT;
+  const uint32_t ring_end = ring_at + S::SLOTS * kSlot;
   // ldmatrix: K's matrices are rows 0 - 7 and 8 - 15 of a block of columns, then of the next; V's two blocks of rows 0 - 7,
   // then of 8 - 15.
-  const uint32_t k_lane = ((lane & 7) + (lane & 8)) * S::PITCH + (lane >> 4) * 16;
-  const uint32_t v_lane = ((lane & 7) + ((lane >> 4) << 3)) * S::PITCH + ((lane >> 3) & 1) * 16;
+  constexpr bool kSwizzled = FAST && S::kSwizzled;
+  constexpr int kRow = kSwizzled ? 128 : S::PITCH;
+  const uint32_t k_lane = ((lane & 7) + (lane & 8)) * kRow, k_odd = lane >> 4;
+  const uint32_t v_lane = ((lane & 7) + ((lane >> 4) << 3)) * kRow, v_odd = (lane >> 3) & 1;
   const uint32_t tail_lane = g * S::PITCH + p.dim * BITS / 8;
+  // (b even: this lane's block b or b + 1 of step s; in a swizzled box block x of row r is at x ^ (r % 8))
+  auto matrix_at = [&](uint32_t half, uint32_t row, uint32_t odd, int s, int b) {
+    if constexpr (kSwizzled) {
+      return half + row + (s * S::kBoxes + b / 8) * S::kBoxBytes + ((((b % 8) | odd) ^ (lane & 7)) << 4);
+    } else {
+      return half + row + 16 * s * S::PITCH + 16 * (b + odd);
+    }
+  };
+
+  // The ring: what is filled next and what is worked on.
+  uint32_t fill_at = ring_at, at = ring_at;
+  int fill_slot = 0, slot = 0;
+  uint32_t phase = 0;
 
   // -- item after item: a request, a cached head and a tile of its query heads
   while (unit_at < last_unit) {
@@ -267,105 +331,150 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
       p.status[3] = length;
     }
 
-    const uint8_t* const k_rows = p.k + kv_head * p.head_stride;
-    const uint8_t* const v_rows = p.v + kv_head * p.head_stride;
     const int32_t* const table = p.tables + request * p.table_stride;
 
     // Tile i of this warp: rows row0 + i * UNIT onwards.
     const int64_t row0 = aligned_first(span) + ((int64_t)u0 * S::kRowWarps + row_warp) * S::ROWS;
     const int tiles = (int)min((int64_t)(u1 - u0), row0 < span.end ? (span.end - row0 + S::UNIT - 1) / S::UNIT : 0);
-    // A lane looks after the address of a step's 16 rows (FAST), or of one row.
-    constexpr int kLeaders = FAST ? SUB : S::ROWS;
-    auto row_of = [&](int i) { return row0 + (int64_t)i * S::UNIT + lane * (FAST ? 16 : 1); };
-    auto led = [&](int i) {
-      const int64_t row = row_of(i);
-      return i < tiles && lane < kLeaders && row < span.end && (FAST || row >= span.first);
-    };
-    auto read_page = [&](int i) { return led(i) ? __ldg(table + (row_of(i) >> p.page_shift)) : 0; };
-    // Byte offset of the row (0 in place of one that does not exist) and the rows of the tile that the token sees.
-    auto offset_of = [&](int i, int32_t page, unsigned& seen) -> int64_t {
-      const bool exists = led(i);
-      const bool good = exists && page >= 0 && page < p.num_pages;
-      if (exists && !good && atomicCAS(p.status, 0, FBGEMM_B200_STATUS_BAD_PAGE) == 0) {
+    auto report_page = [&](int64_t row, int32_t page) {
+      if (atomicCAS(p.status, 0, FBGEMM_B200_STATUS_BAD_PAGE) == 0) {
         p.status[1] = request;
-        p.status[2] = (int32_t)row_of(i);
+        p.status[2] = (int32_t)row;
         p.status[3] = page;
       }
-      seen = __ballot_sync(kAll, good);
-      if constexpr (FAST) {
-        const int64_t row = row0 + (int64_t)i * S::UNIT;
-        seen = (seen & 1 ? 0xffffu : 0u) | (SUB == 2 && (seen & 2) ? 0xffff0000u : 0u);
-        if (row < span.first) {  // (by less than 16)
-          seen &= ~0u << (span.first - row);
-        }
-        if (row + S::ROWS > span.end) {
-          seen &= span.end > row ? kFull >> (row + S::ROWS - span.end) : 0u;
-        }
-      }
-      return good ? page * p.page_stride + (row_of(i) & ((1 << p.page_shift) - 1)) * p.slot_stride : 0;
     };
-
-    // A half tile's rows on their way to `to`.
-    auto copy_rows = [&](uint32_t to, const uint8_t* rows, int64_t off, unsigned seen) {
-      if (FAST || p.aligned) {
-        const int pieces = (row_bytes + 15) / 16;
-#pragma unroll
-        for (int s = 0; s < SUB; ++s) {
-          const uint8_t* step = FAST ? rows + __shfl_sync(kAll, off, s) : rows;
-          constexpr int kRounds = (16 * S::kPieces + 31) / 32;
-#pragma unroll
-          for (int j = 0; j < kRounds; ++j) {
-            const int at = lane + 32 * j, row = at / S::kPieces, piece = at - row * S::kPieces;
-            const int64_t row_off = FAST ? (int64_t)(uint32_t)(row * (uint32_t)p.slot_stride) : __shfl_sync(kAll, off, 16 * s + min(row, 15));
-            if (piece < pieces && (16 * S::kPieces % 32 == 0 || row < 16)) {
-              copy16(to + (16 * s + row) * S::PITCH + piece * 16, step + row_off + piece * 16,
-                     (seen >> (16 * s + row)) & 1 ? 16 : 0);
-            }
-          }
-        }
-      } else if (lane < S::ROWS) {
-        const uint32_t bytes = (seen >> lane) & 1 ? 4 : 0;
-        for (int at = 0; at < row_bytes; at += 4) {
-          copy4(to + lane * S::PITCH + at, rows + off + at, bytes);
-        }
-      }
-    };
-
-    // -- half tile h: K (even) or V (odd) of tile h / 2, into slot h % SLOTS; SLOTS - 1 are on their way
-    int64_t off = 0;
-    unsigned seen = 0;
-    int32_t page_next = read_page(0), page_after = read_page(1);
-    int fill_tile = -1;
-    uint32_t fill_at = ring_at;
-    int fill_slot = 0;
-    auto fill = [&](bool is_v) {
-      if (!is_v) {
-        ++fill_tile;
-        off = offset_of(fill_tile, page_next, seen);
-        page_next = page_after;
-        page_after = read_page(fill_tile + 2);
-      }
-      if (fill_tile < tiles) {
-        copy_rows(fill_at, is_v ? v_rows : k_rows, off, seen);
-        if (lane == 0) {
-          sm_seen[warp][fill_slot] = seen;
-        }
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      fill_at += S::SLOT;
+    auto next_fill = [&] {
+      fill_at += kSlot;
       ++fill_slot;
       if (fill_at == ring_end) {
         fill_at = ring_at;
         fill_slot = 0;
       }
     };
+
+    // -- half tiles come in turn: K and V of a tile, then of the next.  SLOTS - 1 are on their way.
+    int fill_tile = -1;
+    unsigned seen = 0;  // rows of the tile that is filled that the token sees
+    // FAST: every lane knows the pages of the steps.  Otherwise a lane looks after one row.
+    constexpr int kPages = FAST ? SUB : 1;
+    int32_t page[kPages], page_next[kPages], page_after[kPages];
+    int64_t off = 0;
+    auto read_page = [&](int i, int s) {
+      const int64_t row = row0 + (int64_t)i * S::UNIT + (FAST ? 16 * s : lane);
+      const bool there = i < tiles && row < span.end && (FAST || (lane < S::ROWS && row >= span.first));
+      return there ? __ldg(table + (row >> p.page_shift)) : 0;
+    };
+#pragma unroll
+    for (int s = 0; s < kPages; ++s) {
+      page_next[s] = read_page(0, s);
+      page_after[s] = read_page(1, s);
+    }
+    auto next_tile = [&] {
+      ++fill_tile;
+      const int64_t row = row0 + (int64_t)fill_tile * S::UNIT;
+#pragma unroll
+      for (int s = 0; s < kPages; ++s) {
+        page[s] = page_next[s];
+        page_next[s] = page_after[s];
+        page_after[s] = read_page(fill_tile + 2, s);
+      }
+      if (fill_tile >= tiles) {
+        return;
+      }
+      if constexpr (FAST) {
+        seen = kFull;
+        if (row < span.first) {  // (by less than 16)
+          seen &= ~0u << (span.first - row);
+        }
+        if (row + S::ROWS > span.end) {
+          seen &= kFull >> (row + S::ROWS - span.end);
+        }
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+          if ((uint32_t)page[s] >= (uint32_t)p.num_pages) {
+            if (lane == 0 && ((seen >> (16 * s)) & 0xffffu)) {
+              report_page(row + 16 * s + (s == 0 && row < span.first ? span.first - row : 0), page[s]);
+            }
+            seen &= ~(0xffffu << (16 * s));
+          }
+        }
+      } else {
+        const bool there = lane < S::ROWS && row + lane < span.end && row + lane >= span.first;
+        const bool good = there && (uint32_t)page[0] < (uint32_t)p.num_pages;
+        if (there && !good) {
+          report_page(row + lane, page[0]);
+        }
+        seen = __ballot_sync(kAll, good);
+        off = good ? page[0] * p.page_stride + ((row + lane) & ((1 << p.page_shift) - 1)) * p.slot_stride : 0;
+      }
+    };
+    auto fill = [&](bool is_v) {
+      if (!is_v) {
+        next_tile();
+      }
+      if (fill_tile < tiles) {
+        if constexpr (FAST) {
+          if (lane == 0) {
+            sm_seen[warp][fill_slot] = seen;
+            const int row = (int)((row0 + (int64_t)fill_tile * S::UNIT) & ((1 << p.page_shift) - 1));
+            const uint32_t bar = bars + 8 * fill_slot;
+            int steps = 0;
+#pragma unroll
+            for (int s = 0; s < SUB; ++s) {
+              steps += ((seen >> (16 * s)) & 0xffffu) != 0;
+            }
+            barrier_expect(bar, steps * (S::kBoxes * S::kBoxBytes));
+#pragma unroll
+            for (int s = 0; s < SUB; ++s) {
+              if ((seen >> (16 * s)) & 0xffffu) {
+#pragma unroll
+                for (int x = 0; x < S::kBoxes; ++x) {
+                  copy_box(fill_at + (s * S::kBoxes + x) * S::kBoxBytes, is_v ? &v_map : &k_map, 64 * x, kv_head,
+                           (row + 16 * s) & ((1 << p.page_shift) - 1), page[s], bar);
+                }
+              }
+            }
+          }
+        } else {
+          if (lane == 0) {
+            sm_seen[warp][fill_slot] = seen;
+          }
+          const uint8_t* const rows = (is_v ? p.v : p.k) + kv_head * p.head_stride;
+          if (p.aligned) {
+            constexpr int kRounds = (S::ROWS * S::kPieces + 31) / 32;
+#pragma unroll 4
+            for (int j = 0; j < kRounds; ++j) {
+              const int n = lane + 32 * j, r = n / S::kPieces, piece = n - r * S::kPieces;
+              const int64_t row = __shfl_sync(kAll, off, min(r, S::ROWS - 1));
+              if (r < S::ROWS) {  // (pieces behind the row's: zeros)
+                copy16(fill_at + r * S::PITCH + piece * 16, rows + row + (piece * 16 < row_bytes ? piece * 16 : 0),
+                       ((seen >> r) & 1) && piece * 16 < row_bytes ? 16 : 0);
+              }
+            }
+          } else if (lane < S::ROWS) {
+            const uint32_t bytes = (seen >> lane) & 1 ? 4 : 0;
+            for (int n = 0; n < row_bytes; n += 4) {
+              copy4(fill_at + lane * S::PITCH + n, rows + off + n, bytes);
+            }
+          }
+        }
+        next_fill();
+      }
+      if constexpr (!FAST) {
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+    };
+    // The half tile that is worked on next is there, and the one before has been read by all lanes.
     auto arrived = [&] {
-      asm volatile("cp.async.wait_group %0;" ::"n"(S::SLOTS - 2) : "memory");
+      if constexpr (FAST) {
+        if (!barrier_wait(bars + 8 * slot, phase) && atomicCAS(p.status, 0, FBGEMM_B200_STATUS_COPY_TIMEOUT) == 0) {
+          p.status[1] = request;
+        }
+      } else {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S::SLOTS - 2) : "memory");
+      }
       __syncwarp();
     };
-    if (padded) {
-      clear_ring();
-    }
 
     // -- queries as the products take them: head g of a tile in lanes 4g .. 4g + 3, columns in the order of K's registers.
     // Columns of 16 bits: 2c, 2c + 1 and 2c + 8, 2c + 9 of a step of 16.  8-bit codes: 4c .. 4c + 3 of a step.  4-bit codes:
@@ -485,14 +594,13 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
     }
     int exponent = 1;  // 127 + the exponent that V's scales are taken relative to
 
-    uint32_t at = ring_at;
-    int slot = 0;
     auto advance = [&] {
-      at += S::SLOT;
+      at += kSlot;
       ++slot;
       if (at == ring_end) {
         at = ring_at;
         slot = 0;
+        phase ^= 1;
       }
     };
     auto tail_of = [&](uint32_t half, int s, int r) {
@@ -525,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
 #pragma unroll
         for (int b = 0; b < S::kBlocks16; b += 2) {
           uint32_t r[4];
-          load_matrices(r, at + k_lane + 16 * s * S::PITCH + 16 * b);
+          load_matrices(r, matrix_at(at, k_lane, k_odd, s, b));
           if constexpr (BITS == 16) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -594,6 +702,16 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
       // -- weights
       arrived();
       fill(S::SLOTS % 2 != 0);
+      if (kSwizzled && rows_seen != kFull) {  // whatever else the page holds: weights of 0 do not make up for infinities
+        for (int n = lane; n < S::SLOT_FAST / 16; n += 32) {
+          const int row = (n / 8) % 16 + 16 * (n / (S::kBoxes * 128));
+          if (!((rows_seen >> row) & 1)) {
+            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(at + 16 * n), "r"(0) : "memory");
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+      }
       bool more = false;
       float top[NT][2];
 #pragma unroll
@@ -616,6 +734,9 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             v_sb[s][r] = tail_of(at, s, r);
+            if (rows_seen != kFull && !((rows_seen >> (16 * s + 8 * r + g)) & 1)) {
+              v_sb[s][r] = make_float2(0.f, 0.f);
+            }
             largest = max(largest, (__float_as_uint(v_sb[s][r].x) >> 23) & 0xff);
           }
         }
@@ -696,7 +817,7 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
 #pragma unroll
         for (int b = 0; b < S::kBlocks16; b += 2) {
           uint32_t r[4];
-          load_turned(r, at + v_lane + 16 * s * S::PITCH + 16 * b);
+          load_turned(r, matrix_at(at, v_lane, v_odd, s, b));
           if constexpr (BITS == 16) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -731,7 +852,9 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
     }
 
     // -- the warps' results together, where the rings were
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    if constexpr (!FAST) {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    }
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -773,8 +896,8 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
     const bool whole = u0 == 0 && u1 == units;
     const bool none = span.end == span.first;
     float* const part = whole ? nullptr : p.parts + (2 * (int64_t)blockIdx.x + (u0 == 0)) * S::kPartFloats;
-    for (int at = tid; at < heads * (S::DP / 4); at += kThreads) {
-      const int h = at / (S::DP / 4), column = at % (S::DP / 4) * 4;
+    for (int n = tid; n < heads * (S::DP / 4); n += kThreads) {
+      const int h = n / (S::DP / 4), column = n % (S::DP / 4) * 4;
       float top = -INFINITY;
 #pragma unroll
       for (int w = 0; w < S::kRowWarps; ++w) {
@@ -821,6 +944,9 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks) paged_attention_kernel(c
     if (unit_in_request == (int64_t)units * per_request) {
       ++request;
       unit_in_request = 0;
+    }
+    if constexpr (FAST) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncthreads();  // (the rings are filled again)
   }
@@ -940,10 +1066,16 @@ template <typename S, bool BF16, bool FAST>
 cudaError_t launch_of(const PagedAttentionPlan& plan, const PagedAttentionParams& p, bool split, cudaStream_t stream) {
   static std::atomic<uint64_t> asked{0};
   cudaError_t e = allow_shared(paged_attention_kernel<S, BF16, FAST>, S::kShared, asked);
+  CUtensorMap maps[2] = {};
+  if (FAST && e == cudaSuccess) {
+    for (int i = 0; i < 2 && e == cudaSuccess; ++i) {
+      e = encode_rows(&maps[i], i ? p.v : p.k, p, S::kSwizzled, S::kSwizzled ? 64 : S::PITCH / 4, S::BITS, S::kTail);
+    }
+  }
   if (e != cudaSuccess) {
     return e;
   }
-  paged_attention_kernel<S, BF16, FAST><<<(unsigned)plan.workers, kThreads, S::kShared, stream>>>(p);
+  paged_attention_kernel<S, BF16, FAST><<<(unsigned)plan.workers, kThreads, S::kShared, stream>>>(p, maps[0], maps[1]);
   g_launch_count.fetch_add(1, std::memory_order_relaxed);
   e = cudaGetLastError();
   if (e != cudaSuccess || !split) {

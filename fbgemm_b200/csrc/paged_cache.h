@@ -114,7 +114,7 @@ struct PagedAttentionShape {
   bool bf16;          // of q, the output and 16-bit rows
   int32_t dim;
   int32_t group;      // query heads per cached head
-  bool fast;          // rows 16-byte aligned, 16 or more to a page, 16 within 2 GB
+  bool fast;          // rows 16-byte aligned, 16 or more to a page
 };
 struct PagedAttentionPlan {
   int32_t unit;        // rows per unit

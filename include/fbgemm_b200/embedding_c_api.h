@@ -72,6 +72,7 @@ extern "C" {
 #define FBGEMM_B200_STATUS_PEER_TIMEOUT 5 /* a peer's counter did not arrive in time */
 #define FBGEMM_B200_STATUS_NO_PAGES 6   /* free pages, table columns or map capacity ran out */
 #define FBGEMM_B200_STATUS_BAD_PAGE 7   /* a page or slot outside the cache */
+#define FBGEMM_B200_STATUS_COPY_TIMEOUT 8 /* a kernel's own copy did not arrive in time: the results are void */
 
 /* Number of status slots a context owns (see fbgemm_b200_spmdm_launch). */
 #define FBGEMM_B200_STATUS_SLOTS 1024
