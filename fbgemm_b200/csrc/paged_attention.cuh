@@ -33,9 +33,12 @@
 // A weight's rounding is at most half a step of the output's own type, and averages out over the rows; codes are weighed
 // about the middle of their range (sum w (c - 128) = sum w c - 128 sum w, with the rounded w), which keeps it there.
 //
-// Work is split over the chip by paged_cache.h's rule.  A worker is a block of 4 warps that take the tiles of its units
-// in turn and join their results in shared memory; an item that several workers share is left as partial results, and a
-// second launch (paged_attention_join) adds them up in a fixed order.
+// Work is split over the chip by paged_cache.h's rule: a worker is a warp (or the HW warps that share rows), and nothing
+// makes warps wait for one another, so that what a warp does between two items (its results out, the next queries in) is
+// covered by the other warps of the SM; its ring runs on into the next item meanwhile.  (Blocks that joined their warps'
+// results item by item took 77 us for 128 requests of 64 to 4096 4-bit rows.)  An item that several workers share is
+// left as partial results, and a second launch (paged_attention_join) adds them up in a fixed order; a block whose workers
+// all work on one item joins theirs first.
 #pragma once
 
 #include <cuda.h>
@@ -57,6 +60,7 @@ namespace paged {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
+constexpr int kJoinThreads = 256, kJoinTeam = 4;
 // Weights are 2^kShift times as large as in the formula and at most 2^kSlack above their reference: 2^14 at most, and with
 // a scale of less than 2 below 2^15.
 constexpr float kShift = 10.f, kSlack = 4.f;
@@ -185,8 +189,8 @@ struct Shape {
   static constexpr int kBoxBytes = 16 * (kSwizzled ? 128 : PITCH);
   static constexpr int SLOT = ROWS * PITCH;                         // bytes of a half tile
   static constexpr int SLOT_FAST = SUB * kBoxes * kBoxBytes;
-  static constexpr int kRowWarps = kWarps / HW;
-  static constexpr int UNIT = kRowWarps * ROWS;
+  static constexpr int UNIT = ROWS;
+  static constexpr int kWorkers = kWarps / HW;                      // of a block
   static constexpr int KSTEPS = DP / 16;
   static constexpr int MT = DP / 16;                                // 16-column tiles of the output
   static constexpr int kWarpHeads = 8 * NT;
@@ -198,10 +202,7 @@ struct Shape {
   static constexpr int kBlocks = kRegisters <= 90 ? 3 : 2;
   static constexpr int kFit = 222 * 1024 / (kBlocks * kWarps * SLOT);
   static constexpr int SLOTS = kFit > 6 ? 6 : kFit;
-  static constexpr int HP = DP + 4;                                 // floats between heads in the join of the warps
-  static constexpr int kJoin = kRowWarps * kHeads * HP * 4;
-  static constexpr int kRing = kWarps * SLOTS * SLOT;               // (as large as the ring of tensor copies with its alignment)
-  static constexpr int kShared = (kRing > kJoin ? kRing : kJoin) + 1024;
+  static constexpr int kShared = kWarps * SLOTS * SLOT + 1024;      // (aligned for swizzled boxes)
   static_assert(SLOT >= SLOT_FAST, "one size for both");
   static_assert(SLOTS >= 3, "two half tiles on their way");
 };
@@ -224,22 +225,34 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   uint8_t* const smem = smem_start + (-(uint32_t)__cvta_generic_to_shared(smem_start) & 1023);  // swizzled boxes: 1024 bytes
   __shared__ uint64_t sm_bars[kWarps][S::SLOTS];
   __shared__ unsigned sm_seen[kWarps][S::SLOTS];  // rows of a half tile that the token sees
-  __shared__ float sm_m[S::kRowWarps][S::kHeads], sm_l[S::kRowWarps][S::kHeads];
   __shared__ int64_t sm_sums[kWarps];
-  __shared__ int32_t sm_request;
-  __shared__ int64_t sm_unit;
-  float* const sm_o = reinterpret_cast<float*>(smem);  // [row warp][head][HP], in place of the rings
+  __shared__ int32_t sm_request[S::kWorkers];
+  __shared__ int64_t sm_unit[S::kWorkers];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-  const int row_warp = warp / S::HW, head_warp = warp % S::HW;
+  const int head_warp = warp % S::HW;
   const int per_request = p.kv_heads * p.head_tiles;
+  uint8_t* const ring = smem + warp * (S::SLOTS * kSlot);
+  const uint32_t bars = (uint32_t)__cvta_generic_to_shared(&sm_bars[warp][0]);
+  if (FAST && lane < S::SLOTS) {
+    barrier_init(bars + 8 * lane);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (FAST && tid < 2) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(tid ? &v_map : &k_map) : "memory");
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  // -- this worker's units, and the request that the first of them belongs to
+  // -- the units of this block's workers, and the requests that their first ones belong to
   const int chunk = (p.batch + kThreads - 1) / kThreads;
   const int b0 = min(tid * chunk, p.batch), b1 = min(b0 + chunk, p.batch);
+  auto units_of_request = [&](int b) {
+    return (int64_t)units_of(span_of(p.lengths[b], p.window, p.most_rows), S::UNIT) * per_request;
+  };
   int64_t sum = 0;
   for (int b = b0; b < b1; ++b) {
-    sum += (int64_t)units_of(span_of(p.lengths[b], p.window, p.most_rows), S::UNIT) * per_request;
+    sum += units_of_request(b);
   }
   int64_t before = sum;
 #pragma unroll
@@ -250,11 +263,9 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   if (lane == 31) {
     sm_sums[warp] = before;
   }
-  uint8_t* const ring = smem + warp * (S::SLOTS * kSlot);
-  const uint32_t bars = (uint32_t)__cvta_generic_to_shared(&sm_bars[warp][0]);
-  if (FAST && lane < S::SLOTS) {
-    barrier_init(bars + 8 * lane);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  if (tid < S::kWorkers) {
+    sm_request[tid] = 0;
+    sm_unit[tid] = 0;
   }
   __syncthreads();
   before -= sum;
@@ -264,30 +275,27 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     before += w < warp ? sm_sums[w] : 0;
     total += sm_sums[w];
   }
-  const int64_t per = units_per_worker(total, gridDim.x);
-  const int64_t first_unit = (int64_t)blockIdx.x * per, last_unit = min(first_unit + per, total);
-  if (first_unit >= total) {
-    if (tid == 0 && p.open) {
-      p.open[blockIdx.x] = make_int4(0, 0, 0, 0);
-    }
-    return;
-  }
-  if (first_unit >= before && first_unit < before + sum) {
-    for (int b = b0; b < b1; ++b) {
-      const int64_t n = (int64_t)units_of(span_of(p.lengths[b], p.window, p.most_rows), S::UNIT) * per_request;
-      if (first_unit < before + n) {
-        sm_request = b;
-        sm_unit = first_unit - before;
-        break;
+  const int64_t per = units_per_worker(total, p.workers);
+#pragma unroll
+  for (int w = 0; w < S::kWorkers; ++w) {
+    const int64_t first = ((int64_t)blockIdx.x * S::kWorkers + w) * per;
+    if (first >= before && first < before + sum) {
+      int64_t from = before;
+      for (int b = b0; b < b1; ++b) {
+        const int64_t n = units_of_request(b);
+        if (first < from + n) {
+          sm_request[w] = b;
+          sm_unit[w] = first - from;
+          break;
+        }
+        from += n;
       }
-      before += n;
     }
   }
   __syncthreads();
-  int request = sm_request;
-  int64_t unit_in_request = sm_unit;
-  int64_t unit_at = first_unit;
-  int4 opened = make_int4(0, 0, 0, 0);
+  const int worker = blockIdx.x * S::kWorkers + warp / S::HW;
+  const int64_t first_unit = worker * per, last_unit = min(first_unit + per, total);
+  int left = (int)max(last_unit - first_unit, (int64_t)0);  // units still to be worked on
 
   const int row_bytes = p.dim * BITS / 8 + S::kTail;
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
@@ -313,168 +321,215 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   int fill_slot = 0, slot = 0;
   uint32_t phase = 0;
 
-  // -- item after item: a request, a cached head and a tile of its query heads
-  while (unit_at < last_unit) {
-    const int32_t length = p.lengths[request];
-    const RowSpan span = span_of(length, p.window, p.most_rows);
-    const int32_t units = units_of(span, S::UNIT);
-    const int item = (int)(unit_in_request / units);
-    const int u0 = (int)(unit_in_request - (int64_t)item * units);
-    const int u1 = (int)min((int64_t)units, u0 + (last_unit - unit_at));
-    const int kv_head = item / p.head_tiles, first_head = (item - kv_head * p.head_tiles) * S::kHeads;
-    const int heads = min(p.group - first_head, S::kHeads);  // of this tile
-    const int q_head0 = kv_head * p.group + first_head;
-    if ((length < 0 || length > p.most_rows) && tid == 0 && item == 0 && u0 == 0 &&
-        atomicCAS(p.status, 0, FBGEMM_B200_STATUS_SIZE_MISMATCH) == 0) {
-      p.status[1] = request;
-      p.status[2] = 0;
-      p.status[3] = length;
-    }
-
-    const int32_t* const table = p.tables + request * p.table_stride;
-
-    // Tile i of this warp: rows row0 + i * UNIT onwards.
-    const int64_t row0 = aligned_first(span) + ((int64_t)u0 * S::kRowWarps + row_warp) * S::ROWS;
-    const int tiles = (int)min((int64_t)(u1 - u0), row0 < span.end ? (span.end - row0 + S::UNIT - 1) / S::UNIT : 0);
-    auto report_page = [&](int64_t row, int32_t page) {
-      if (atomicCAS(p.status, 0, FBGEMM_B200_STATUS_BAD_PAGE) == 0) {
-        p.status[1] = request;
-        p.status[2] = (int32_t)row;
-        p.status[3] = page;
+  // A place in the line of units: tile u of an item (a cached head and a tile of its query heads) of a request.
+  struct Place {
+    int request, item, u, units;
+    RowSpan span;
+  };
+  auto enter = [&](Place& w, int request) {
+    w.request = request;
+    w.span = span_of(p.lengths[request], p.window, p.most_rows);
+    w.units = units_of(w.span, S::UNIT);
+  };
+  auto next_unit = [&](Place& w) {  // (the caller knows that there is one)
+    if (++w.u == w.units) {
+      w.u = 0;
+      if (++w.item == per_request) {
+        w.item = 0;
+        enter(w, w.request + 1);
       }
-    };
-    auto next_fill = [&] {
+    }
+  };
+  Place now, ahead;
+  enter(now, sm_request[warp / S::HW]);
+  now.item = (int)(sm_unit[warp / S::HW] / now.units);
+  now.u = (int)(sm_unit[warp / S::HW] - (int64_t)now.item * now.units);
+  ahead = now;
+  // Whether all of the block's units are of one item: it joins its results itself.
+  bool together = false, block_begins = false, block_ends = false;
+  if constexpr (S::kWorkers > 1) {
+    const int64_t block_first = (int64_t)blockIdx.x * S::kWorkers * per;
+    const int64_t block_units = min(block_first + S::kWorkers * per, total) - block_first;
+    const int units = units_of(span_of(p.lengths[sm_request[0]], p.window, p.most_rows), S::UNIT);
+    const int u = (int)(sm_unit[0] % units);
+    together = block_units > per && u + block_units <= units;
+    block_begins = u == 0;
+    block_ends = u + block_units == units;
+  }
+
+  // -- half tiles come in turn: K and V of a tile, then of the next.  SLOTS - 1 are on their way, and the pages of the tile
+  // behind them.
+  int to_read = left;           // tiles whose pages have not been read
+  constexpr int kPages = FAST ? SUB : 1;
+  int32_t page[kPages], page_next[kPages];  // FAST: every lane knows the pages of the steps, else those of its own row
+  int row_fill = 0, row_next = 0;           // the tile's first row
+  int head_fill = 0, head_next = 0;         // its cached head
+  unsigned seen = 0, seen_next = 0;         // its rows that the token sees
+  int request_next = 0;
+  bool fill_more = false, next_more = false;
+  int64_t off = 0;
+  auto read_pages = [&] {
+    next_more = to_read > 0;
+    if (!next_more) {
+      return;
+    }
+    const int row = aligned_first(ahead.span) + ahead.u * S::ROWS;
+    row_next = row;
+    head_next = ahead.item / p.head_tiles;
+    request_next = ahead.request;
+    seen_next = kFull;
+    if (row < ahead.span.first) {  // (by less than 16)
+      seen_next &= ~0u << (ahead.span.first - row);
+    }
+    if (ahead.span.end - row < S::ROWS) {
+      seen_next &= ahead.span.end > row ? kFull >> (S::ROWS - (ahead.span.end - row)) : 0u;
+    }
+    const int32_t* const table = p.tables + ahead.request * p.table_stride;
+#pragma unroll
+    for (int s = 0; s < kPages; ++s) {
+      const bool there = FAST ? ((seen_next >> (16 * s)) & 0xffffu) != 0 : (seen_next >> lane) & (lane < S::ROWS);
+      page_next[s] = there ? __ldg(table + ((row + (FAST ? 16 * s : lane)) >> p.page_shift)) : 0;
+    }
+    if (--to_read > 0) {
+      next_unit(ahead);
+    }
+  };
+  auto report_page = [&](int request, int row, int32_t number) {
+    if (atomicCAS(p.status, 0, FBGEMM_B200_STATUS_BAD_PAGE) == 0) {
+      p.status[1] = request;
+      p.status[2] = row;
+      p.status[3] = number;
+    }
+  };
+  auto next_tile = [&] {
+    fill_more = next_more;
+    if (!fill_more) {
+      return;
+    }
+    row_fill = row_next;
+    head_fill = head_next;
+    seen = seen_next;
+#pragma unroll
+    for (int s = 0; s < kPages; ++s) {
+      page[s] = page_next[s];
+    }
+    if constexpr (FAST) {
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) {
+        if ((uint32_t)page[s] >= (uint32_t)p.num_pages) {
+          const unsigned lost = (seen >> (16 * s)) & 0xffffu;
+          if (lane == 0 && lost) {
+            report_page(request_next, row_fill + 16 * s + __ffs(lost) - 1, page[s]);
+          }
+          seen &= ~(0xffffu << (16 * s));
+        }
+      }
+    } else {
+      const bool there = lane < S::ROWS && ((seen >> (lane & 31)) & 1);
+      const bool good = there && (uint32_t)page[0] < (uint32_t)p.num_pages;
+      if (there && !good) {
+        report_page(request_next, row_fill + lane, page[0]);
+      }
+      seen = __ballot_sync(kAll, good);
+      off = good ? page[0] * p.page_stride + ((row_fill + lane) & ((1 << p.page_shift) - 1)) * p.slot_stride : 0;
+    }
+    read_pages();
+  };
+  auto fill = [&](bool is_v) {
+    if (!is_v) {
+      next_tile();
+    }
+    if (fill_more) {
+      if constexpr (FAST) {
+        if (lane == 0) {
+          sm_seen[warp][fill_slot] = seen;
+          const uint32_t bar = bars + 8 * fill_slot;
+          const int first = row_fill & ((1 << p.page_shift) - 1);
+          int steps = 0;
+#pragma unroll
+          for (int s = 0; s < SUB; ++s) {
+            steps += ((seen >> (16 * s)) & 0xffffu) != 0;
+          }
+          barrier_expect(bar, steps * (S::kBoxes * S::kBoxBytes));
+#pragma unroll
+          for (int s = 0; s < SUB; ++s) {
+            if ((seen >> (16 * s)) & 0xffffu) {
+#pragma unroll
+              for (int x = 0; x < S::kBoxes; ++x) {
+                copy_box(fill_at + (s * S::kBoxes + x) * S::kBoxBytes, is_v ? &v_map : &k_map, 64 * x, head_fill,
+                         (first + 16 * s) & ((1 << p.page_shift) - 1), page[s], bar);
+              }
+            }
+          }
+        }
+      } else {
+        if (lane == 0) {
+          sm_seen[warp][fill_slot] = seen;
+        }
+        const uint8_t* const rows = (is_v ? p.v : p.k) + head_fill * p.head_stride;
+        if (p.aligned) {
+          constexpr int kRounds = (S::ROWS * S::kPieces + 31) / 32;
+#pragma unroll 4
+          for (int j = 0; j < kRounds; ++j) {
+            const int n = lane + 32 * j, r = n / S::kPieces, piece = n - r * S::kPieces;
+            const int64_t row = __shfl_sync(kAll, off, min(r, S::ROWS - 1));
+            if (r < S::ROWS) {  // (pieces behind the row's: zeros)
+              copy16(fill_at + r * S::PITCH + piece * 16, rows + row + (piece * 16 < row_bytes ? piece * 16 : 0),
+                     ((seen >> r) & 1) && piece * 16 < row_bytes ? 16 : 0);
+            }
+          }
+        } else if (lane < S::ROWS) {
+          const uint32_t bytes = (seen >> lane) & 1 ? 4 : 0;
+          for (int n = 0; n < row_bytes; n += 4) {
+            copy4(fill_at + lane * S::PITCH + n, rows + off + n, bytes);
+          }
+        }
+      }
       fill_at += kSlot;
       ++fill_slot;
       if (fill_at == ring_end) {
         fill_at = ring_at;
         fill_slot = 0;
       }
-    };
-
-    // -- half tiles come in turn: K and V of a tile, then of the next.  SLOTS - 1 are on their way.
-    int fill_tile = -1;
-    unsigned seen = 0;  // rows of the tile that is filled that the token sees
-    // FAST: every lane knows the pages of the steps.  Otherwise a lane looks after one row.
-    constexpr int kPages = FAST ? SUB : 1;
-    int32_t page[kPages], page_next[kPages], page_after[kPages];
-    int64_t off = 0;
-    auto read_page = [&](int i, int s) {
-      const int64_t row = row0 + (int64_t)i * S::UNIT + (FAST ? 16 * s : lane);
-      const bool there = i < tiles && row < span.end && (FAST || (lane < S::ROWS && row >= span.first));
-      return there ? __ldg(table + (row >> p.page_shift)) : 0;
-    };
-#pragma unroll
-    for (int s = 0; s < kPages; ++s) {
-      page_next[s] = read_page(0, s);
-      page_after[s] = read_page(1, s);
     }
-    auto next_tile = [&] {
-      ++fill_tile;
-      const int64_t row = row0 + (int64_t)fill_tile * S::UNIT;
+    if constexpr (!FAST) {
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
+  // The half tile that is worked on next is there, and the one before has been read by all lanes.
+  auto arrived = [&] {
+    if constexpr (FAST) {
+      if (!barrier_wait(bars + 8 * slot, phase) && atomicCAS(p.status, 0, FBGEMM_B200_STATUS_COPY_TIMEOUT) == 0) {
+        p.status[1] = now.request;
+      }
+    } else {
+      asm volatile("cp.async.wait_group %0;" ::"n"(S::SLOTS - 2) : "memory");
+    }
+    __syncwarp();
+  };
+  read_pages();
 #pragma unroll
-      for (int s = 0; s < kPages; ++s) {
-        page[s] = page_next[s];
-        page_next[s] = page_after[s];
-        page_after[s] = read_page(fill_tile + 2, s);
+  for (int h = 0; h < S::SLOTS - 1; ++h) {
+    fill(h & 1);
+  }
+  int4 opened = make_int4(0, 0, 0, 0);
+
+  // -- item after item
+  while (left > 0) {
+    const int request = now.request, item = now.item;
+    const bool begins = now.u == 0, ends = now.units - now.u <= left, none = now.span.end == now.span.first;
+    const int tiles = ends ? now.units - now.u : left;
+    const int kv_head = item / p.head_tiles, first_head = (item - kv_head * p.head_tiles) * S::kHeads + head_warp * S::kWarpHeads;
+    const int heads = min(p.group - first_head, S::kWarpHeads);  // of this warp, may be none
+    const int q_head0 = kv_head * p.group + first_head;
+    if (begins && item == 0 && head_warp == 0 && lane == 0) {
+      const int32_t length = p.lengths[request];
+      if ((length < 0 || length > p.most_rows) && atomicCAS(p.status, 0, FBGEMM_B200_STATUS_SIZE_MISMATCH) == 0) {
+        p.status[1] = request;
+        p.status[2] = 0;
+        p.status[3] = length;
       }
-      if (fill_tile >= tiles) {
-        return;
-      }
-      if constexpr (FAST) {
-        seen = kFull;
-        if (row < span.first) {  // (by less than 16)
-          seen &= ~0u << (span.first - row);
-        }
-        if (row + S::ROWS > span.end) {
-          seen &= kFull >> (row + S::ROWS - span.end);
-        }
-#pragma unroll
-        for (int s = 0; s < SUB; ++s) {
-          if ((uint32_t)page[s] >= (uint32_t)p.num_pages) {
-            if (lane == 0 && ((seen >> (16 * s)) & 0xffffu)) {
-              report_page(row + 16 * s + (s == 0 && row < span.first ? span.first - row : 0), page[s]);
-            }
-            seen &= ~(0xffffu << (16 * s));
-          }
-        }
-      } else {
-        const bool there = lane < S::ROWS && row + lane < span.end && row + lane >= span.first;
-        const bool good = there && (uint32_t)page[0] < (uint32_t)p.num_pages;
-        if (there && !good) {
-          report_page(row + lane, page[0]);
-        }
-        seen = __ballot_sync(kAll, good);
-        off = good ? page[0] * p.page_stride + ((row + lane) & ((1 << p.page_shift) - 1)) * p.slot_stride : 0;
-      }
-    };
-    auto fill = [&](bool is_v) {
-      if (!is_v) {
-        next_tile();
-      }
-      if (fill_tile < tiles) {
-        if constexpr (FAST) {
-          if (lane == 0) {
-            sm_seen[warp][fill_slot] = seen;
-            const int row = (int)((row0 + (int64_t)fill_tile * S::UNIT) & ((1 << p.page_shift) - 1));
-            const uint32_t bar = bars + 8 * fill_slot;
-            int steps = 0;
-#pragma unroll
-            for (int s = 0; s < SUB; ++s) {
-              steps += ((seen >> (16 * s)) & 0xffffu) != 0;
-            }
-            barrier_expect(bar, steps * (S::kBoxes * S::kBoxBytes));
-#pragma unroll
-            for (int s = 0; s < SUB; ++s) {
-              if ((seen >> (16 * s)) & 0xffffu) {
-#pragma unroll
-                for (int x = 0; x < S::kBoxes; ++x) {
-                  copy_box(fill_at + (s * S::kBoxes + x) * S::kBoxBytes, is_v ? &v_map : &k_map, 64 * x, kv_head,
-                           (row + 16 * s) & ((1 << p.page_shift) - 1), page[s], bar);
-                }
-              }
-            }
-          }
-        } else {
-          if (lane == 0) {
-            sm_seen[warp][fill_slot] = seen;
-          }
-          const uint8_t* const rows = (is_v ? p.v : p.k) + kv_head * p.head_stride;
-          if (p.aligned) {
-            constexpr int kRounds = (S::ROWS * S::kPieces + 31) / 32;
-#pragma unroll 4
-            for (int j = 0; j < kRounds; ++j) {
-              const int n = lane + 32 * j, r = n / S::kPieces, piece = n - r * S::kPieces;
-              const int64_t row = __shfl_sync(kAll, off, min(r, S::ROWS - 1));
-              if (r < S::ROWS) {  // (pieces behind the row's: zeros)
-                copy16(fill_at + r * S::PITCH + piece * 16, rows + row + (piece * 16 < row_bytes ? piece * 16 : 0),
-                       ((seen >> r) & 1) && piece * 16 < row_bytes ? 16 : 0);
-              }
-            }
-          } else if (lane < S::ROWS) {
-            const uint32_t bytes = (seen >> lane) & 1 ? 4 : 0;
-            for (int n = 0; n < row_bytes; n += 4) {
-              copy4(fill_at + lane * S::PITCH + n, rows + off + n, bytes);
-            }
-          }
-        }
-        next_fill();
-      }
-      if constexpr (!FAST) {
-        asm volatile("cp.async.commit_group;" ::: "memory");
-      }
-    };
-    // The half tile that is worked on next is there, and the one before has been read by all lanes.
-    auto arrived = [&] {
-      if constexpr (FAST) {
-        if (!barrier_wait(bars + 8 * slot, phase) && atomicCAS(p.status, 0, FBGEMM_B200_STATUS_COPY_TIMEOUT) == 0) {
-          p.status[1] = request;
-        }
-      } else {
-        asm volatile("cp.async.wait_group %0;" ::"n"(S::SLOTS - 2) : "memory");
-      }
-      __syncwarp();
-    };
+    }
 
     // -- queries as the products take them: head g of a tile in lanes 4g .. 4g + 3, columns in the order of K's registers.
     // Columns of 16 bits: 2c, 2c + 1 and 2c + 8, 2c + 9 of a step of 16.  8-bit codes: 4c .. 4c + 3 of a step.  4-bit codes:
@@ -482,9 +537,9 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     uint32_t qf[NT][S::KSTEPS][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int head = head_warp * S::kWarpHeads + 8 * n + g;
+      const int head = 8 * n + g;
       const bool there = head < heads;
-      const uint8_t* q = p.q + request * p.q_token + (q_head0 + (there ? head : 0)) * p.q_head;
+      const uint8_t* q = p.q + request * p.q_token + (there ? q_head0 + head : 0) * p.q_head;
       if constexpr (BITS == 4) {
 #pragma unroll
         for (int k = 0; k < S::KSTEPS; k += 2) {
@@ -509,10 +564,6 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
           }
         }
       }
-    }
-#pragma unroll
-    for (int h = 0; h < S::SLOTS - 1; ++h) {
-      fill(h & 1);
     }
 
     float factor[NT][2], q_sum[NT][2];  // heads 2c and 2c + 1
@@ -851,17 +902,14 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
       advance();
     }
 
-    // -- the warps' results together, where the rings were
-    if constexpr (!FAST) {
-      asm volatile("cp.async.wait_all;" ::: "memory");
-    }
-    __syncthreads();
+    // -- this warp's result: whole, or a part of one
+    float scale_l[NT][2], scale_o[NT][2], add_o[NT][2];
+    const bool whole = begins && ends;  // (never if the block joins its results)
+    const float unit = kQuantized ? __uint_as_float((uint32_t)exponent << 23) : 1.f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const int h = head_warp * S::kWarpHeads + 8 * n + 2 * c + x;
-        const float unit = kQuantized ? __uint_as_float((uint32_t)exponent << 23) : 1.f;
         float sum_l = l[n][x], sum_b = 0.f;
         if constexpr (kQuantized) {
           sum_b = __fmaf_rn(__fmul_rn(w_sum[n][x], unit), -kMiddle, bias_sum[n][x]);
@@ -873,59 +921,121 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
             sum_b += __shfl_xor_sync(kAll, sum_b, d);
           }
         }
-        if (g == 0) {
-          sm_m[row_warp][h] = m[n][x];
-          sm_l[row_warp][h] = sum_l;
+        const float inv = !whole ? 1.f : none ? 0.f : __fdiv_rn(1.f, sum_l);  // no row at all: zeros
+        scale_l[n][x] = sum_l;
+        scale_o[n][x] = inv;
+        add_o[n][x] = sum_b;
+      }
+    }
+    float* const part = whole      ? nullptr
+                        : together ? reinterpret_cast<float*>(smem) + (warp / S::HW) * S::kPartFloats
+                                   : p.parts + (2 * (int64_t)worker + begins) * S::kPartFloats;
+    if (together) {
+      __syncthreads();  // (all rings have been read)
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int h = 8 * n + 2 * c + x;
+        if (h >= heads) {
+          continue;
         }
-        float* const to = sm_o + (row_warp * S::kHeads + h) * S::HP;
+        const int64_t row = (int64_t)request * p.kv_heads * p.group + q_head0 + h;
+        const int in_part = head_warp * S::kWarpHeads + h;
+        if (g == 0) {
+          if (!whole) {
+            part[in_part] = m[n][x];
+            part[S::kHeads + in_part] = scale_l[n][x];
+          } else if (p.lse) {
+            const float from = m[n][x] == -INFINITY ? 0.f : m[n][x];
+            p.lse[row] = none ? -INFINITY : __fmaf_rn(from, kLn2, logf(__fmul_rn(scale_l[n][x], kUnshift)));
+          }
+        }
+        uint16_t* const out = static_cast<uint16_t*>(p.out) + row * p.dim;
+        float* const to = part + 2 * S::kHeads + in_part * S::DP;
 #pragma unroll
         for (int t = 0; t < S::MT; ++t) {
-          float2 v = make_float2(o[n][t][x], o[n][t][2 + x]);
-          if constexpr (BITS == 16) {
-            to[16 * t + g] = v.x;
-            to[16 * t + 8 + g] = v.y;
+          float a = o[n][t][x], b = o[n][t][2 + x];
+          if constexpr (kQuantized) {
+            a = __fmaf_rn(__fmul_rn(a, 1.f / kCode), unit, add_o[n][x]);
+            b = __fmaf_rn(__fmul_rn(b, 1.f / kCode), unit, add_o[n][x]);
+          }
+          // 16-bit rows: columns g and g + 8 of a step of 16; quantized ones: two columns side by side
+          const int column = BITS == 16 ? 16 * t + g : BITS == 8 ? 16 * t + 2 * g : 32 * (t / 2) + 4 * g + 2 * (t % 2);
+          if (whole) {
+            if (column < p.dim) {
+              const uint32_t r = pack<BF16>(__fmul_rn(a, scale_o[n][x]), __fmul_rn(b, scale_o[n][x]));
+              if constexpr (BITS == 16) {
+                out[column] = (uint16_t)r;
+                out[column + 8] = (uint16_t)(r >> 16);
+              } else {
+                *reinterpret_cast<uint32_t*>(out + column) = r;
+              }
+            }
+          } else if constexpr (BITS == 16) {
+            to[column] = a;
+            to[column + 8] = b;
           } else {
-            v.x = __fmaf_rn(__fmul_rn(v.x, 1.f / kCode), unit, sum_b);
-            v.y = __fmaf_rn(__fmul_rn(v.y, 1.f / kCode), unit, sum_b);
-            *reinterpret_cast<float2*>(to + (BITS == 8 ? 16 * t + 2 * g : 32 * (t / 2) + 4 * g + 2 * (t % 2))) = v;
+            *reinterpret_cast<float2*>(to + column) = make_float2(a, b);
           }
         }
       }
     }
+    if (begins && !ends && !(together && block_ends)) {  // others end what this worker began: it names them
+      const int64_t last = last_unit - left + now.units - 1;
+      opened = make_int4((int)(last / per - worker), request, item, 0);
+    }
+    left -= tiles;
+    if (left > 0) {
+      now.u += tiles - 1;
+      next_unit(now);
+    }
+  }
+  if (p.open && head_warp == 0 && lane == 0) {
+    p.open[worker] = opened;
+  }
+  if (together) {
+    const bool idle = first_unit >= total;  // (an idle warp has met no barrier yet)
+    if (idle) {
+      __syncthreads();
+    }
     __syncthreads();
-    const bool whole = u0 == 0 && u1 == units;
-    const bool none = span.end == span.first;
-    float* const part = whole ? nullptr : p.parts + (2 * (int64_t)blockIdx.x + (u0 == 0)) * S::kPartFloats;
+    const int active = (int)min((total - (int64_t)blockIdx.x * S::kWorkers * per + per - 1) / per, (int64_t)S::kWorkers);
+    const float* const parts = reinterpret_cast<const float*>(smem);
+    const int item = (int)(sm_unit[0] / units_of(span_of(p.lengths[sm_request[0]], p.window, p.most_rows), S::UNIT));
+    const int kv_head = item / p.head_tiles, first_head = (item - kv_head * p.head_tiles) * S::kHeads;
+    const int heads = min(p.group - first_head, S::kHeads);
+    const bool whole = block_begins && block_ends;
+    float* const part = p.parts + (2 * (int64_t)blockIdx.x * S::kWorkers + block_begins) * S::kPartFloats;
     for (int n = tid; n < heads * (S::DP / 4); n += kThreads) {
       const int h = n / (S::DP / 4), column = n % (S::DP / 4) * 4;
       float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < S::kRowWarps; ++w) {
-        top = fmaxf(top, sm_m[w][h]);
+      for (int w = 0; w < active; ++w) {
+        top = fmaxf(top, parts[w * S::kPartFloats + h]);
       }
       const float from = top == -INFINITY ? 0.f : top;
       float sum_l = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < S::kRowWarps; ++w) {
-        const float f = exp2_of(sm_m[w][h] - from);
-        const float4 x = *reinterpret_cast<const float4*>(sm_o + (w * S::kHeads + h) * S::HP + column);
-        sum_l = __fmaf_rn(f, sm_l[w][h], sum_l);
+      for (int w = 0; w < active; ++w) {
+        const float f = exp2_of(parts[w * S::kPartFloats + h] - from);
+        const float4 x = *reinterpret_cast<const float4*>(parts + w * S::kPartFloats + 2 * S::kHeads + h * S::DP + column);
+        sum_l = __fmaf_rn(f, parts[w * S::kPartFloats + S::kHeads + h], sum_l);
         v.x = __fmaf_rn(f, x.x, v.x);
         v.y = __fmaf_rn(f, x.y, v.y);
         v.z = __fmaf_rn(f, x.z, v.z);
         v.w = __fmaf_rn(f, x.w, v.w);
       }
       if (whole) {
-        const float inv = none ? 0.f : __fdiv_rn(1.f, sum_l);  // no row at all: zeros
-        const int64_t row = (int64_t)request * p.kv_heads * p.group + q_head0 + h;
+        const float inv = __fdiv_rn(1.f, sum_l);
+        const int64_t row = ((int64_t)sm_request[0] * p.kv_heads + kv_head) * p.group + first_head + h;
         if (column < p.dim) {
-          const uint2 r = make_uint2(pack<BF16>(__fmul_rn(v.x, inv), __fmul_rn(v.y, inv)),
-                                     pack<BF16>(__fmul_rn(v.z, inv), __fmul_rn(v.w, inv)));
-          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + (row * p.dim + column) * 2) = r;
+          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + (row * p.dim + column) * 2) =
+              make_uint2(pack<BF16>(__fmul_rn(v.x, inv), __fmul_rn(v.y, inv)),
+                         pack<BF16>(__fmul_rn(v.z, inv), __fmul_rn(v.w, inv)));
         }
         if (column == 0 && p.lse) {
-          p.lse[row] = none ? -INFINITY : __fmaf_rn(from, kLn2, logf(__fmul_rn(sum_l, kUnshift)));
+          p.lse[row] = __fmaf_rn(from, kLn2, logf(__fmul_rn(sum_l, kUnshift)));
         }
       } else {
         *reinterpret_cast<float4*>(part + 2 * S::kHeads + h * S::DP + column) = v;
@@ -935,102 +1045,113 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
         }
       }
     }
-    if (u0 == 0 && u1 < units) {  // others end what this worker began: it names them
-      const int64_t end = unit_at + units;
-      opened = make_int4((int)((end - 1) / per - blockIdx.x), request, item, 0);
+    if (!whole) {  // the other workers' parts: nothing
+      for (int n = tid; n < (active - 1) * S::kHeads; n += kThreads) {
+        float* const other = p.parts + 2 * ((int64_t)blockIdx.x * S::kWorkers + 1 + n / S::kHeads) * S::kPartFloats;
+        other[n % S::kHeads] = -INFINITY;
+        other[S::kHeads + n % S::kHeads] = 0.f;
+      }
     }
-    unit_at += u1 - u0;
-    unit_in_request += u1 - u0;
-    if (unit_in_request == (int64_t)units * per_request) {
-      ++request;
-      unit_in_request = 0;
-    }
-    if constexpr (FAST) {
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
-    __syncthreads();  // (the rings are filled again)
-  }
-  if (tid == 0 && p.open) {
-    p.open[blockIdx.x] = opened;
   }
 }
 
-// One block per worker and query head of a tile: the item that the worker began, if others end it.
+// A block looks after a few workers, one after the other: if others end the item that a worker began, its parts are added
+// up, the heads by the blocks of the grid's second dimension and the groups of kJoinTeam warps, the parts by the warps of
+// a group.
 template <typename S, bool BF16>
-__global__ void __launch_bounds__(kThreads) paged_attention_join(const PagedAttentionParams p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  __shared__ float sm_o[kWarps][S::DP];
-  __shared__ float sm_l[kWarps];
-  __shared__ float sm_m[kWarps];
-  const int4 opened = p.open[blockIdx.x];
-  const int kv_head = opened.z / p.head_tiles, first_head = (opened.z - kv_head * p.head_tiles) * S::kHeads;
-  const int h = blockIdx.y;
-  if (opened.x == 0 || h >= p.group - first_head) {
-    return;
-  }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = opened.x + 1;
-  auto part_of = [&](int i) {  // what the worker began, then what the next ones ended
-    return p.parts + (2 * ((int64_t)blockIdx.x + i) + (i == 0)) * S::kPartFloats;
-  };
-  float top = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    top = fmaxf(top, part_of(i)[h]);
-  }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    top = fmaxf(top, __shfl_xor_sync(kAll, top, d));
-  }
-  if (lane == 0) {
-    sm_m[warp] = top;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    top = fmaxf(top, sm_m[w]);
-  }
-  const float base = top == -INFINITY ? 0.f : top;
+__global__ void __launch_bounds__(kJoinThreads) paged_attention_join(const PagedAttentionParams p) {
+  constexpr int kTeams = kJoinThreads / 32 / kJoinTeam;
   constexpr int kCols = S::DP / 32;
-  float v[kCols], sum_l = 0.f;
+  __shared__ float sm_o[kTeams][kJoinTeam][S::DP];
+  __shared__ float sm_m[kTeams][kJoinTeam], sm_l[kTeams][kJoinTeam];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = warp / kJoinTeam, mate = warp % kJoinTeam;
+  for (int worker = blockIdx.x; worker < p.workers; worker += gridDim.x) {
+    const int4 opened = p.open[worker];
+    if (opened.x == 0) {
+      continue;
+    }
+    const int kv_head = opened.z / p.head_tiles, first_head = (opened.z - kv_head * p.head_tiles) * S::kHeads;
+    const int heads = min(p.group - first_head, S::kHeads);
+    const int n = opened.x + 1;
+    auto part_of = [&](int i) {  // what the worker began, then what the next ones ended
+      return p.parts + (2 * ((int64_t)worker + i) + (i == 0)) * S::kPartFloats;
+    };
+    for (int h0 = blockIdx.y * kTeams; h0 < heads; h0 += gridDim.y * kTeams) {
+      const int h = h0 + team;
+      float v[kCols], sum_l = 0.f, top = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < kCols; ++j) {
-    v[j] = 0.f;
-  }
+      for (int j = 0; j < kCols; ++j) {
+        v[j] = 0.f;
+      }
+      if (h < heads) {
+        for (int i = mate + kJoinTeam * lane; i < n; i += kJoinTeam * 32) {
+          top = fmaxf(top, part_of(i)[h]);
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+          top = fmaxf(top, __shfl_xor_sync(kAll, top, d));
+        }
+        const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll 4
-  for (int i = warp; i < n; i += kWarps) {
-    const float* part = part_of(i);
-    const float f = exp2_of(part[h] - base);
-    sum_l = __fmaf_rn(f, part[S::kHeads + h], sum_l);
+        for (int i = mate; i < n; i += kJoinTeam) {
+          const float* part = part_of(i);
+          const float m = part[h];
+          if (m == -INFINITY && part[S::kHeads + h] == 0.f) {
+            continue;
+          }
+          const float f = exp2_of(m - base);
+          sum_l = __fmaf_rn(f, part[S::kHeads + h], sum_l);
 #pragma unroll
-    for (int j = 0; j < kCols; j += 2) {
-      const float2 x = *reinterpret_cast<const float2*>(part + 2 * S::kHeads + h * S::DP + 32 * j + 2 * lane);
-      v[j] = __fmaf_rn(f, x.x, v[j]);
-      v[j + 1] = __fmaf_rn(f, x.y, v[j + 1]);
+          for (int j = 0; j < kCols; j += 2) {
+            const float2 x = *reinterpret_cast<const float2*>(part + 2 * S::kHeads + h * S::DP + 32 * j + 2 * lane);
+            v[j] = __fmaf_rn(f, x.x, v[j]);
+            v[j + 1] = __fmaf_rn(f, x.y, v[j + 1]);
+          }
+        }
+      }
+      if (lane == 0) {
+        sm_m[team][mate] = top;
+        sm_l[team][mate] = sum_l;
+      }
+#pragma unroll
+      for (int j = 0; j < kCols; j += 2) {
+        *reinterpret_cast<float2*>(&sm_o[team][mate][32 * j + 2 * lane]) = make_float2(v[j], v[j + 1]);
+      }
+      __syncthreads();
+      if (h < heads && mate == 0) {
+        float all = -INFINITY, total = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinTeam; ++w) {
+          all = fmaxf(all, sm_m[team][w]);
+        }
+        const float base = all == -INFINITY ? 0.f : all;
+        float f[kJoinTeam];
+#pragma unroll
+        for (int w = 0; w < kJoinTeam; ++w) {
+          // (a warp without parts: 0; one whose parts' scores are all -inf adds its sum of 0)
+          f[w] = exp2_of(sm_m[team][w] - base);
+          total = __fmaf_rn(f[w], sm_l[team][w], total);
+        }
+        const int64_t row = ((int64_t)opened.y * p.kv_heads + kv_head) * p.group + first_head + h;
+        const float inv = __fdiv_rn(1.f, total);
+        for (int column = 2 * lane; column < p.dim; column += 64) {
+          float a = 0.f, b = 0.f;
+#pragma unroll
+          for (int w = 0; w < kJoinTeam; ++w) {
+            const float2 x = *reinterpret_cast<const float2*>(&sm_o[team][w][column]);
+            a = __fmaf_rn(f[w], x.x, a);
+            b = __fmaf_rn(f[w], x.y, b);
+          }
+          *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.out) + (row * p.dim + column) * 2) =
+              pack<BF16>(__fmul_rn(a, inv), __fmul_rn(b, inv));
+        }
+        if (lane == 0 && p.lse) {
+          p.lse[row] = __fmaf_rn(base, kLn2, logf(__fmul_rn(total, kUnshift)));
+        }
+      }
+      __syncthreads();
     }
-  }
-#pragma unroll
-  for (int j = 0; j < kCols; j += 2) {
-    *reinterpret_cast<float2*>(&sm_o[warp][32 * j + 2 * lane]) = make_float2(v[j], v[j + 1]);
-  }
-  if (lane == 0) {
-    sm_l[warp] = sum_l;
-  }
-  __syncthreads();
-  sum_l = sm_l[0] + sm_l[1] + sm_l[2] + sm_l[3];
-  const int64_t row = (int64_t)opened.y * p.kv_heads * p.group + kv_head * p.group + first_head + h;
-  const float inv = __fdiv_rn(1.f, sum_l);
-  for (int column = 2 * threadIdx.x; column < p.dim; column += 2 * kThreads) {
-    float a = 0.f, b = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      a += sm_o[w][column];
-      b += sm_o[w][column + 1];
-    }
-    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.out) + (row * p.dim + column) * 2) =
-        pack<BF16>(__fmul_rn(a, inv), __fmul_rn(b, inv));
-  }
-  if (threadIdx.x == 0 && p.lse) {
-    p.lse[row] = __fmaf_rn(base, kLn2, logf(__fmul_rn(sum_l, kUnshift)));
   }
 }
 
@@ -1042,7 +1163,9 @@ PagedAttentionPlan plan_of(int group, int64_t sms) {
   r.unit = S::UNIT;
   r.tile_heads = S::kHeads;
   r.head_tiles = (group + S::kHeads - 1) / S::kHeads;
-  r.workers = (int32_t)(sms * S::kBlocks);
+  r.blocks = (int32_t)(sms * S::kBlocks);
+  r.workers = r.blocks * S::kWorkers;
+  r.joiners = (int32_t)(2 * sms);
   r.part_floats = S::kPartFloats;
   return r;
 }
@@ -1075,21 +1198,25 @@ cudaError_t launch_of(const PagedAttentionPlan& plan, const PagedAttentionParams
   if (e != cudaSuccess) {
     return e;
   }
-  paged_attention_kernel<S, BF16, FAST><<<(unsigned)plan.workers, kThreads, S::kShared, stream>>>(p, maps[0], maps[1]);
+  // Blocks come to their SM while the launch before ends, and wait there for its results.
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)plan.blocks);
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = S::kShared;
+  config.stream = stream;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  e = cudaLaunchKernelEx(&config, paged_attention_kernel<S, BF16, FAST>, p, maps[0], maps[1]);
   g_launch_count.fetch_add(1, std::memory_order_relaxed);
-  e = cudaGetLastError();
   if (e != cudaSuccess || !split) {
     return e;
   }
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)plan.workers, (unsigned)(p.group < S::kHeads ? p.group : S::kHeads));
-  config.blockDim = dim3(kThreads);
-  config.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its blocks wait for the first launch themselves
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &attr;
-  config.numAttrs = 1;
+  config.gridDim = dim3((unsigned)plan.joiners, 4);
+  config.blockDim = dim3(kJoinThreads);
+  config.dynamicSmemBytes = 0;
   e = cudaLaunchKernelEx(&config, paged_attention_join<S, BF16>, p);
   g_launch_count.fetch_add(1, std::memory_order_relaxed);
   return e;

@@ -21,8 +21,8 @@ namespace fbgemm_b200 {
 //
 // A request's rows are cut into units of `unit` rows, the last one short; every (request, cached head, head tile) has
 // units_of() of them, at least one, so that a request without rows is somebody's too.  All units stand in one line,
-// request after request, head after head, and each worker (a block) takes the same number of neighbours: the chip is
-// filled whatever the lengths are, long requests are split, short ones share a worker.
+// request after request, head after head, and each worker (a warp, or several that share rows) takes the same number of
+// neighbours: the chip is filled whatever the lengths are, long requests are split, short ones share a worker.
 
 // Rows [first, end) that a request's new token sees: `length` rows in the cache, the last `window` of them (0: all).
 struct RowSpan {
@@ -120,7 +120,9 @@ struct PagedAttentionPlan {
   int32_t unit;        // rows per unit
   int32_t tile_heads;  // query heads of a tile
   int32_t head_tiles;
+  int32_t blocks;
   int32_t workers;
+  int32_t joiners;
   size_t part_floats;  // of one partial result
 };
 PagedAttentionPlan plan_paged_attention(const PagedAttentionShape& s, int64_t sms);
