@@ -111,6 +111,9 @@ int64_t workspace_bytes_of(const PagedAttentionPlan& plan) {
   return (int64_t)plan.workers * (2 * (int64_t)plan.part_floats * 4 + 16);
 }
 
+// Rows up to which an item is left to one block.
+constexpr int64_t kShortItem = 512;
+
 int check_heads(const fbgemm_b200_paged_cache& c, int32_t q_heads) {
   return q_heads >= 1 && q_heads <= 16384 && q_heads % c.kv_heads == 0
       ? 0
@@ -345,9 +348,14 @@ int fbgemm_b200_paged_attention(
   const PagedAttentionShape shape = shape_of(*cache, q_heads, dtype);
   DeviceGuard guard(ctx->device);
   const PagedAttentionPlan plan = plan_paged_attention(shape, sm_count());
+  if ((int64_t)batch * cache->kv_heads * plan.head_tiles > 0x7fffffffLL) {
+    return refuse("paged_attention: 2^31 heads of all requests or more");
+  }
   const int64_t most = (int64_t)width * cache->page_size;
   const int64_t span = window > 0 && window < most ? window : most;
-  const bool split = span + (window > 0 ? 15 : 0) > plan.unit;  // (items of one unit have one worker)
+  // Short items are a block's each: one launch, no workspace.  Longer ones are split over the chip.
+  const bool short_items = span <= kShortItem;
+  const bool split = !short_items;
   if (split && (!workspace || !aligned(workspace, 16) || workspace_bytes < workspace_bytes_of(plan))) {
     return refuse("paged_attention: workspace missing, unaligned or too small (fbgemm_b200_paged_attention_workspace)");
   }
@@ -382,6 +390,7 @@ int fbgemm_b200_paged_attention(
   p.window = window;
   p.workers = plan.workers;
   p.aligned = rows_aligned(*cache);
+  p.block_per_item = short_items;
   const cudaError_t e = launch_paged_attention(shape, plan, p, split, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? 0 : fail_cuda(e, "paged_attention launch");
 } catch (...) {

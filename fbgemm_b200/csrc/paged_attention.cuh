@@ -60,7 +60,7 @@ namespace paged {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kJoinThreads = 256, kJoinTeam = 4;
+
 // Weights are 2^kShift times as large as in the formula and at most 2^kSlack above their reference: 2^14 at most, and with
 // a scale of less than 2 below 2^15.
 constexpr float kShift = 10.f, kSlack = 4.f;
@@ -162,9 +162,16 @@ __device__ __forceinline__ void copy_box(uint32_t to, const CUtensorMap* map, in
       : "memory");
 }
 
-// Nibbles i and i + 4 of a word as subnormal fp16.
+// Nibbles i and i + 4 of a word as subnormal fp16, c 2^-20.  (The even ones by a product: the units for shifts and masks
+// are the busier ones.)
 __device__ __forceinline__ uint32_t nibbles(uint32_t w, int i) {
-  return (i == 0 ? w << 4 : w >> (4 * i - 4)) & 0x00f000f0u;
+  const uint32_t x = i < 2 ? w : w >> 8;
+  if (i % 2 == 1) {
+    return x & 0x00f000f0u;
+  }
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x & 0x000f000fu), "r"(0x4c004c00u));  // times 16
+  return r;
 }
 
 __device__ __forceinline__ float2 halves(uint32_t w) {
@@ -241,9 +248,26 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   if (FAST && tid < 2) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(tid ? &v_map : &k_map) : "memory");
   }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // The join may come to its SMs from here on; what it reads before it waits for this launch (the lengths) was there by now.
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
+  int left;                         // units still to be worked on
+  int64_t last_unit = 0, per = 1;
+  int64_t total = 0;
+  const int worker = blockIdx.x * S::kWorkers + warp / S::HW;
+  if (p.block_per_item) {
+    // -- a block takes an item, its workers equal shares of it
+    const int request = blockIdx.x / per_request;
+    const int units = units_of(span_of(p.lengths[request], p.window, p.most_rows), S::UNIT);
+    const int share = (units + S::kWorkers - 1) / S::kWorkers, first = share * (warp / S::HW);
+    left = max(min(share, units - first), 0);
+    if (tid < S::kWorkers) {
+      sm_request[tid] = request;
+      sm_unit[tid] = (int64_t)(blockIdx.x - request * per_request) * units + share * tid;
+    }
+    __syncthreads();
+  } else {
   // -- the units of this block's workers, and the requests that their first ones belong to
   const int chunk = (p.batch + kThreads - 1) / kThreads;
   const int b0 = min(tid * chunk, p.batch), b1 = min(b0 + chunk, p.batch);
@@ -269,13 +293,12 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   }
   __syncthreads();
   before -= sum;
-  int64_t total = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     before += w < warp ? sm_sums[w] : 0;
     total += sm_sums[w];
   }
-  const int64_t per = units_per_worker(total, p.workers);
+  per = units_per_worker(total, p.workers);
 #pragma unroll
   for (int w = 0; w < S::kWorkers; ++w) {
     const int64_t first = ((int64_t)blockIdx.x * S::kWorkers + w) * per;
@@ -293,9 +316,10 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     }
   }
   __syncthreads();
-  const int worker = blockIdx.x * S::kWorkers + warp / S::HW;
-  const int64_t first_unit = worker * per, last_unit = min(first_unit + per, total);
-  int left = (int)max(last_unit - first_unit, (int64_t)0);  // units still to be worked on
+  const int64_t first_unit = worker * per;
+  last_unit = min(first_unit + per, total);
+  left = (int)max(last_unit - first_unit, (int64_t)0);
+  }
 
   const int row_bytes = p.dim * BITS / 8 + S::kTail;
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
@@ -347,7 +371,9 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   ahead = now;
   // Whether all of the block's units are of one item: it joins its results itself.
   bool together = false, block_begins = false, block_ends = false;
-  if constexpr (S::kWorkers > 1) {
+  if (p.block_per_item) {
+    together = block_begins = block_ends = true;
+  } else if constexpr (S::kWorkers > 1) {
     const int64_t block_first = (int64_t)blockIdx.x * S::kWorkers * per;
     const int64_t block_units = min(block_first + S::kWorkers * per, total) - block_first;
     const int units = units_of(span_of(p.lengths[sm_request[0]], p.window, p.most_rows), S::UNIT);
@@ -513,6 +539,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     fill(h & 1);
   }
   int4 opened = make_int4(0, 0, 0, 0);
+  const bool idle = left == 0;
 
   // -- item after item
   while (left > 0) {
@@ -904,7 +931,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
 
     // -- this warp's result: whole, or a part of one
     float scale_l[NT][2], scale_o[NT][2], add_o[NT][2];
-    const bool whole = begins && ends;  // (never if the block joins its results)
+    const bool whole = begins && ends && !together;
     const float unit = kQuantized ? __uint_as_float((uint32_t)exponent << 23) : 1.f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -996,14 +1023,17 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     p.open[worker] = opened;
   }
   if (together) {
-    const bool idle = first_unit >= total;  // (an idle warp has met no barrier yet)
-    if (idle) {
+    if (idle) {  // (it has met no barrier yet)
       __syncthreads();
     }
     __syncthreads();
-    const int active = (int)min((total - (int64_t)blockIdx.x * S::kWorkers * per + per - 1) / per, (int64_t)S::kWorkers);
     const float* const parts = reinterpret_cast<const float*>(smem);
-    const int item = (int)(sm_unit[0] / units_of(span_of(p.lengths[sm_request[0]], p.window, p.most_rows), S::UNIT));
+    const RowSpan span = span_of(p.lengths[sm_request[0]], p.window, p.most_rows);
+    const int units = units_of(span, S::UNIT), item = (int)(sm_unit[0] / units);
+    const bool none = span.end == span.first;
+    const int active = p.block_per_item
+        ? (units + (units + S::kWorkers - 1) / S::kWorkers - 1) / ((units + S::kWorkers - 1) / S::kWorkers)
+        : (int)min((total - (int64_t)blockIdx.x * S::kWorkers * per + per - 1) / per, (int64_t)S::kWorkers);
     const int kv_head = item / p.head_tiles, first_head = (item - kv_head * p.head_tiles) * S::kHeads;
     const int heads = min(p.group - first_head, S::kHeads);
     const bool whole = block_begins && block_ends;
@@ -1027,7 +1057,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
         v.w = __fmaf_rn(f, x.w, v.w);
       }
       if (whole) {
-        const float inv = __fdiv_rn(1.f, sum_l);
+        const float inv = none ? 0.f : __fdiv_rn(1.f, sum_l);  // no row at all: zeros
         const int64_t row = ((int64_t)sm_request[0] * p.kv_heads + kv_head) * p.group + first_head + h;
         if (column < p.dim) {
           *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + (row * p.dim + column) * 2) =
@@ -1035,7 +1065,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
                          pack<BF16>(__fmul_rn(v.z, inv), __fmul_rn(v.w, inv)));
         }
         if (column == 0 && p.lse) {
-          p.lse[row] = __fmaf_rn(from, kLn2, logf(__fmul_rn(sum_l, kUnshift)));
+          p.lse[row] = none ? -INFINITY : __fmaf_rn(from, kLn2, logf(__fmul_rn(sum_l, kUnshift)));
         }
       } else {
         *reinterpret_cast<float4*>(part + 2 * S::kHeads + h * S::DP + column) = v;
@@ -1055,61 +1085,130 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   }
 }
 
-// A block looks after a few workers, one after the other: if others end the item that a worker began, its parts are added
-// up, the heads by the blocks of the grid's second dimension and the groups of kJoinTeam warps, the parts by the warps of
-// a group.
-template <typename S, bool BF16>
-__global__ void __launch_bounds__(kJoinThreads) paged_attention_join(const PagedAttentionParams p) {
-  constexpr int kTeams = kJoinThreads / 32 / kJoinTeam;
-  constexpr int kCols = S::DP / 32;
-  __shared__ float sm_o[kTeams][kJoinTeam][S::DP];
-  __shared__ float sm_m[kTeams][kJoinTeam], sm_l[kTeams][kJoinTeam];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = warp / kJoinTeam, mate = warp % kJoinTeam;
-  for (int worker = blockIdx.x; worker < p.workers; worker += gridDim.x) {
-    const int4 opened = p.open[worker];
-    if (opened.x == 0) {
-      continue;
+// Adds up the parts of items that several workers share, in their order: a block takes a few heads of an item, TEAM warps a
+// head.  BY_ITEM: block x takes item x, whose workers follow from the lengths as in the kernel before (few items, many
+// workers each: 64 blocks and 4 us for one request of 131072 rows; a pass over all workers' records took 38).
+// Otherwise block x takes the item that worker x began, if others end it (many items, most of them whole).
+template <typename S, bool BF16, bool BY_ITEM, int TEAM>
+__global__ void __launch_bounds__(kThreads) paged_attention_join(const PagedAttentionParams p) {
+  constexpr int kTeams = kWarps / TEAM, kCols = S::DP / 32;
+  __shared__ float sm_o[kTeams][TEAM][S::DP];
+  __shared__ float sm_m[kTeams][TEAM], sm_l[kTeams][TEAM];
+  __shared__ int64_t sm_sums[2][kWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = warp / TEAM, mate = warp % TEAM;
+  int worker = blockIdx.x, n, request, item;
+  if constexpr (BY_ITEM) {
+    // (the lengths are not the kernel's before: they were there when it began)
+    const int per_request = p.kv_heads * p.head_tiles;
+    request = blockIdx.x / per_request;
+    item = blockIdx.x - request * per_request;
+    int64_t before = 0, total = 0;
+    for (int b = threadIdx.x; b < p.batch; b += kThreads) {
+      const int64_t units = units_of(span_of(p.lengths[b], p.window, p.most_rows), S::UNIT);
+      total += units;
+      before += b < request ? units : 0;
     }
-    const int kv_head = opened.z / p.head_tiles, first_head = (opened.z - kv_head * p.head_tiles) * S::kHeads;
-    const int heads = min(p.group - first_head, S::kHeads);
-    const int n = opened.x + 1;
-    auto part_of = [&](int i) {  // what the worker began, then what the next ones ended
-      return p.parts + (2 * ((int64_t)worker + i) + (i == 0)) * S::kPartFloats;
-    };
-    for (int h0 = blockIdx.y * kTeams; h0 < heads; h0 += gridDim.y * kTeams) {
-      const int h = h0 + team;
-      float v[kCols], sum_l = 0.f, top = -INFINITY;
+    const int64_t units = units_of(span_of(p.lengths[request], p.window, p.most_rows), S::UNIT);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+      total += __shfl_xor_sync(kAll, total, d);
+      before += __shfl_xor_sync(kAll, before, d);
+    }
+    if (lane == 0) {
+      sm_sums[0][warp] = total;
+      sm_sums[1][warp] = before;
+    }
+    __syncthreads();
+    total = before = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      total += sm_sums[0][w] * per_request;
+      before += sm_sums[1][w] * per_request;
+    }
+    const int64_t per = units_per_worker(total, p.workers);
+    const int64_t start = before + item * units, end = start + units;
+    worker = (int)(start / per);
+    n = (int)((end - 1) / per) - worker + 1;
+    const int64_t block_first = worker / S::kWorkers * S::kWorkers * per;
+    if (start == block_first && end == min(block_first + S::kWorkers * per, total)) {
+      n = 1;  // the whole of what a block had, and joined
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // (by every block: none of this launch ends before the other)
+  } else {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int4 opened = p.open[worker];
+    n = opened.x + 1;
+    request = opened.y;
+    item = opened.z;
+  }
+  if (n == 1) {
+    return;
+  }
+  const int kv_head = item / p.head_tiles, first_head = (item - kv_head * p.head_tiles) * S::kHeads;
+  const int heads = min(p.group - first_head, S::kHeads);
+  auto part_of = [&](int i) {  // what the worker began, then what the next ones ended
+    return p.parts + (2 * ((int64_t)worker + i) + (i == 0)) * S::kPartFloats;
+  };
+  for (int h0 = blockIdx.y * kTeams; h0 < heads; h0 += gridDim.y * kTeams) {
+    const int h = h0 + team;
+    float v[kCols], sum_l = 0.f, top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) {
+      v[j] = 0.f;
+    }
+    for (int i0 = mate * 32; h < heads && i0 < n; i0 += TEAM * 32) {  // 32 parts at a time, each lane one's maximum and sum
+      const int i = i0 + lane;
+      float m = -INFINITY, l = 0.f;
+      if (i < n) {
+        m = part_of(i)[h];
+        l = part_of(i)[S::kHeads + h];
+      }
+      float t = m;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) {
+        t = fmaxf(t, __shfl_xor_sync(kAll, t, d));
+      }
+      t = fmaxf(t, top);
+      const float base = t == -INFINITY ? 0.f : t;
+      const float fade = top == t ? 1.f : exp2_of(top - base);
+      top = t;
+      const float f = exp2_of(m - base);
+      sum_l = __fmul_rn(sum_l, fade);
 #pragma unroll
       for (int j = 0; j < kCols; ++j) {
-        v[j] = 0.f;
+        v[j] = __fmul_rn(v[j], fade);
       }
-      if (h < heads) {
-        for (int i = mate + kJoinTeam * lane; i < n; i += kJoinTeam * 32) {
-          top = fmaxf(top, part_of(i)[h]);
-        }
+      // (joined in their block: nothing is left in the others' parts)
+      unsigned todo = __ballot_sync(kAll, i < n && !(m == -INFINITY && l == 0.f));
+      while (todo) {
+        float2 x[4][kCols / 2];
+        float fs[4], ls[4];
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) {
-          top = fmaxf(top, __shfl_xor_sync(kAll, top, d));
-        }
-        const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll 4
-        for (int i = mate; i < n; i += kJoinTeam) {
-          const float* part = part_of(i);
-          const float m = part[h];
-          if (m == -INFINITY && part[S::kHeads + h] == 0.f) {
-            continue;
-          }
-          const float f = exp2_of(m - base);
-          sum_l = __fmaf_rn(f, part[S::kHeads + h], sum_l);
+        for (int k = 0; k < 4; ++k) {
+          const int from = todo ? __ffs(todo) - 1 : -1;
+          todo &= todo - 1;
+          fs[k] = from < 0 ? 0.f : __shfl_sync(kAll, f, from & 31);
+          ls[k] = from < 0 ? 0.f : __shfl_sync(kAll, l, from & 31);
 #pragma unroll
-          for (int j = 0; j < kCols; j += 2) {
-            const float2 x = *reinterpret_cast<const float2*>(part + 2 * S::kHeads + h * S::DP + 32 * j + 2 * lane);
-            v[j] = __fmaf_rn(f, x.x, v[j]);
-            v[j + 1] = __fmaf_rn(f, x.y, v[j + 1]);
+          for (int j = 0; j < kCols / 2; ++j) {
+            x[k][j] = make_float2(0.f, 0.f);
+            if (from >= 0) {
+              x[k][j] = *reinterpret_cast<const float2*>(part_of(i0 + from) + 2 * S::kHeads + h * S::DP + 64 * j + 2 * lane);
+            }
           }
         }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          sum_l = __fmaf_rn(fs[k], ls[k], sum_l);
+#pragma unroll
+          for (int j = 0; j < kCols / 2; ++j) {
+            v[2 * j] = __fmaf_rn(fs[k], x[k][j].x, v[2 * j]);
+            v[2 * j + 1] = __fmaf_rn(fs[k], x[k][j].y, v[2 * j + 1]);
+          }
+        }
       }
+    }
+    if constexpr (TEAM > 1) {
       if (lane == 0) {
         sm_m[team][mate] = top;
         sm_l[team][mate] = sum_l;
@@ -1119,37 +1218,49 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join(const Paged
         *reinterpret_cast<float2*>(&sm_o[team][mate][32 * j + 2 * lane]) = make_float2(v[j], v[j + 1]);
       }
       __syncthreads();
-      if (h < heads && mate == 0) {
-        float all = -INFINITY, total = 0.f;
+    }
+    if (h < heads && mate == 0) {
+      if constexpr (TEAM > 1) {
+        float all = top;
 #pragma unroll
-        for (int w = 0; w < kJoinTeam; ++w) {
+        for (int w = 1; w < TEAM; ++w) {
           all = fmaxf(all, sm_m[team][w]);
         }
         const float base = all == -INFINITY ? 0.f : all;
-        float f[kJoinTeam];
+        const float own = exp2_of(top - base);
+        sum_l = __fmul_rn(sum_l, own);
 #pragma unroll
-        for (int w = 0; w < kJoinTeam; ++w) {
-          // (a warp without parts: 0; one whose parts' scores are all -inf adds its sum of 0)
-          f[w] = exp2_of(sm_m[team][w] - base);
-          total = __fmaf_rn(f[w], sm_l[team][w], total);
+        for (int j = 0; j < kCols; ++j) {
+          v[j] = __fmul_rn(v[j], own);
         }
-        const int64_t row = ((int64_t)opened.y * p.kv_heads + kv_head) * p.group + first_head + h;
-        const float inv = __fdiv_rn(1.f, total);
-        for (int column = 2 * lane; column < p.dim; column += 64) {
-          float a = 0.f, b = 0.f;
 #pragma unroll
-          for (int w = 0; w < kJoinTeam; ++w) {
-            const float2 x = *reinterpret_cast<const float2*>(&sm_o[team][w][column]);
-            a = __fmaf_rn(f[w], x.x, a);
-            b = __fmaf_rn(f[w], x.y, b);
+        for (int w = 1; w < TEAM; ++w) {
+          const float f = exp2_of(sm_m[team][w] - base);
+          sum_l = __fmaf_rn(f, sm_l[team][w], sum_l);
+#pragma unroll
+          for (int j = 0; j < kCols; j += 2) {
+            const float2 x = *reinterpret_cast<const float2*>(&sm_o[team][w][32 * j + 2 * lane]);
+            v[j] = __fmaf_rn(f, x.x, v[j]);
+            v[j + 1] = __fmaf_rn(f, x.y, v[j + 1]);
           }
-          *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.out) + (row * p.dim + column) * 2) =
-              pack<BF16>(__fmul_rn(a, inv), __fmul_rn(b, inv));
         }
-        if (lane == 0 && p.lse) {
-          p.lse[row] = __fmaf_rn(base, kLn2, logf(__fmul_rn(total, kUnshift)));
+        top = all;
+      }
+      const int64_t row = ((int64_t)request * p.kv_heads + kv_head) * p.group + first_head + h;
+      const float inv = __fdiv_rn(1.f, sum_l);
+#pragma unroll
+      for (int j = 0; j < kCols; j += 2) {
+        const int column = 32 * j + 2 * lane;
+        if (column < p.dim) {
+          *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.out) + (row * p.dim + column) * 2) =
+              pack<BF16>(__fmul_rn(v[j], inv), __fmul_rn(v[j + 1], inv));
         }
       }
+      if (lane == 0 && p.lse) {
+        p.lse[row] = __fmaf_rn(top == -INFINITY ? 0.f : top, kLn2, logf(__fmul_rn(sum_l, kUnshift)));
+      }
+    }
+    if constexpr (TEAM > 1) {
       __syncthreads();
     }
   }
@@ -1165,7 +1276,6 @@ PagedAttentionPlan plan_of(int group, int64_t sms) {
   r.head_tiles = (group + S::kHeads - 1) / S::kHeads;
   r.blocks = (int32_t)(sms * S::kBlocks);
   r.workers = r.blocks * S::kWorkers;
-  r.joiners = (int32_t)(2 * sms);
   r.part_floats = S::kPartFloats;
   return r;
 }
@@ -1203,7 +1313,7 @@ cudaError_t launch_of(const PagedAttentionPlan& plan, const PagedAttentionParams
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)plan.blocks);
+  config.gridDim = dim3((unsigned)(p.block_per_item ? (int64_t)p.batch * p.kv_heads * p.head_tiles : plan.blocks));
   config.blockDim = dim3(kThreads);
   config.dynamicSmemBytes = S::kShared;
   config.stream = stream;
@@ -1214,10 +1324,15 @@ cudaError_t launch_of(const PagedAttentionPlan& plan, const PagedAttentionParams
   if (e != cudaSuccess || !split) {
     return e;
   }
-  config.gridDim = dim3((unsigned)plan.joiners, 4);
-  config.blockDim = dim3(kJoinThreads);
+  const int64_t items = (int64_t)p.batch * p.kv_heads * p.head_tiles;
   config.dynamicSmemBytes = 0;
-  e = cudaLaunchKernelEx(&config, paged_attention_join<S, BF16>, p);
+  if (items <= plan.workers) {
+    config.gridDim = dim3((unsigned)items, (unsigned)(p.group < S::kHeads ? p.group : S::kHeads));
+    e = cudaLaunchKernelEx(&config, paged_attention_join<S, BF16, true, kWarps>, p);
+  } else {
+    config.gridDim = dim3((unsigned)plan.workers, (unsigned)(S::kHeads / 8));
+    e = cudaLaunchKernelEx(&config, paged_attention_join<S, BF16, false, 1>, p);
+  }
   g_launch_count.fetch_add(1, std::memory_order_relaxed);
   return e;
 }

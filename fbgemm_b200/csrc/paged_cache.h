@@ -106,6 +106,7 @@ struct PagedAttentionParams {
   float scale_log2;                               // softmax scale * log2(e)
   int32_t num_pages, page_shift, batch, kv_heads, group, head_tiles, dim, window, workers;
   bool aligned;                                   // rows are 16-byte aligned
+  bool block_per_item;                            // items are short: a block takes one, and joins its warps' results
 };
 
 // Which kernel a cache takes (paged_attention_kernels.cu).
@@ -122,7 +123,6 @@ struct PagedAttentionPlan {
   int32_t head_tiles;
   int32_t blocks;
   int32_t workers;
-  int32_t joiners;
   size_t part_floats;  // of one partial result
 };
 PagedAttentionPlan plan_paged_attention(const PagedAttentionShape& s, int64_t sms);
