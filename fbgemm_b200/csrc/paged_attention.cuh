@@ -355,13 +355,11 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     w.span = span_of(p.lengths[request], p.window, p.most_rows);
     w.units = units_of(w.span, S::UNIT);
   };
-  auto next_unit = [&](Place& w) {  // (the caller knows that there is one)
-    if (++w.u == w.units) {
-      w.u = 0;
-      if (++w.item == per_request) {
-        w.item = 0;
-        enter(w, w.request + 1);
-      }
+  auto next_item = [&](Place& w) {  // (the caller knows that there is one)
+    w.u = 0;
+    if (++w.item == per_request) {
+      w.item = 0;
+      enter(w, w.request + 1);
     }
   };
   Place now, ahead;
@@ -388,20 +386,22 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   int to_read = left;           // tiles whose pages have not been read
   constexpr int kPages = FAST ? SUB : 1;
   int32_t page[kPages], page_next[kPages];  // FAST: every lane knows the pages of the steps, else those of its own row
-  int row_fill = 0, row_next = 0;           // the tile's first row
-  int head_fill = 0, head_next = 0;         // its cached head
+  int row_fill = 0, row_next = aligned_first(ahead.span) + ahead.u * S::ROWS;  // the tile's first row
+  int head_fill = 0, head_next = ahead.item / p.head_tiles, head_ahead = head_next;  // its cached head
   unsigned seen = 0, seen_next = 0;         // its rows that the token sees
   int request_next = 0;
-  bool fill_more = false, next_more = false;
+  bool fill_more = false;
   int64_t off = 0;
+  const int32_t* table = p.tables + ahead.request * p.table_stride;
+  const int page_mask = (1 << p.page_shift) - 1;
+  int row_ahead = row_next;
   auto read_pages = [&] {
-    next_more = to_read > 0;
-    if (!next_more) {
+    if (to_read <= 0) {
       return;
     }
-    const int row = aligned_first(ahead.span) + ahead.u * S::ROWS;
+    const int row = row_ahead;
     row_next = row;
-    head_next = ahead.item / p.head_tiles;
+    head_next = head_ahead;
     request_next = ahead.request;
     seen_next = kFull;
     if (row < ahead.span.first) {  // (by less than 16)
@@ -410,14 +410,17 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     if (ahead.span.end - row < S::ROWS) {
       seen_next &= ahead.span.end > row ? kFull >> (S::ROWS - (ahead.span.end - row)) : 0u;
     }
-    const int32_t* const table = p.tables + ahead.request * p.table_stride;
 #pragma unroll
     for (int s = 0; s < kPages; ++s) {
       const bool there = FAST ? ((seen_next >> (16 * s)) & 0xffffu) != 0 : (seen_next >> lane) & (lane < S::ROWS);
       page_next[s] = there ? __ldg(table + ((row + (FAST ? 16 * s : lane)) >> p.page_shift)) : 0;
     }
-    if (--to_read > 0) {
-      next_unit(ahead);
+    row_ahead += S::ROWS;
+    if (++ahead.u == ahead.units && to_read > 1) {
+      next_item(ahead);
+      head_ahead = ahead.item / p.head_tiles;
+      row_ahead = aligned_first(ahead.span);
+      table = p.tables + ahead.request * p.table_stride;
     }
   };
   auto report_page = [&](int request, int row, int32_t number) {
@@ -428,7 +431,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     }
   };
   auto next_tile = [&] {
-    fill_more = next_more;
+    fill_more = to_read > 0;
     if (!fill_more) {
       return;
     }
@@ -440,14 +443,21 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
       page[s] = page_next[s];
     }
     if constexpr (FAST) {
+      bool good = true;
 #pragma unroll
       for (int s = 0; s < SUB; ++s) {
-        if ((uint32_t)page[s] >= (uint32_t)p.num_pages) {
-          const unsigned lost = (seen >> (16 * s)) & 0xffffu;
-          if (lane == 0 && lost) {
-            report_page(request_next, row_fill + 16 * s + __ffs(lost) - 1, page[s]);
+        good = good && (uint32_t)page[s] < (uint32_t)p.num_pages;
+      }
+      if (!good) {
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+          if ((uint32_t)page[s] >= (uint32_t)p.num_pages) {
+            const unsigned lost = (seen >> (16 * s)) & 0xffffu;
+            if (lane == 0 && lost) {
+              report_page(request_next, row_fill + 16 * s + __ffs(lost) - 1, page[s]);
+            }
+            seen &= ~(0xffffu << (16 * s));
           }
-          seen &= ~(0xffffu << (16 * s));
         }
       }
     } else {
@@ -457,8 +467,9 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
         report_page(request_next, row_fill + lane, page[0]);
       }
       seen = __ballot_sync(kAll, good);
-      off = good ? page[0] * p.page_stride + ((row_fill + lane) & ((1 << p.page_shift) - 1)) * p.slot_stride : 0;
+      off = good ? page[0] * p.page_stride + ((row_fill + lane) & page_mask) * p.slot_stride : 0;
     }
+    --to_read;
     read_pages();
   };
   auto fill = [&](bool is_v) {
@@ -466,15 +477,20 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
       next_tile();
     }
     if (fill_more) {
+      if (lane == 0 && !is_v) {
+        sm_seen[warp][fill_slot] = seen;
+      }
       if constexpr (FAST) {
         if (lane == 0) {
-          sm_seen[warp][fill_slot] = seen;
           const uint32_t bar = bars + 8 * fill_slot;
-          const int first = row_fill & ((1 << p.page_shift) - 1);
-          int steps = 0;
+          const CUtensorMap* const map = is_v ? &v_map : &k_map;
+          int steps = SUB;
+          if (seen != kFull) {
+            steps = 0;
 #pragma unroll
-          for (int s = 0; s < SUB; ++s) {
-            steps += ((seen >> (16 * s)) & 0xffffu) != 0;
+            for (int s = 0; s < SUB; ++s) {
+              steps += ((seen >> (16 * s)) & 0xffffu) != 0;
+            }
           }
           barrier_expect(bar, steps * (S::kBoxes * S::kBoxBytes));
 #pragma unroll
@@ -482,16 +498,13 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
             if ((seen >> (16 * s)) & 0xffffu) {
 #pragma unroll
               for (int x = 0; x < S::kBoxes; ++x) {
-                copy_box(fill_at + (s * S::kBoxes + x) * S::kBoxBytes, is_v ? &v_map : &k_map, 64 * x, head_fill,
-                         (first + 16 * s) & ((1 << p.page_shift) - 1), page[s], bar);
+                copy_box(fill_at + (s * S::kBoxes + x) * S::kBoxBytes, map, 64 * x, head_fill, (row_fill + 16 * s) & page_mask,
+                         page[s], bar);
               }
             }
           }
         }
       } else {
-        if (lane == 0) {
-          sm_seen[warp][fill_slot] = seen;
-        }
         const uint8_t* const rows = (is_v ? p.v : p.k) + head_fill * p.head_stride;
         if (p.aligned) {
           constexpr int kRounds = (S::ROWS * S::kPieces + 31) / 32;
@@ -1015,8 +1028,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     }
     left -= tiles;
     if (left > 0) {
-      now.u += tiles - 1;
-      next_unit(now);
+      next_item(now);
     }
   }
   if (p.open && head_warp == 0 && lane == 0) {
