@@ -111,8 +111,12 @@ int64_t workspace_bytes_of(const PagedAttentionPlan& plan) {
   return (int64_t)plan.workers * (2 * (int64_t)plan.part_floats * 4 + 16);
 }
 
-// Rows up to which an item is left to one block.
-constexpr int64_t kShortItem = 512;
+// Whether a request's rows for a cached head are left to one block each (one launch, no workspace), as far as the host
+// knows their number; longer ones are split over the chip.
+bool short_items(const fbgemm_b200_paged_cache& c, int32_t width, int32_t window) {
+  const int64_t most = (int64_t)width * c.page_size;
+  return (window > 0 && window < most ? window : most) <= 512;
+}
 
 int check_heads(const fbgemm_b200_paged_cache& c, int32_t q_heads) {
   return q_heads >= 1 && q_heads <= 16384 && q_heads % c.kv_heads == 0
@@ -293,13 +297,18 @@ int64_t fbgemm_b200_paged_attention_workspace(
     fbgemm_b200_ctx* ctx,
     const fbgemm_b200_paged_cache* cache,
     int32_t q_heads,
-    int32_t dtype) try {
+    int32_t dtype,
+    int32_t width,
+    int32_t window) try {
   int rc = check_call(ctx, 0);
   rc = rc ? rc : check_cache(cache);
   rc = rc ? rc : check_dtype(*cache, dtype);
   rc = rc ? rc : check_heads(*cache, q_heads);
   if (rc) {
     return rc;
+  }
+  if (short_items(*cache, width, window)) {
+    return 0;
   }
   DeviceGuard guard(ctx->device);
   return workspace_bytes_of(plan_paged_attention(shape_of(*cache, q_heads, dtype), sm_count()));
@@ -352,10 +361,7 @@ int fbgemm_b200_paged_attention(
     return refuse("paged_attention: 2^31 heads of all requests or more");
   }
   const int64_t most = (int64_t)width * cache->page_size;
-  const int64_t span = window > 0 && window < most ? window : most;
-  // Short items are a block's each: one launch, no workspace.  Longer ones are split over the chip.
-  const bool short_items = span <= kShortItem;
-  const bool split = !short_items;
+  const bool split = !short_items(*cache, width, window);
   if (split && (!workspace || !aligned(workspace, 16) || workspace_bytes < workspace_bytes_of(plan))) {
     return refuse("paged_attention: workspace missing, unaligned or too small (fbgemm_b200_paged_attention_workspace)");
   }
@@ -390,7 +396,7 @@ int fbgemm_b200_paged_attention(
   p.window = window;
   p.workers = plan.workers;
   p.aligned = rows_aligned(*cache);
-  p.block_per_item = short_items;
+  p.block_per_item = !split;
   const cudaError_t e = launch_paged_attention(shape, plan, p, split, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? 0 : fail_cuda(e, "paged_attention launch");
 } catch (...) {

@@ -24,6 +24,7 @@ find wrong in the tensors' contents shows in status slot ``slot``
 from __future__ import annotations
 
 import ctypes as C
+from itertools import accumulate
 from typing import NamedTuple
 
 import torch
@@ -31,6 +32,7 @@ import torch
 from . import embedding as E
 
 _DTYPE = {torch.float16: 1, torch.bfloat16: 2}      # FBGEMM_B200_OUT_F16, _BF16
+_CONTIGUOUS = torch.contiguous_format
 _IN_DTYPE = {torch.float16: 2, torch.bfloat16: 3}   # FBGEMM_B200_IN_F16, _BF16
 
 
@@ -73,13 +75,14 @@ class PagedKVCache:
         self.num_pages, self.page_size, self.kv_heads = k.shape[:3]
         self.head_dim = head_dim
         self.device = k.device
+        self._index = k.get_device()
         size = k.element_size()
         self._struct = E._capi.PagedCache(
             k=k.data_ptr(), v=v.data_ptr(), num_pages=self.num_pages, page_stride=strides[0] * size,
             slot_stride=strides[1] * size, head_stride=strides[2] * size, page_size=self.page_size, kv_heads=self.kv_heads,
             head_dim=head_dim, in_dtype=0 if bit_rate else _IN_DTYPE[k.dtype], bit_rate=bit_rate or 0)
         self._address = C.addressof(self._struct)
-        self._workspace = {}   # (query heads, type) -> bytes
+        self._workspace = {}   # (query heads, type, width, window) -> bytes
         E._capi.check(E._capi.lib().fbgemm_b200_paged_cache_check(C.byref(self._struct)), "PagedKVCache")
 
     @classmethod
@@ -108,40 +111,28 @@ class PagedKVCache:
     def __reduce__(self):   # a copy describes its own tensors
         return PagedKVCache, (self._k, self._v, self.bit_rate)
 
-    def _workspace_bytes(self, heads: int, dtype) -> int:
-        n = self._workspace.get((heads, dtype))
+    def _workspace_bytes(self, heads: int, dtype, width: int, window: int) -> int:
+        key = heads, dtype, width, window
+        n = self._workspace.get(key)
         if n is None:
+            if dtype not in _DTYPE or self._index < 0:
+                return 0    # (the call itself refuses)
             rc = E._capi.lib().fbgemm_b200_paged_attention_workspace(
-                E._handle_of(self._k.get_device()), C.byref(self._struct), heads, _DTYPE[dtype])
-            n = self._workspace[heads, dtype] = E._capi.check(rc, "fbgemm_b200_paged_attention_workspace")
+                _context(self._index), C.byref(self._struct), heads, _DTYPE[dtype], width, window)
+            n = E._capi.check(rc, "fbgemm_b200_paged_attention_workspace")
+            if len(self._workspace) >= 1024:    # (a width for every step of long generations)
+                self._workspace.clear()
+            self._workspace[key] = n
         return n
 
 
-def _on(device: int, **tensors) -> None:
-    for name, x in tensors.items():
-        if x is not None and x.get_device() != device:
-            raise ValueError(f"{name} lies on {x.device}, not with the other tensors")
-    if device < 0:
-        raise ValueError("the tensors have to lie on a CUDA device")
+def _context(device: int):
+    """The context's address; None for host tensors, which the call refuses."""
+    return E._handle_of(device) if device >= 0 else None
 
 
-def _vector(x: torch.Tensor, dtype, n: int, name: str) -> None:
-    if x.dtype != dtype:
-        raise TypeError(f"{name} is {dtype}, got {x.dtype}")
-    if x.dim() != 1 or x.shape[0] != n or not x.is_contiguous():
-        raise ValueError(f"{name} is a contiguous vector of {n}")
-
-
-def _tables(x: torch.Tensor, batch: int) -> int:
-    """The table's row stride."""
-    if x.dtype != torch.int32:
-        raise TypeError(f"block_tables is torch.int32, got {x.dtype}")
-    if x.dim() != 2 or x.shape[0] != batch:
-        raise ValueError(f"block_tables is [{batch}, pages of a request]")
-    rows, columns = x.stride()
-    if columns != 1 and x.shape[1] > 1:
-        raise ValueError("block_tables has its columns side by side")
-    return rows if batch > 1 else max(rows, x.shape[1])
+def _stream(device: int):
+    return E._current_stream(device) if device >= 0 else None
 
 
 class PagedSlots(NamedTuple):
@@ -172,39 +163,14 @@ def paged_slots(lengths: torch.Tensor, new_tokens: torch.Tensor, block_tables: t
     num_free}.  Give the outputs' ``lengths`` and ``num_free`` to the next step;
     they are not the inputs' memory."""
     batch = lengths.shape[0]
-    _vector(lengths, torch.int32, batch, "lengths")
-    _vector(new_tokens, torch.int32, batch, "new_tokens")
-    _vector(num_free, torch.int32, 1, "num_free")
-    _vector(free_pages, torch.int32, free_pages.numel(), "free_pages")
-    stride = _tables(block_tables, batch)
-    device = lengths.get_device()
-    _on(device, new_tokens=new_tokens, block_tables=block_tables, free_pages=free_pages, num_free=num_free)
-    slots = torch.empty(capacity, dtype=torch.int64, device=lengths.device)
-    rest = torch.empty(2 * capacity + 2 * batch + 2, dtype=torch.int32, device=lengths.device)
-    positions, requests, offsets, lengths_out, num_free_out = rest.split_with_sizes([capacity, capacity, batch + 1, batch, 1])
-    rc = E._capi.native().paged_slots(
-        E._handle_of(device), batch, lengths, new_tokens, block_tables, block_tables.shape[1], stride, free_pages,
-        free_pages.shape[0], num_free, page_size, capacity, slots, positions, requests, offsets, lengths_out, num_free_out,
-        slot, E._current_stream(device))
+    device = lengths.device
+    slots = torch.empty(capacity, dtype=torch.int64, device=device)
+    rest = torch.empty(2 * capacity + 2 * batch + 2, dtype=torch.int32, device=device)
+    dev = lengths.get_device()
+    rc = E._capi.native().paged_slots(_context(dev), lengths, new_tokens, block_tables, free_pages, num_free, page_size, capacity,
+                                      slots, rest, slot, _stream(dev))
     E._capi.check(rc, "fbgemm_b200_paged_slots")
-    return PagedSlots(slots, positions, requests, offsets, lengths_out, num_free_out)
-
-
-def _heads(x: torch.Tensor, tokens: int, heads: int, dim: int, dtype, name: str):
-    """Token and head stride of [tokens, heads, dim]."""
-    if x.dtype != dtype:
-        raise TypeError(f"{name} is {dtype}, got {x.dtype}")
-    if x.dim() != 3 or x.shape[0] != tokens or x.shape[1] != heads or x.shape[2] != dim:
-        raise ValueError(f"{name} is [{tokens}, {heads}, {dim}], got {list(x.shape)}")
-    t, h, c = x.stride()
-    if c != 1:
-        raise ValueError(f"{name} has a head's values side by side")
-    return t if tokens > 1 else 0, h if heads > 1 else 0
-
-
-def _activation_type(cache: PagedKVCache, dtype, name: str) -> None:
-    if dtype not in _DTYPE or (cache.dtype is not None and dtype != cache.dtype):
-        raise TypeError(f"{name} is {cache.dtype or 'float16 or bfloat16'}, got {dtype}")
+    return PagedSlots(slots, *rest.split_with_sizes((capacity, capacity, batch + 1, batch, 1)))
 
 
 def rotary_append(cache: PagedKVCache, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
@@ -227,52 +193,24 @@ def rotary_append(cache: PagedKVCache, q: torch.Tensor | None, k: torch.Tensor, 
     A position outside the table leaves its token's query unturned and its rows
     unstored (status {1, token, 0, position}); a slot outside the cache stores
     nothing (status {7, token, 0, slot})."""
-    _activation_type(cache, k.dtype, "k")
-    tokens, dim = k.shape[0], cache.head_dim
-    ks = _heads(k, tokens, cache.kv_heads, dim, k.dtype, "k")
-    vs = _heads(v, tokens, cache.kv_heads, dim, k.dtype, "v")
-    _vector(slots, torch.int64, tokens, "slots")
-    device = cache._k.get_device()
-    heads, qs = 0, (0, 0)
-    if q is not None:
-        heads = q.shape[1] if q.dim() == 3 else 0
-        qs = _heads(q, tokens, heads, dim, k.dtype, "q")
-        if q_out is None:
-            q_out = torch.empty((tokens, heads, dim), dtype=k.dtype, device=q.device)
-        elif q_out.dtype != k.dtype or q_out.shape != q.shape or not q_out.is_contiguous():
-            raise ValueError("q_out is a contiguous tensor of q's shape and type")
-    elif q_out is not None:
-        raise ValueError("q_out without q")
-    max_pos, rot, axes, stride, ends = 0, 0, 0, 0, (0, 0, 0, 0)
-    if cos_sin is not None:
-        if positions is None:
-            raise ValueError("cos_sin goes with positions")
-        if cos_sin.dtype != torch.float32 or positions.dtype != torch.int32:
-            raise TypeError("cos_sin is float32, positions are int32")
-        if cos_sin.dim() != 2 or not cos_sin.is_contiguous():
-            raise ValueError("cos_sin is [max_pos, rot_dim], contiguous")
-        max_pos, rot = cos_sin.shape
-        if sections is None:
-            _vector(positions, torch.int32, tokens, "positions")
-            axes, ends = 1, (rot // 2, 0, 0, 0)
-        else:
-            axes = len(sections)
-            if not 1 <= axes <= 4 or min(sections) < 0 or sum(sections) * 2 != rot:
-                raise ValueError("sections are the pairs of 1 to 4 axes, rot_dim / 2 in all")
-            if positions.shape != (axes, tokens) or (positions.stride(1) != 1 and tokens > 1):
-                raise ValueError("with sections, positions is [axes, tokens]")
-            stride = positions.stride(0)
-            total, ends = 0, []
-            for n in sections:
-                total += n
-                ends.append(total)
-            ends += [0] * (4 - axes)
-    elif positions is not None or sections is not None:
-        raise ValueError("positions and sections go with cos_sin")
-    _on(device, q=q, k=k, v=v, slots=slots, positions=positions, cos_sin=cos_sin, q_out=q_out)
-    rc = E._capi.native().rotary_append(
-        E._handle_of(device), cache._address, tokens, heads, _DTYPE[k.dtype], q, *qs, k, *ks, v, *vs, q_out, slots, positions,
-        stride, cos_sin, max_pos, rot, int(interleaved), axes, *ends, slot, E._current_stream(device))
+    if q is None:
+        if q_out is not None:
+            raise ValueError("q_out without q")
+    elif q_out is None:
+        q_out = torch.empty_like(q, memory_format=_CONTIGUOUS)
+    if cos_sin is None:
+        if positions is not None or sections is not None:
+            raise ValueError("positions and sections go with cos_sin")
+    elif positions is None:
+        raise ValueError("cos_sin goes with positions")
+    ends = None
+    if sections is not None:
+        if not 1 <= len(sections) <= 4 or min(sections) < 0:
+            raise ValueError("sections are the pairs of 1 to 4 axes")
+        ends = tuple(accumulate(sections))
+    dev = cache._index
+    rc = E._capi.native().rotary_append(_context(dev), cache._address, dev, q, k, v, q_out, slots, positions, cos_sin,
+                                        interleaved, ends, slot, _stream(dev))
     E._capi.check(rc, "fbgemm_b200_rotary_append")
     return q_out
 
@@ -297,25 +235,16 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, block_tables: torch.Te
     weights enter the sum over rows as 16-bit numbers.  A page outside the cache
     is left out (status {7, request, row, page}); a length that is negative or
     beyond the table is brought within it (status {3, request, 0, length})."""
-    if q.dim() != 3:
-        raise ValueError("q is [batch, heads, head_dim]")
-    batch, heads, dim = q.shape
-    dtype = q.dtype
-    _activation_type(cache, dtype, "q")
-    qs = _heads(q, batch, heads, cache.head_dim, dtype, "q")
-    stride = _tables(block_tables, batch)
-    _vector(lengths, torch.int32, batch, "lengths")
-    device = q.get_device()
-    _on(device, block_tables=block_tables, lengths=lengths, cache=cache._k, out=out)
     if out is None:
-        out = torch.empty((batch, heads, dim), dtype=dtype, device=q.device)
-    elif out.dtype != dtype or out.shape != q.shape or not out.is_contiguous():
-        raise ValueError("out is a contiguous tensor of q's shape and type")
-    lse = torch.empty((batch, heads), dtype=torch.float32, device=q.device) if return_lse else None
-    n = cache._workspace_bytes(heads, dtype)
-    workspace = torch.empty(n, dtype=torch.uint8, device=q.device)   # the call's own: calls on several streams, captured ones too, share nothing
-    rc = E._capi.native().paged_attention(
-        E._handle_of(device), cache._address, batch, heads, _DTYPE[dtype], q, *qs, block_tables, block_tables.shape[1], stride,
-        lengths, dim ** -0.5 if scale is None else scale, window, out, lse, workspace, n, slot, E._current_stream(device))
+        out = torch.empty_like(q, memory_format=_CONTIGUOUS)
+    batch, heads = q.shape[:2]
+    lse = torch.empty((batch, heads), dtype=torch.float32, device=cache.device) if return_lse else None
+    # The call's own workspace: calls on several streams, captured ones too, share nothing.
+    workspace, n = None, cache._workspace_bytes(heads, q.dtype, block_tables.shape[-1], window)
+    if n:
+        workspace = torch.empty(n, dtype=torch.uint8, device=cache.device)
+    dev = cache._index
+    rc = E._capi.native().paged_attention(_context(dev), cache._address, dev, q, block_tables, lengths, scale, window, out, lse,
+                                          workspace, n, slot, _stream(dev))
     E._capi.check(rc, "fbgemm_b200_paged_attention")
     return (out, lse) if return_lse else out
