@@ -258,6 +258,7 @@ int fbgemm_b200_rotary_append(
     p.rot = r.rot_dim;
     p.axes = r.axes;
     p.interleaved = r.interleaved != 0;
+    p.angles_aligned = aligned(r.cos_sin, 16);
     p.positions = positions;
     p.positions_stride = positions_stride;
   }

@@ -86,6 +86,7 @@ struct RotaryAppendParams {
   int32_t heads, kv_heads, dim, rot, page_shift, axes;
   int32_t section_end[4];                      // pairs [section_end[a - 1], section_end[a]) turn by axis a
   int32_t interleaved, bf16, bits;             // bits: 16, 8 or 4
+  bool angles_aligned;                         // cos_sin to 16 bytes
 };
 cudaError_t launch_rotary_append(const RotaryAppendParams& p, cudaStream_t stream);
 
