@@ -92,7 +92,7 @@ __device__ __forceinline__ void load_angles(float* x, const RotaryAppendParams& 
 // WARP: a warp takes a token.  Otherwise block x takes token x, block y a share of its heads (queries, then keys, then
 // values).
 template <typename T, int BITS, int LANES, bool WARP>
-__global__ void __launch_bounds__(kThreads) rotary_append_kernel(const RotaryAppendParams p) {
+__global__ void __launch_bounds__(kThreads, 8) rotary_append_kernel(const RotaryAppendParams p) {
   constexpr int kGroups = (WARP ? 32 : kThreads) / LANES;  // heads at a time
   const int64_t t = WARP ? (int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32 : blockIdx.x;
   if (t >= p.tokens) {
