@@ -108,7 +108,7 @@ PagedAttentionShape shape_of(const fbgemm_b200_paged_cache& c, int32_t q_heads, 
 }
 
 int64_t workspace_bytes_of(const PagedAttentionPlan& plan) {
-  return (int64_t)plan.workers * (2 * (int64_t)plan.part_floats * 4 + 16);
+  return 2 * (int64_t)plan.workers * (2 * (int64_t)plan.part_floats * 4 + 16);  // (workers of either size)
 }
 
 // Whether a request's rows for a cached head are left to one block each (one launch, no workspace), as far as the host
@@ -382,7 +382,7 @@ int fbgemm_b200_paged_attention(
   p.lse = lse;
   if (split) {
     p.parts = static_cast<float*>(workspace);
-    p.open = reinterpret_cast<int4*>(p.parts + 2 * plan.part_floats * plan.workers);
+    p.open = reinterpret_cast<int4*>(p.parts + 2 * plan.part_floats * 2 * plan.workers);
   }
   p.status = ctx->status + 4 * slot;
   p.most_rows = most;
@@ -398,6 +398,9 @@ int fbgemm_b200_paged_attention(
   p.workers = plan.workers;
   p.aligned = rows_aligned(*cache);
   p.block_per_item = !split;
+  // (no more units than that: the second workers' blocks would only come and go)
+  const int64_t span = window > 0 && window < most ? window : most;
+  p.two = split && (int64_t)batch * cache->kv_heads * plan.head_tiles * (span / plan.unit + 1) >= kUnitsForTwo * plan.workers;
   const cudaError_t e = launch_paged_attention(shape, plan, p, split, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? 0 : fail_cuda(e, "paged_attention launch");
 } catch (...) {

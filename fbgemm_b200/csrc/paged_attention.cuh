@@ -253,7 +253,8 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   int left;                         // units still to be worked on
-  int64_t last_unit = 0, per = 1;
+  int64_t last_unit = 0;
+  UnitSplit split = {1, 0, 1};
   int64_t total = 0;
   const int worker = blockIdx.x * S::kWorkers + warp / S::HW;
   if (p.block_per_item) {
@@ -298,10 +299,10 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     before += w < warp ? sm_sums[w] : 0;
     total += sm_sums[w];
   }
-  per = units_per_worker(total, p.workers);
+  split = split_units(total, p.workers, p.two);
 #pragma unroll
   for (int w = 0; w < S::kWorkers; ++w) {
-    const int64_t first = ((int64_t)blockIdx.x * S::kWorkers + w) * per;
+    const int64_t first = split.first((int64_t)blockIdx.x * S::kWorkers + w);
     if (first >= before && first < before + sum) {
       int64_t from = before;
       for (int b = b0; b < b1; ++b) {
@@ -316,8 +317,8 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     }
   }
   __syncthreads();
-  const int64_t first_unit = worker * per;
-  last_unit = min(first_unit + per, total);
+  const int64_t first_unit = split.first(worker);
+  last_unit = min(first_unit + split.units_of(worker), total);
   left = (int)max(last_unit - first_unit, (int64_t)0);
   }
 
@@ -372,7 +373,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   if (p.block_per_item) {
     together = block_begins = block_ends = true;
   } else if constexpr (S::kWorkers > 1) {
-    const int64_t block_first = (int64_t)blockIdx.x * S::kWorkers * per;
+    const int64_t block_first = split.first((int64_t)blockIdx.x * S::kWorkers), per = split.units_of(blockIdx.x * S::kWorkers);
     const int64_t block_units = min(block_first + S::kWorkers * per, total) - block_first;
     const int units = units_of(span_of(p.lengths[sm_request[0]], p.window, p.most_rows), S::UNIT);
     const int u = (int)(sm_unit[0] % units);
@@ -683,7 +684,9 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
         l[n][x] = w_sum[n][x] = bias_sum[n][x] = 0.f;
       }
     }
-    int exponent = 1;  // 127 + the exponent that V's scales are taken relative to
+    // V's scales are taken relative to 2^(exponent - 127) = 1 / v_unit, and are below scale_limit, twice that.
+    int exponent = 1;
+    float v_unit = __uint_as_float(253u << 23), scale_limit = __uint_as_float(2u << 23);
 
     auto advance = [&] {
       at += kSlot;
@@ -818,29 +821,41 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
         }
       }
       float2 v_sb[SUB][2];
-      unsigned largest = 0;
+      float largest = 0.f;
       if constexpr (kQuantized) {
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             v_sb[s][r] = tail_of(at, s, r);
-            if (rows_seen != kFull && !((rows_seen >> (16 * s + 8 * r + g)) & 1)) {
-              v_sb[s][r] = make_float2(0.f, 0.f);
-            }
-            largest = max(largest, (__float_as_uint(v_sb[s][r].x) >> 23) & 0xff);
           }
         }
-        largest = min(largest, 253u);
-        more |= (int)largest > exponent;
+        if (rows_seen != kFull) {
+#pragma unroll
+          for (int s = 0; s < SUB; ++s) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              if (!((rows_seen >> (16 * s + 8 * r + g)) & 1)) {
+                v_sb[s][r] = make_float2(0.f, 0.f);
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+          largest = fmaxf(largest, fmaxf(fabsf(v_sb[s][0].x), fabsf(v_sb[s][1].x)));
+        }
+        more |= largest >= scale_limit;
       }
       if (__any_sync(kAll, more)) {
         float fade_scale = 1.f;
         if constexpr (kQuantized) {
-          const int to = (int)__reduce_max_sync(kAll, largest);
+          const int to = (int)min(__reduce_max_sync(kAll, __float_as_uint(largest) >> 23), 253u);
           if (to > exponent) {
             fade_scale = to - exponent > 126 ? 0.f : __uint_as_float((uint32_t)(127 - (to - exponent)) << 23);
             exponent = to;
+            scale_limit = __uint_as_float((uint32_t)(exponent + 1) << 23);
+            v_unit = __uint_as_float((uint32_t)(254 - exponent) << 23);
           }
         }
 #pragma unroll
@@ -872,7 +887,6 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
         }
       }
       uint32_t wt[NT][SUB][2];
-      const float v_unit = __uint_as_float((uint32_t)(254 - exponent) << 23);
 #pragma unroll
       for (int s = 0; s < SUB; ++s) {
 #pragma unroll
@@ -1024,7 +1038,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     }
     if (begins && !ends && !(together && block_ends)) {  // others end what this worker began: it names them
       const int64_t last = last_unit - left + now.units - 1;
-      opened = make_int4((int)(last / per - worker), request, item, 0);
+      opened = make_int4((int)(split.worker_of(last) - worker), request, item, 0);
     }
     left -= tiles;
     if (left > 0) {
@@ -1045,7 +1059,9 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     const bool none = span.end == span.first;
     const int active = p.block_per_item
         ? (units + (units + S::kWorkers - 1) / S::kWorkers - 1) / ((units + S::kWorkers - 1) / S::kWorkers)
-        : (int)min((total - (int64_t)blockIdx.x * S::kWorkers * per + per - 1) / per, (int64_t)S::kWorkers);
+        : (int)min((total - split.first(blockIdx.x * S::kWorkers) + split.units_of(blockIdx.x * S::kWorkers) - 1) /
+                       split.units_of(blockIdx.x * S::kWorkers),
+                   (int64_t)S::kWorkers);
     const int kv_head = item / p.head_tiles, first_head = (item - kv_head * p.head_tiles) * S::kHeads;
     const int heads = min(p.group - first_head, S::kHeads);
     const bool whole = block_begins && block_ends;
@@ -1137,12 +1153,12 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join(const PagedAtte
       total += sm_sums[0][w] * per_request;
       before += sm_sums[1][w] * per_request;
     }
-    const int64_t per = units_per_worker(total, p.workers);
+    const UnitSplit split = split_units(total, p.workers, p.two);
     const int64_t start = before + item * units, end = start + units;
-    worker = (int)(start / per);
-    n = (int)((end - 1) / per) - worker + 1;
-    const int64_t block_first = worker / S::kWorkers * S::kWorkers * per;
-    if (start == block_first && end == min(block_first + S::kWorkers * per, total)) {
+    worker = (int)split.worker_of(start);
+    n = (int)split.worker_of(end - 1) - worker + 1;
+    const int block = worker / S::kWorkers * S::kWorkers;
+    if (start == split.first(block) && end == min(split.first(block) + S::kWorkers * split.units_of(block), total)) {
       n = 1;  // the whole of what a block had, and joined
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");  // (by every block: none of this launch ends before the other)
@@ -1292,19 +1308,33 @@ PagedAttentionPlan plan_of(int group, int64_t sms) {
   return r;
 }
 
-// More than 48 KB of shared memory have to be asked for, once per kernel and device.
-template <typename Kernel>
-cudaError_t allow_shared(Kernel kernel, int bytes, std::atomic<uint64_t>& asked) {
+// Sets attributes of a kernel once per device.
+template <typename F>
+cudaError_t once_per_device(std::atomic<uint64_t>& done, F&& set) {
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
   const uint64_t bit = 1ull << (device & 63);
-  if (e == cudaSuccess && (device > 63 || !(asked.load(std::memory_order_relaxed) & bit))) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && (device > 63 || !(done.load(std::memory_order_relaxed) & bit))) {
+    e = set();
     if (e == cudaSuccess) {
-      asked.fetch_or(bit, std::memory_order_relaxed);
+      done.fetch_or(bit, std::memory_order_relaxed);
     }
   }
   return e;
+}
+template <typename Kernel>
+cudaError_t prefer_shared(Kernel kernel, std::atomic<uint64_t>& done) {
+  return once_per_device(done, [=] {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  });
+}
+// (More than 48 KB have to be asked for.)
+template <typename Kernel>
+cudaError_t allow_shared(Kernel kernel, int bytes, std::atomic<uint64_t>& done) {
+  return once_per_device(done, [=] {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  });
 }
 
 template <typename S, bool BF16, bool FAST>
@@ -1325,7 +1355,9 @@ cudaError_t launch_of(const PagedAttentionPlan& plan, const PagedAttentionParams
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)(p.block_per_item ? (int64_t)p.batch * p.kv_heads * p.head_tiles : plan.blocks));
+  config.gridDim = dim3((unsigned)(p.block_per_item ? (int64_t)p.batch * p.kv_heads * p.head_tiles
+                                   : p.two          ? 2 * plan.blocks
+                                                    : plan.blocks));
   config.blockDim = dim3(kThreads);
   config.dynamicSmemBytes = S::kShared;
   config.stream = stream;
@@ -1338,12 +1370,21 @@ cudaError_t launch_of(const PagedAttentionPlan& plan, const PagedAttentionParams
   }
   const int64_t items = (int64_t)p.batch * p.kv_heads * p.head_tiles;
   config.dynamicSmemBytes = 0;
+  // (all kernels with the same share of the SM for shared memory: it is not changed between them)
   if (items <= plan.workers) {
     config.gridDim = dim3((unsigned)items, (unsigned)(p.group < S::kHeads ? p.group : S::kHeads));
-    e = cudaLaunchKernelEx(&config, paged_attention_join<S, BF16, true, kWarps>, p);
+    static std::atomic<uint64_t> known{0};
+    e = prefer_shared(paged_attention_join<S, BF16, true, kWarps>, known);
+    if (e == cudaSuccess) {
+      e = cudaLaunchKernelEx(&config, paged_attention_join<S, BF16, true, kWarps>, p);
+    }
   } else {
-    config.gridDim = dim3((unsigned)plan.workers, (unsigned)(S::kHeads / 8));
-    e = cudaLaunchKernelEx(&config, paged_attention_join<S, BF16, false, 1>, p);
+    config.gridDim = dim3((unsigned)(p.two ? 2 * plan.workers : plan.workers), (unsigned)(S::kHeads / 8));
+    static std::atomic<uint64_t> known{0};
+    e = prefer_shared(paged_attention_join<S, BF16, false, 1>, known);
+    if (e == cudaSuccess) {
+      e = cudaLaunchKernelEx(&config, paged_attention_join<S, BF16, false, 1>, p);
+    }
   }
   g_launch_count.fetch_add(1, std::memory_order_relaxed);
   return e;

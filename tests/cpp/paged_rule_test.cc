@@ -32,7 +32,9 @@ int main() {
   CHECK(aligned_first(span_of(100, 71, 999)) == 16 && units_of(span_of(100, 71, 999), 64) == 2);
   CHECK(units_of(span_of(80, 64, 999), 64) == 1 && units_of(span_of(79, 64, 999), 64) == 2);
   CHECK(units_of(span_of(2147483647, 0, 2147483647), 64) == 33554432);
-  CHECK(units_per_worker(0, 444) == 1 && units_per_worker(444, 444) == 1 && units_per_worker(445, 444) == 2);
+  CHECK(split_units(0, 444, true).big == 1 && split_units(444, 444, true).big == 1 && split_units(445, 444, true).big == 2);
+  CHECK(split_units(444 * 39, 444, true).small == 0 && split_units(444 * 40, 444, true).small == 10);
+  CHECK(split_units(444 * 40, 444, false).small == 0);
 
   const std::vector<std::vector<int32_t>> batches = {
       {1}, {0}, {131072}, {0, 0, 0}, {1, 64, 65, 0, 5000}, std::vector<int32_t>(1000, 77), {5, 100000, 3, 3, 70000, 0}};
@@ -49,15 +51,25 @@ int main() {
             total += units.back();
           }
         }
-        const int64_t per = units_per_worker(total, workers);
-        CHECK(per * workers >= total);
-        for (size_t i = 0; i < start.size(); ++i) {
-          const int64_t first = start[i] / per, last = (start[i] + units[i] - 1) / per;
-          CHECK(last < workers);
-          // as the kernel names them: (end - 1) / per - the worker that begins
-          CHECK((start[i] + units[i] - 1) / per - first == last - first);
-          if (units[i] == 1) {
-            CHECK(first == last);  // an item of one unit needs no joining
+        for (bool two : {false, true}) {
+          const UnitSplit s = split_units(total, workers, two);
+          // every unit has one worker, and each worker's are neighbours
+          int64_t next = 0;
+          for (int64_t w = 0; w < 2 * workers; ++w) {
+            CHECK(s.small == 0 && w >= workers ? s.units_of(w) == 0 : s.first(w) == next);
+            const int64_t end = s.first(w) + s.units_of(w);
+            for (int64_t u : {s.first(w), end - 1}) {
+              CHECK(u >= total || s.units_of(w) == 0 || s.worker_of(u) == w);
+            }
+            next = end > next ? end : next;
+          }
+          CHECK(next >= total);
+          for (size_t i = 0; i < start.size(); ++i) {
+            const int64_t first = s.worker_of(start[i]), last = s.worker_of(start[i] + units[i] - 1);
+            CHECK(first <= last && last < 2 * workers);
+            if (units[i] == 1) {
+              CHECK(first == last);  // an item of one unit needs no joining
+            }
           }
         }
       }
