@@ -6,6 +6,8 @@ using namespace fbgemm_b200;
 
 namespace {
 
+constexpr int64_t kMostRows = 0x7fffff00LL;  // of a request, as far as its block table goes
+
 bool aligned(const void* p, uintptr_t to) {
   return reinterpret_cast<uintptr_t>(p) % to == 0;
 }
@@ -161,8 +163,8 @@ int fbgemm_b200_paged_slots(
   if (batch < 1 || batch > FBGEMM_B200_PAGED_MAX_BATCH) {
     return refuse("paged_slots: 1 to 16384 requests");
   }
-  if (!power_of_two(page_size) || width < 0 || (int64_t)width * page_size > 0x7fffffffLL) {
-    return refuse("paged_slots: page_size is a power of two, 65536 at most, and width * page_size < 2^31");
+  if (!power_of_two(page_size) || width < 0 || (int64_t)width * page_size > kMostRows) {
+    return refuse("paged_slots: page_size is a power of two, 65536 at most, and width * page_size <= 2^31 - 256");
   }
   if (capacity < 0 || free_capacity < 0 || table_stride < width) {
     return refuse("paged_slots: negative capacity, or table rows that overlap");
@@ -345,8 +347,8 @@ int fbgemm_b200_paged_attention(
   if (rc) {
     return rc;
   }
-  if (batch < 0 || width < 0 || window < 0 || (int64_t)width * cache->page_size > 0x7fffffffLL) {
-    return refuse("paged_attention: negative size or window, or width * page_size >= 2^31");
+  if (batch < 0 || width < 0 || window < 0 || (int64_t)width * cache->page_size > kMostRows) {
+    return refuse("paged_attention: negative size or window, or width * page_size > 2^31 - 256");
   }
   if (batch == 0) {
     return 0;
@@ -397,6 +399,7 @@ int fbgemm_b200_paged_attention(
   p.window = window;
   p.workers = plan.workers;
   p.aligned = rows_aligned(*cache);
+  p.tall = cache->page_size >= 32;
   p.block_per_item = !split;
   // (no more units than that: the second workers' blocks would only come and go)
   const int64_t span = window > 0 && window < most ? window : most;

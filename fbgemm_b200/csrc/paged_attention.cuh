@@ -51,10 +51,10 @@
 namespace fbgemm_b200 {
 
 // The rows at `rows` (K's or V's) as a tensor [page][slot][head][columns] for copies of 16 rows of a head: 16-bit columns in
-// swizzled boxes of 64, quantized rows as 4-byte words in boxes of `box`, whose end is filled with zeros
+// swizzled boxes of 64, quantized rows as 4-byte words in boxes of `box`, whose end is filled with zeros, `height` rows high
 // (paged_attention_dispatch.cu).
-cudaError_t encode_rows(CUtensorMap* map, const uint8_t* rows, const PagedAttentionParams& p, bool swizzled, int box, int bits,
-                        int tail_bytes);
+cudaError_t encode_rows(CUtensorMap* map, const uint8_t* rows, const PagedAttentionParams& p, bool swizzled, int box, int height,
+                        int bits, int tail_bytes);
 
 namespace paged {
 
@@ -194,6 +194,7 @@ struct Shape {
   static constexpr bool kSwizzled = BITS == 16;                     // by tensor copies: boxes of 16 rows of 128 bytes
   static constexpr int kBoxes = kSwizzled ? DP / 64 : 1;            // of a step
   static constexpr int kBoxBytes = 16 * (kSwizzled ? 128 : PITCH);
+  static constexpr bool kTall = SUB == 2 && kBoxes == 1;            // two steps' boxes may be one, of a page of 32 rows
   static constexpr int SLOT = ROWS * PITCH;                         // bytes of a half tile
   static constexpr int SLOT_FAST = SUB * kBoxes * kBoxBytes;
   static constexpr int UNIT = ROWS;
@@ -395,6 +396,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   int64_t off = 0;
   const int32_t* table = p.tables + ahead.request * p.table_stride;
   const int page_mask = (1 << p.page_shift) - 1;
+  const bool tall = S::kTall && p.tall;
   int row_ahead = row_next;
   auto read_pages = [&] {
     if (to_read <= 0) {
@@ -405,7 +407,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     head_next = head_ahead;
     request_next = ahead.request;
     seen_next = kFull;
-    if (row < ahead.span.first) {  // (by less than 16)
+    if (row < ahead.span.first) {  // (by less than 32)
       seen_next &= ~0u << (ahead.span.first - row);
     }
     if (ahead.span.end - row < S::ROWS) {
@@ -413,8 +415,12 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     }
 #pragma unroll
     for (int s = 0; s < kPages; ++s) {
-      const bool there = FAST ? ((seen_next >> (16 * s)) & 0xffffu) != 0 : (seen_next >> lane) & (lane < S::ROWS);
-      page_next[s] = there ? __ldg(table + ((row + (FAST ? 16 * s : lane)) >> p.page_shift)) : 0;
+      if (FAST && s > 0 && tall) {
+        break;
+      }
+      const unsigned rows_of = FAST ? (tall ? seen_next : (seen_next >> (16 * s)) & 0xffffu)
+                                    : (seen_next >> lane) & (lane < S::ROWS);  // that this page is needed for
+      page_next[s] = rows_of ? __ldg(table + ((row + (FAST ? 16 * s : lane)) >> p.page_shift)) : 0;
     }
     row_ahead += S::ROWS;
     if (++ahead.u == ahead.units && to_read > 1) {
@@ -445,6 +451,9 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     }
     if constexpr (FAST) {
       bool good = true;
+      if (S::kTall && tall) {
+        page[SUB - 1] = page[0];
+      }
 #pragma unroll
       for (int s = 0; s < SUB; ++s) {
         good = good && (uint32_t)page[s] < (uint32_t)p.num_pages;
@@ -485,6 +494,12 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
         if (lane == 0) {
           const uint32_t bar = bars + 8 * fill_slot;
           const CUtensorMap* const map = is_v ? &v_map : &k_map;
+          if (S::kTall && tall) {
+            barrier_expect(bar, seen ? SUB * S::kBoxBytes : 0);
+            if (seen) {
+              copy_box(fill_at, map, 0, head_fill, row_fill & page_mask, page[0], bar);
+            }
+          } else {
           int steps = SUB;
           if (seen != kFull) {
             steps = 0;
@@ -503,6 +518,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
                          page[s], bar);
               }
             }
+          }
           }
         }
       } else {
@@ -1344,7 +1360,8 @@ cudaError_t launch_of(const PagedAttentionPlan& plan, const PagedAttentionParams
   CUtensorMap maps[2] = {};
   if (FAST && e == cudaSuccess) {
     for (int i = 0; i < 2 && e == cudaSuccess; ++i) {
-      e = encode_rows(&maps[i], i ? p.v : p.k, p, S::kSwizzled, S::kSwizzled ? 64 : S::PITCH / 4, S::BITS, S::kTail);
+      e = encode_rows(&maps[i], i ? p.v : p.k, p, S::kSwizzled, S::kSwizzled ? 64 : S::PITCH / 4, S::kTall && p.tall ? 32 : 16,
+                      S::BITS, S::kTail);
     }
   }
   if (e != cudaSuccess) {

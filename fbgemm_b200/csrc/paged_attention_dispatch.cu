@@ -12,8 +12,8 @@ PagedVariants variants_of(const PagedAttentionShape& s) {
 
 }  // namespace
 
-cudaError_t encode_rows(CUtensorMap* map, const uint8_t* rows, const PagedAttentionParams& p, bool swizzled, int box, int bits,
-                        int tail_bytes) {
+cudaError_t encode_rows(CUtensorMap* map, const uint8_t* rows, const PagedAttentionParams& p, bool swizzled, int box, int height,
+                        int bits, int tail_bytes) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -35,7 +35,7 @@ cudaError_t encode_rows(CUtensorMap* map, const uint8_t* rows, const PagedAttent
   const cuuint64_t dims[4] = {columns, (cuuint64_t)p.kv_heads, (cuuint64_t)1 << p.page_shift, (cuuint64_t)p.num_pages};
   const cuuint64_t strides[3] = {(cuuint64_t)(p.kv_heads > 1 ? p.head_stride : 16), (cuuint64_t)p.slot_stride,
                                  (cuuint64_t)(p.num_pages > 1 ? p.page_stride : 16)};
-  const cuuint32_t boxes[4] = {(cuuint32_t)box, 1, 16, 1};
+  const cuuint32_t boxes[4] = {(cuuint32_t)box, 1, (cuuint32_t)height, 1};
   const cuuint32_t steps[4] = {1, 1, 1, 1};
   const CUresult r = encode(map, swizzled ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT32, 4,
                             const_cast<uint8_t*>(rows), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,

@@ -35,9 +35,9 @@ FBGEMM_B200_HD RowSpan span_of(int32_t length, int32_t window, int64_t most) {
   return RowSpan{(int32_t)first, (int32_t)end};
 }
 
-// Units are counted from a multiple of 16 rows, so that 16 rows of a step lie in one page of 16 or more.
+// Units are counted from a multiple of 32 rows, so that 16 rows of a step lie in one page of 16 or more, and 32 in one of 32.
 FBGEMM_B200_HD int32_t aligned_first(RowSpan s) {
-  return s.first & ~15;
+  return s.first & ~31;
 }
 FBGEMM_B200_HD int32_t units_of(RowSpan s, int32_t unit) {
   const int32_t n = (int32_t)(((int64_t)s.end - aligned_first(s) + unit - 1) / unit);
@@ -129,6 +129,7 @@ struct PagedAttentionParams {
   float scale_log2;                               // softmax scale * log2(e)
   int32_t num_pages, page_shift, batch, kv_heads, group, head_tiles, dim, window, workers;  // workers of the first size
   bool aligned;                                   // rows are 16-byte aligned
+  bool tall;                                      // pages of 32 rows or more
   bool two;                                       // there are workers of either size
   bool block_per_item;                            // items are short: a block takes one, and joins its warps' results
 };

@@ -238,7 +238,7 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, block_tables: torch.Te
     if out is None:
         out = torch.empty_like(q, memory_format=_CONTIGUOUS)
     batch, heads = q.shape[:2]
-    lse = torch.empty((batch, heads), dtype=torch.float32, device=cache.device) if return_lse else None
+    lse = lengths.new_empty((batch, heads), dtype=torch.float32) if return_lse else None
     # The call's own workspace: calls on several streams, captured ones too, share nothing.
     workspace, n = None, cache._workspace_bytes(heads, q.dtype, block_tables.shape[-1], window)
     if n:

@@ -906,7 +906,7 @@ FBGEMM_B200_API int fbgemm_b200_paged_cache_check(const fbgemm_b200_paged_cache*
  * lengths, num_free_out = num_free, block_tables unchanged, and the record
  * {NO_PAGES, first request that does not fit, its new length, num_free} is in
  * status slot `slot`.  batch <= FBGEMM_B200_PAGED_MAX_BATCH, width * page_size
- * < 2^31.  Inputs and outputs do not overlap.  One launch, nothing allocated.
+ * <= 2^31 - 256.  Inputs and outputs do not overlap.  One launch, nothing allocated.
  */
 #define FBGEMM_B200_PAGED_MAX_BATCH 16384
 FBGEMM_B200_API int fbgemm_b200_paged_slots(
@@ -1005,7 +1005,7 @@ FBGEMM_B200_API int64_t fbgemm_b200_paged_attention_workspace(
  * A page outside the cache is recorded (BAD_PAGE, request, row, page) and its
  * rows are left out; a negative length, or one beyond the table, is recorded
  * (SIZE_MISMATCH, request, 0, length) and brought within it.  width *
- * page_size < 2^31.  At most two launches, nothing allocated.
+ * page_size <= 2^31 - 256.  At most two launches, nothing allocated.
  */
 FBGEMM_B200_API int fbgemm_b200_paged_attention(
     fbgemm_b200_ctx* ctx,

@@ -29,8 +29,9 @@ int main() {
   // units
   CHECK(units_of(span_of(0, 0, 9), 64) == 1 && units_of(span_of(1, 0, 9), 64) == 1);
   CHECK(units_of(span_of(64, 0, 999), 64) == 1 && units_of(span_of(65, 0, 999), 64) == 2);
-  CHECK(aligned_first(span_of(100, 71, 999)) == 16 && units_of(span_of(100, 71, 999), 64) == 2);
-  CHECK(units_of(span_of(80, 64, 999), 64) == 1 && units_of(span_of(79, 64, 999), 64) == 2);
+  CHECK(aligned_first(span_of(100, 71, 999)) == 0 && units_of(span_of(100, 71, 999), 64) == 2);
+  CHECK(aligned_first(span_of(100, 61, 999)) == 32 && units_of(span_of(100, 61, 999), 64) == 2);
+  CHECK(units_of(span_of(96, 64, 999), 64) == 1 && units_of(span_of(95, 64, 999), 64) == 2);
   CHECK(units_of(span_of(2147483647, 0, 2147483647), 64) == 33554432);
   CHECK(split_units(0, 444, true).big == 1 && split_units(444, 444, true).big == 1 && split_units(445, 444, true).big == 2);
   CHECK(split_units(444 * 39, 444, true).small == 0 && split_units(444 * 40, 444, true).small == 10);

@@ -282,64 +282,67 @@ def test_rows_that_append_stores_are_rows_that_the_lookups_read():
 # ---- attention ---------------------------------------------------------------
 
 def values(rows, bits, dim):
-    """Cached rows [.., row bytes or values] in 64 bits; (values, scale, centred codes, bias about the centre)."""
+    """Cached rows [.., row bytes or values] in 64 bits; (scale, codes about the middle of their range, bias about it)."""
     if bits == 16:
-        return rows.double().numpy(), None
+        return rows.double(), None
     at = dim * bits // 8
-    sb = rows[..., at:].contiguous().view(torch.float32 if bits == 8 else torch.float16).double().numpy()
-    codes = rows[..., :at].numpy()
+    scale, bias = rows[..., at:].contiguous().view(torch.float32 if bits == 8 else torch.float16).double().split(1, -1)
+    codes = rows[..., :at]
     if bits == 4:
-        codes = np.stack([codes & 15, codes >> 4], -1).reshape(codes.shape[:-1] + (dim,))
-    scale, bias = sb[..., :1], sb[..., 1:]
+        codes = torch.stack([codes & 15, codes >> 4], -1).flatten(-2)
     middle = 128 if bits == 8 else 8
-    c = codes.astype(np.float64)
+    c = codes.double()
     return c * scale + bias, (scale, c - middle, bias + middle * scale)
 
 
-def check_attention(cache, q, tables, lengths, scale=None, window=0, **kw):
+def check_attention(cache, q, tables, lengths, scale=None, window=0, requests=None):
     """Against the formula in 64 bits, within what the roundings add up to."""
     B, H, D = q.shape
     bits = cache.bit_rate or 16
     K, page, G = cache.kv_heads, cache.page_size, H // cache.kv_heads
-    out, lse = paged.paged_attention(cache, q, tables, lengths, scale=scale, window=window, return_lse=True, **kw)
+    out, lse = paged.paged_attention(cache, q, tables, lengths, scale=scale, window=window, return_lse=True)
     ok, info = F.status_read(0)
     assert ok, info
     again = paged.paged_attention(cache, q, tables, lengths, scale=scale, window=window)
     assert torch.equal(out.view(torch.int16), again.view(torch.int16))      # a fixed order of sums
     scale = D ** -0.5 if scale is None else scale
-    got, got_lse = out.double().cpu().numpy(), lse.double().cpu().numpy()
     # A weight is rounded to fp16, beside bf16 rows to bf16.
     weight = HALF_STEP[torch.bfloat16 if cache.dtype == torch.bfloat16 else torch.float16]
     for b, n in enumerate(lengths.tolist()):
-        t = np.arange(max(0, n - window) if window else 0, n)
-        if n == 0:
-            assert (got[b] == 0).all() and (got_lse[b] == -np.inf).all()
+        if requests is not None and b not in requests:
             continue
-        where = tables[b].cpu().numpy()[t // page]
-        kd, kq = values(cache.k[torch.from_numpy(where).to(DEV).long(), torch.from_numpy(t % page).to(DEV)].cpu(), bits, D)
-        vd, vq = values(cache.v[torch.from_numpy(where).to(DEV).long(), torch.from_numpy(t % page).to(DEV)].cpu(), bits, D)
-        for h in range(H):
-            x, kh = q[b, h].double().cpu().numpy(), h // G
-            s = scale * (kd[:, kh] @ x)
-            top = s.max()
-            e = np.exp(s - top)
-            p = e / e.sum()
-            o, full_lse = p @ vd[:, kh], top + np.log(e.sum())
-            # Scores: D products summed in fp32 (the tensor cores may drop bits below 2^-22 of a step's largest term, D / 16
-            # steps), five more operations; codes and centred biases beside quantized rows.
-            size = np.abs(x) @ np.abs(kd[:, kh]).T if kq is None else (
-                (np.abs(kq[0]) * np.abs(kq[1]))[:, kh] @ np.abs(x) + np.abs(kq[2][:, kh, 0]) * np.abs(x).sum())
-            off = scale * size.max() * (D / 16 + 8) * 2.0 ** -22 + (np.abs(s).max() + 16) * 2.0 ** -22
-            # Sums over rows: a step of 16 drops as much, and joining splits and warps a few more; ex2 is off by 2^-22.
-            steps = (len(t) / 16 + 64) * 2.0 ** -22
-            mass = p @ np.abs(vd[:, kh])
-            heavy = mass if vq is None else p @ (np.abs(vq[0]) * np.abs(vq[1]))[:, kh]
-            both = mass if vq is None else heavy + p @ np.abs(vq[2][:, kh])
-            # fp16 weights below 2^-28 of the largest (2^-14 once more of the largest scale) lose bits
-            small = len(t) * 2.0 ** -38 * (np.abs(vd).max() if vq is None else np.abs(vq[0]).max() * 128)
-            most = HALF_STEP[q.dtype] * np.abs(o) + weight * heavy + (2 * off + steps) * both + small + 2.0 ** -25
-            assert (np.abs(got[b, h] - o) <= most).all(), (b, h, n, np.abs(got[b, h] - o).max(), most.min())
-            assert abs(got_lse[b, h] - full_lse) <= 2 * off + steps + abs(full_lse) * 2.0 ** -22, (b, h, n)
+        got, got_lse = out[b].double().view(K, G, D), lse[b].double().view(K, G)
+        if n == 0:
+            assert (got == 0).all() and (got_lse == -math.inf).all()
+            continue
+        t = torch.arange(max(0, n - window) if window else 0, n, device=DEV)
+        where = tables[b, t // page].long()
+        kd, kq = values(cache.k[where, t % page], bits, D)     # [rows, K, D]
+        vd, vq = values(cache.v[where, t % page], bits, D)
+        x = q[b].double().view(K, G, D)
+        s = scale * torch.einsum("kgd,tkd->kgt", x, kd)
+        top = s.amax(-1, keepdim=True)
+        e = (s - top).exp()
+        p = e / e.sum(-1, keepdim=True)
+        o, full_lse = torch.einsum("kgt,tkd->kgd", p, vd), (top + e.sum(-1, keepdim=True).log()).squeeze(-1)
+        # Scores: D products summed in fp32 (the tensor cores may drop bits below 2^-22 of a step's largest term, D / 16
+        # steps), five more operations; codes and centred biases beside quantized rows.
+        size = torch.einsum("kgd,tkd->kgt", x.abs(), kd.abs()) if kq is None else (
+            torch.einsum("kgd,tkd->kgt", x.abs(), kq[0].abs() * kq[1].abs())
+            + kq[2].abs()[..., 0].T[:, None] * x.abs().sum(-1, keepdim=True))
+        off = abs(scale) * size.amax(-1) * (D / 16 + 8) * 2.0 ** -22 + (s.abs().amax(-1) + 16) * 2.0 ** -22
+        # Sums over rows: a step of 16 drops as much, and joining splits and warps a few more; ex2 is off by 2^-22.
+        steps = (len(t) / 16 + 64) * 2.0 ** -22
+        mass = torch.einsum("kgt,tkd->kgd", p, vd.abs())
+        heavy = mass if vq is None else torch.einsum("kgt,tkd->kgd", p, vq[0].abs() * vq[1].abs())
+        both = mass if vq is None else heavy + torch.einsum("kgt,tkd->kgd", p, vq[2].abs().expand(-1, -1, D))
+        # fp16 numbers below 2^-14 are 2^-24 apart, so a small weight is off by 2^-25; weights are 2^10 times their size
+        # relative to a row's that is not above the largest (and beside quantized rows to the largest scale): 2^-35 each.
+        small = len(t) * 2.0 ** -35 * (vd.abs().max() if vq is None else vq[0].abs().max() * 128)
+        most = HALF_STEP[q.dtype] * o.abs() + weight * heavy + (2 * off[..., None] + steps) * both + small + 2.0 ** -25
+        bad = (got - o).abs() - most
+        assert (bad <= 0).all(), (b, n, (got - o).abs().max(), bad.max())
+        assert ((got_lse - full_lse).abs() <= 2 * off + steps + full_lse.abs() * 2.0 ** -22).all(), (b, n)
     return out, lse
 
 
@@ -409,6 +412,11 @@ ATTENTIONS = [
     ([513, 60], 11, 1, 160, 4, "f16", 256, "heads", None, 0),
     ([513, 60], 4, 2, 256, 4, "f16", 16, "pages last", 132, 0),
     ([30000, 5], 2, 1, 64, 4, "f16", 16, "heads", None, 0),
+    # windows that begin in either half of a page, pages of 32 rows and more for two steps of 16
+    ([1000, 47, 0, 33, 2077], 8, 2, 64, 16, "bf16", 32, "heads", None, 45),
+    ([1000, 47, 0, 33, 2077], 8, 2, 128, 8, "f16", 64, "heads", None, 531),
+    ([1000, 47, 0, 33, 2077], 8, 2, 128, 4, "bf16", 32, "tokens", None, 16),
+    ([15, 16, 17, 31, 32, 33], 4, 1, 64, 8, "bf16", 128, "heads", None, 9),
 ]
 
 
@@ -433,15 +441,40 @@ def test_attention(lengths, heads, kv, dim, bits, kind, page, order, pitch, wind
 
 @pytest.mark.parametrize("bits,kind", [(16, "bf16"), (16, "f16"), (8, "bf16"), (4, "f16")])
 def test_attention_of_many_requests_of_all_lengths(bits, kind):
-    """More items than workers, and requests that share pages."""
+    """Requests that share pages, short ones alone and among longer ones (more items than workers)."""
     rng = np.random.default_rng(bits)
-    lengths = [int(x) for x in np.exp(rng.uniform(0, 6, 150))]
     pages, page = 60, 16
     cache = make_cache(pages, page, 4, 64, bits, TYPES[kind])
     fill(cache)
-    tables = torch.from_numpy(rng.integers(0, pages, (150, 26)).astype(np.int32)).to(DEV)
-    q = torch.randn(150, 8, 64, device=DEV).to(TYPES[kind])
-    check_attention(cache, q, tables, torch.tensor(lengths, dtype=torch.int32, device=DEV), scale=0.3)
+    for B, longest in ((150, 400), (500, 1500)):
+        lengths = [int(x) for x in np.exp(rng.uniform(-1, math.log(longest), B))]
+        tables = torch.from_numpy(rng.integers(0, pages, (B, longest // page + 1)).astype(np.int32)).to(DEV)
+        q = torch.randn(B, 8, 64, device=DEV).to(TYPES[kind])
+        check_attention(cache, q, tables, torch.tensor(lengths, dtype=torch.int32, device=DEV), scale=0.3)
+
+
+@pytest.mark.parametrize("bits,kind,page", [(16, "bf16", 16), (8, "f16", 64), (4, "f16", 8)])
+def test_attention_with_workers_of_either_size(bits, kind, page):
+    """So long that a second set of workers takes the last quarter; the requests go over the same pages again and again."""
+    rng = np.random.default_rng(bits)
+    pages = 3000 // page
+    cache = make_cache(pages, page, 8, 64, bits, TYPES[kind])
+    fill(cache)
+    lengths = [300_001, 5, 250_000, 0, 40_000]
+    tables = torch.from_numpy(rng.integers(0, pages, (5, 300_001 // page + 1)).astype(np.int32)).to(DEV)
+    q = torch.randn(5, 8, 64, device=DEV).to(TYPES[kind])
+    check_attention(cache, q, tables, torch.tensor(lengths, dtype=torch.int32, device=DEV))
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+def test_attention_over_one_page_of_one_head(bits):
+    """Dimensions of one have no stride."""
+    for page in (1, 16, 64):
+        cache = make_cache(1, page, 1, 64, bits, torch.float16)
+        fill(cache)
+        q = torch.randn(3, 2, 64, device=DEV).half()
+        tables = torch.zeros(3, 1, dtype=torch.int32, device=DEV)
+        check_attention(cache, q, tables, torch.tensor([page, 0, (page + 1) // 2], dtype=torch.int32, device=DEV))
 
 
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
@@ -575,8 +608,9 @@ def test_attention_beyond_4_gb_of_cache():
     check_attention(cache, torch.randn(1, 4, 256, device=DEV).bfloat16(), tables, torch.tensor([77], dtype=torch.int32, device=DEV))
 
 
-def test_attention_without_a_table_or_a_request():
-    cache = paged.PagedKVCache.allocate(2, 16, 1, 64, device=DEV)
+@pytest.mark.parametrize("page,bits", [(16, None), (64, None), (8, None), (64, 8), (32, 4)])
+def test_attention_without_a_table_or_a_request(page, bits):
+    cache = paged.PagedKVCache.allocate(2, page, 1, 64, bit_rate=bits, device=DEV)
     q = torch.randn(3, 2, 64, device=DEV).bfloat16()
     out, lse = paged.paged_attention(cache, q, torch.zeros(3, 0, dtype=torch.int32, device=DEV),
                                      torch.zeros(3, dtype=torch.int32, device=DEV), return_lse=True)
