@@ -197,6 +197,7 @@ SIGNATURES = {
 
 _lib = None
 _native = None
+_paged = None
 _build_error = None   # why the library was loaded as it was found
 
 
@@ -213,6 +214,20 @@ def native():
             raise Fbgemmb200Error(f"{_build.NATIVE_PATH} cannot be loaded: {e}{built}") from e
         _native = _native_calls
     return _native
+
+
+def paged():
+    """The CPython extension of the paged key-value cache (paged_calls.c)."""
+    global _paged
+    if _paged is None:
+        lib()
+        try:
+            from . import _paged_calls
+        except ImportError as e:
+            built = f"; building it failed: {_build_error}" if _build_error else ""
+            raise Fbgemmb200Error(f"{_build.PAGED_PATH} cannot be loaded: {e}{built}") from e
+        _paged = _paged_calls
+    return _paged
 
 
 def lib() -> C.CDLL:

@@ -32,6 +32,8 @@ CXX_SOURCES = ["generators.cc", "host_copy.cc"]
 NATIVE_SOURCE = "native_calls.c"  # the CPython extension, linked against the library beside it
 # (named and stamped for the interpreter it is built for: another one builds its own, and does not load this one)
 NATIVE_PATH = os.path.join(PKG_DIR, "_native_calls" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+PAGED_SOURCE = "paged_calls.c"     # and the one of the paged key-value cache
+PAGED_PATH = os.path.join(PKG_DIR, "_paged_calls" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -57,7 +59,7 @@ def _sources():
 
 def _fingerprint() -> str:
     h = hashlib.sha256()
-    paths = _sources() + [os.path.join(CSRC, NATIVE_SOURCE)]
+    paths = _sources() + [os.path.join(CSRC, NATIVE_SOURCE), os.path.join(CSRC, PAGED_SOURCE)]
     for d in (CSRC, os.path.join(INCLUDE, "fbgemm_b200")):
         for name in sorted(os.listdir(d)):
             if name.endswith((".h", ".cuh")):
@@ -72,7 +74,7 @@ def _fingerprint() -> str:
 
 
 def needs_build() -> bool:
-    if not all(os.path.exists(p) for p in (LIB_PATH, NATIVE_PATH, STAMP_PATH)):
+    if not all(os.path.exists(p) for p in (LIB_PATH, NATIVE_PATH, PAGED_PATH, STAMP_PATH)):
         return True
     with open(STAMP_PATH) as f:
         return f.read().strip() != _fingerprint()
@@ -115,9 +117,10 @@ def build(force: bool = False, verbose: bool = False) -> str:
     unnamed = os.path.join(PKG_DIR, "_native_calls.so")   # any interpreter would load a file of this name
     if os.path.exists(unnamed) and unnamed != NATIVE_PATH:
         os.remove(unnamed)
-    subprocess.run([shutil.which("gcc") or "cc", "-O2", "-Wall", "-shared", "-fPIC", "-I", INCLUDE,
-                    "-I", sysconfig.get_paths()["include"], os.path.join(CSRC, NATIVE_SOURCE), "-o", NATIVE_PATH,
-                    "-L", PKG_DIR, "-l:" + os.path.basename(LIB_PATH), "-Wl,-rpath,$ORIGIN"], check=True)
+    for source, path in ((NATIVE_SOURCE, NATIVE_PATH), (PAGED_SOURCE, PAGED_PATH)):
+        subprocess.run([shutil.which("gcc") or "cc", "-O2", "-Wall", "-shared", "-fPIC", "-I", INCLUDE,
+                        "-I", sysconfig.get_paths()["include"], os.path.join(CSRC, source), "-o", path,
+                        "-L", PKG_DIR, "-l:" + os.path.basename(LIB_PATH), "-Wl,-rpath,$ORIGIN"], check=True)
     with open(STAMP_PATH, "w") as f:
         f.write(_fingerprint())
     return LIB_PATH

@@ -167,7 +167,7 @@ def paged_slots(lengths: torch.Tensor, new_tokens: torch.Tensor, block_tables: t
     slots = torch.empty(capacity, dtype=torch.int64, device=device)
     rest = torch.empty(2 * capacity + 2 * batch + 2, dtype=torch.int32, device=device)
     dev = lengths.get_device()
-    rc = E._capi.native().paged_slots(_context(dev), lengths, new_tokens, block_tables, free_pages, num_free, page_size, capacity,
+    rc = E._capi.paged().paged_slots(_context(dev), lengths, new_tokens, block_tables, free_pages, num_free, page_size, capacity,
                                       slots, rest, slot, _stream(dev))
     E._capi.check(rc, "fbgemm_b200_paged_slots")
     return PagedSlots(slots, *rest.split_with_sizes((capacity, capacity, batch + 1, batch, 1)))
@@ -209,7 +209,7 @@ def rotary_append(cache: PagedKVCache, q: torch.Tensor | None, k: torch.Tensor, 
             raise ValueError("sections are the pairs of 1 to 4 axes")
         ends = tuple(accumulate(sections))
     dev = cache._index
-    rc = E._capi.native().rotary_append(_context(dev), cache._address, dev, q, k, v, q_out, slots, positions, cos_sin,
+    rc = E._capi.paged().rotary_append(_context(dev), cache._address, dev, q, k, v, q_out, slots, positions, cos_sin,
                                         interleaved, ends, slot, _stream(dev))
     E._capi.check(rc, "fbgemm_b200_rotary_append")
     return q_out
@@ -244,7 +244,7 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, block_tables: torch.Te
     if n:
         workspace = torch.empty(n, dtype=torch.uint8, device=cache.device)
     dev = cache._index
-    rc = E._capi.native().paged_attention(_context(dev), cache._address, dev, q, block_tables, lengths, scale, window, out, lse,
+    rc = E._capi.paged().paged_attention(_context(dev), cache._address, dev, q, block_tables, lengths, scale, window, out, lse,
                                           workspace, n, slot, _stream(dev))
     E._capi.check(rc, "fbgemm_b200_paged_attention")
     return (out, lse) if return_lse else out

@@ -210,3 +210,25 @@ def test_nothing_to_do_is_no_call():
     assert _capi.lib().fbgemm_b200_rotary_append(Stand.handle, C.byref(c_cache()), 0, 4, 1, None, 0, 0, None, 0, 0, None, 0, 0,
                                                  None, None, None, 0, None, 0, None) == 0
     assert E is paged.E
+
+
+def test_numbers_and_arrays_are_no_tensors():
+    for wrong in (5, 1.5, None, [1]):
+        for call, arguments, name in ((paged.paged_attention, attention_arguments, "q"),
+                                      (paged.paged_attention, attention_arguments, "block_tables"),
+                                      (paged.paged_attention, attention_arguments, "lengths"),
+                                      (paged.rotary_append, append_arguments, "k"), (paged.rotary_append, append_arguments, "slots"),
+                                      (paged.paged_slots, slots_arguments, "lengths"), (paged.paged_slots, slots_arguments, "num_free")):
+            with pytest.raises((TypeError, AttributeError)):
+                call(**arguments(**{name: wrong}))
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    many = torch.zeros(1, dtype=torch.int32).expand(1, 1).as_strided((2, 2 ** 31), (0, 0))
+    for call, arguments, bad in ((paged.paged_attention, attention_arguments, dict(window=2 ** 31)),
+                                 (paged.paged_attention, attention_arguments, dict(window=-1)),
+                                 (paged.paged_attention, attention_arguments, dict(block_tables=many)),
+                                 (paged.paged_slots, slots_arguments, dict(page_size=2 ** 33)),
+                                 (paged.paged_slots, slots_arguments, dict(block_tables=many))):
+        with pytest.raises(ValueError):
+            call(**arguments(**bad))
