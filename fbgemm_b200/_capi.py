@@ -188,7 +188,7 @@ SIGNATURES = {
                                           C.c_int, _p]),
     "fbgemm_b200_rotary_append": (C.c_int, [_p, _cachep, _i64, _i32, _i32, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p,
                                             _p, _p, _i64, C.POINTER(Rotary), C.c_int, _p]),
-    "fbgemm_b200_paged_attention_workspace": (_i64, [_p, _cachep, _i32, _i32, _i32, _i32]),
+    "fbgemm_b200_paged_attention_workspace": (_i64, [_p, _cachep, _i32, _i32, _i32, _i32, _i32]),
     "fbgemm_b200_paged_attention": (C.c_int, [_p, _cachep, _i32, _i32, _i32, _p, _i64, _i64, _p, _i32, _i64, _p, C.c_float,
                                               _i32, _p, _p, _p, _i64, C.c_int, _p]),
     "fbgemm_b200_float_to_fused_8bit_rowwise": (C.c_int, [_p, _i64, C.c_int32, _p, _p]),

@@ -113,11 +113,15 @@ int64_t workspace_bytes_of(const PagedAttentionPlan& plan) {
   return 2 * (int64_t)plan.workers * (2 * (int64_t)plan.part_floats * 4 + 16);  // (workers of either size)
 }
 
-// Whether a request's rows for a cached head are left to one block each (one launch, no workspace), as far as the host
-// knows their number; longer ones are split over the chip.
-bool short_items(const fbgemm_b200_paged_cache& c, int32_t width, int32_t window) {
+// Rows that a request can have, as far as the host knows.
+int64_t span_most(const fbgemm_b200_paged_cache& c, int32_t width, int32_t window) {
   const int64_t most = (int64_t)width * c.page_size;
-  return (window > 0 && window < most ? window : most) <= 512;
+  return window > 0 && window < most ? window : most;
+}
+
+int32_t cluster_of(const fbgemm_b200_paged_cache& c, const PagedAttentionPlan& plan, int64_t batch, int32_t width,
+                   int32_t window) {
+  return blocks_of_item(span_most(c, width, window), batch * c.kv_heads * plan.head_tiles, plan.blocks);
 }
 
 int check_heads(const fbgemm_b200_paged_cache& c, int32_t q_heads) {
@@ -299,6 +303,7 @@ int fbgemm_b200_rotary_append(
 int64_t fbgemm_b200_paged_attention_workspace(
     fbgemm_b200_ctx* ctx,
     const fbgemm_b200_paged_cache* cache,
+    int32_t batch,
     int32_t q_heads,
     int32_t dtype,
     int32_t width,
@@ -310,11 +315,9 @@ int64_t fbgemm_b200_paged_attention_workspace(
   if (rc) {
     return rc;
   }
-  if (short_items(*cache, width, window)) {
-    return 0;
-  }
   DeviceGuard guard(ctx->device);
-  return workspace_bytes_of(plan_paged_attention(shape_of(*cache, q_heads, dtype), sm_count()));
+  const PagedAttentionPlan plan = plan_paged_attention(shape_of(*cache, q_heads, dtype), sm_count());
+  return cluster_of(*cache, plan, batch, width, window) ? 0 : workspace_bytes_of(plan);
 } catch (...) {
   return thrown();
 }
@@ -364,7 +367,8 @@ int fbgemm_b200_paged_attention(
     return refuse("paged_attention: 2^31 heads of all requests or more");
   }
   const int64_t most = (int64_t)width * cache->page_size;
-  const bool split = !short_items(*cache, width, window);
+  const int32_t cluster = cluster_of(*cache, plan, batch, width, window);
+  const bool split = cluster == 0;
   if (split && (!workspace || !aligned(workspace, 16) || workspace_bytes < workspace_bytes_of(plan))) {
     return refuse("paged_attention: workspace missing, unaligned or too small (fbgemm_b200_paged_attention_workspace)");
   }
@@ -400,9 +404,9 @@ int fbgemm_b200_paged_attention(
   p.workers = plan.workers;
   p.aligned = rows_aligned(*cache);
   p.tall = cache->page_size >= 32;
-  p.block_per_item = !split;
+  p.cluster = cluster;
   // (no more units than that: the second workers' blocks would only come and go)
-  const int64_t span = window > 0 && window < most ? window : most;
+  const int64_t span = span_most(*cache, width, window);
   p.two = split && (int64_t)batch * cache->kv_heads * plan.head_tiles * (span / plan.unit + 1) >= kUnitsForTwo * plan.workers;
   const cudaError_t e = launch_paged_attention(shape, plan, p, split, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? 0 : fail_cuda(e, "paged_attention launch");

@@ -38,7 +38,8 @@
 // covered by the other warps of the SM; its ring runs on into the next item meanwhile.  (Blocks that joined their warps'
 // results item by item took 77 us for 128 requests of 64 to 4096 4-bit rows.)  An item that several workers share is
 // left as partial results, and a second launch (paged_attention_join) adds them up in a fixed order; a block whose workers
-// all work on one item joins theirs first.
+// all work on one item joins theirs first.  Short items are left to a block each, or to a cluster of two, four or eight that
+// joins its results through distributed shared memory: one launch.
 #pragma once
 
 #include <cuda.h>
@@ -162,6 +163,28 @@ __device__ __forceinline__ void copy_box(uint32_t to, const CUtensorMap* map, in
       : "memory");
 }
 
+// ---- the blocks of a cluster --------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// Where block `rank` of the cluster has what lies at `at` here.
+__device__ __forceinline__ uint32_t in_block(uint32_t at, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float load_remote(uint32_t at) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 load_remote4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
 // Nibbles i and i + 4 of a word as subnormal fp16, c 2^-20.  (The even ones by a product: the units for shifts and masks
 // are the busier ones.)
 __device__ __forceinline__ uint32_t nibbles(uint32_t w, int i) {
@@ -213,6 +236,7 @@ struct Shape {
   static constexpr int kShared = kWarps * SLOTS * SLOT + 1024;      // (aligned for swizzled boxes)
   static_assert(SLOT >= SLOT_FAST, "one size for both");
   static_assert(SLOTS >= 3, "two half tiles on their way");
+  static_assert(kWarps * SLOTS * SLOT_FAST >= (kWorkers + 1) * kPartFloats * 4, "results take the rings' place");
 };
 
 // ---- the kernel -------------------------------------------------------------------------------------------------------
@@ -258,15 +282,20 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   UnitSplit split = {1, 0, 1};
   int64_t total = 0;
   const int worker = blockIdx.x * S::kWorkers + warp / S::HW;
-  if (p.block_per_item) {
-    // -- a block takes an item, its workers equal shares of it
-    const int request = blockIdx.x / per_request;
+  const int rank = p.cluster ? blockIdx.x % p.cluster : 0;  // of this block in its cluster
+  int block_item = 0, block_active = S::kWorkers;           // the item of blocks that join their results, workers that have some
+  if (p.cluster) {
+    // -- a cluster of blocks takes an item, its workers equal shares of it
+    const int at = blockIdx.x / p.cluster, request = at / per_request;
     const int units = units_of(span_of(p.lengths[request], p.window, p.most_rows), S::UNIT);
-    const int share = (units + S::kWorkers - 1) / S::kWorkers, first = share * (warp / S::HW);
+    const int workers = p.cluster * S::kWorkers, share = (units + workers - 1) / workers;
+    const int first = share * (rank * S::kWorkers + warp / S::HW);
     left = max(min(share, units - first), 0);
+    block_item = at - request * per_request;
+    block_active = min(max((units - share * rank * S::kWorkers + share - 1) / share, 0), S::kWorkers);
     if (tid < S::kWorkers) {
       sm_request[tid] = request;
-      sm_unit[tid] = (int64_t)(blockIdx.x - request * per_request) * units + share * tid;
+      sm_unit[tid] = (int64_t)block_item * units + min(share * (rank * S::kWorkers + tid), units - 1);
     }
     __syncthreads();
   } else {
@@ -371,7 +400,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   ahead = now;
   // Whether all of the block's units are of one item: it joins its results itself.
   bool together = false, block_begins = false, block_ends = false;
-  if (p.block_per_item) {
+  if (p.cluster) {
     together = block_begins = block_ends = true;
   } else if constexpr (S::kWorkers > 1) {
     const int64_t block_first = split.first((int64_t)blockIdx.x * S::kWorkers), per = split.units_of(blockIdx.x * S::kWorkers);
@@ -381,6 +410,8 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     together = block_units > per && u + block_units <= units;
     block_begins = u == 0;
     block_ends = u + block_units == units;
+    block_item = (int)(sm_unit[0] / units);
+    block_active = (int)((block_units + per - 1) / per);
   }
 
   // -- half tiles come in turn: K and V of a tile, then of the next.  SLOTS - 1 are on their way, and the pages of the tile
@@ -1069,29 +1100,37 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
       __syncthreads();
     }
     __syncthreads();
-    const float* const parts = reinterpret_cast<const float*>(smem);
     const RowSpan span = span_of(p.lengths[sm_request[0]], p.window, p.most_rows);
-    const int units = units_of(span, S::UNIT), item = (int)(sm_unit[0] / units);
     const bool none = span.end == span.first;
-    const int active = p.block_per_item
-        ? (units + (units + S::kWorkers - 1) / S::kWorkers - 1) / ((units + S::kWorkers - 1) / S::kWorkers)
-        : (int)min((total - split.first(blockIdx.x * S::kWorkers) + split.units_of(blockIdx.x * S::kWorkers) - 1) /
-                       split.units_of(blockIdx.x * S::kWorkers),
-                   (int64_t)S::kWorkers);
-    const int kv_head = item / p.head_tiles, first_head = (item - kv_head * p.head_tiles) * S::kHeads;
+    const int kv_head = block_item / p.head_tiles, first_head = (block_item - kv_head * p.head_tiles) * S::kHeads;
     const int heads = min(p.group - first_head, S::kHeads);
+    const float* const parts = reinterpret_cast<const float*>(smem);
+    auto results_out = [&](int h, int column, float4 v, float from, float sum_l) {
+      const float inv = none ? 0.f : __fdiv_rn(1.f, sum_l);  // no row at all: zeros
+      const int64_t row = ((int64_t)sm_request[0] * p.kv_heads + kv_head) * p.group + first_head + h;
+      if (column < p.dim) {
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + (row * p.dim + column) * 2) =
+            make_uint2(pack<BF16>(__fmul_rn(v.x, inv), __fmul_rn(v.y, inv)),
+                       pack<BF16>(__fmul_rn(v.z, inv), __fmul_rn(v.w, inv)));
+      }
+      if (column == 0 && p.lse) {
+        p.lse[row] = none ? -INFINITY : __fmaf_rn(from, kLn2, logf(__fmul_rn(sum_l, kUnshift)));
+      }
+    };
     const bool whole = block_begins && block_ends;
-    float* const part = p.parts + (2 * (int64_t)blockIdx.x * S::kWorkers + block_begins) * S::kPartFloats;
+    // A part of an item goes to where the join looks for it, or to the end of the workers' results for the cluster's blocks.
+    float* const part = p.cluster > 1 ? reinterpret_cast<float*>(smem) + S::kWorkers * S::kPartFloats
+                                      : p.parts + (2 * (int64_t)blockIdx.x * S::kWorkers + block_begins) * S::kPartFloats;
     for (int n = tid; n < heads * (S::DP / 4); n += kThreads) {
       const int h = n / (S::DP / 4), column = n % (S::DP / 4) * 4;
       float top = -INFINITY;
-      for (int w = 0; w < active; ++w) {
+      for (int w = 0; w < block_active; ++w) {
         top = fmaxf(top, parts[w * S::kPartFloats + h]);
       }
       const float from = top == -INFINITY ? 0.f : top;
       float sum_l = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int w = 0; w < active; ++w) {
+      for (int w = 0; w < block_active; ++w) {
         const float f = exp2_of(parts[w * S::kPartFloats + h] - from);
         const float4 x = *reinterpret_cast<const float4*>(parts + w * S::kPartFloats + 2 * S::kHeads + h * S::DP + column);
         sum_l = __fmaf_rn(f, parts[w * S::kPartFloats + S::kHeads + h], sum_l);
@@ -1100,17 +1139,8 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
         v.z = __fmaf_rn(f, x.z, v.z);
         v.w = __fmaf_rn(f, x.w, v.w);
       }
-      if (whole) {
-        const float inv = none ? 0.f : __fdiv_rn(1.f, sum_l);  // no row at all: zeros
-        const int64_t row = ((int64_t)sm_request[0] * p.kv_heads + kv_head) * p.group + first_head + h;
-        if (column < p.dim) {
-          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + (row * p.dim + column) * 2) =
-              make_uint2(pack<BF16>(__fmul_rn(v.x, inv), __fmul_rn(v.y, inv)),
-                         pack<BF16>(__fmul_rn(v.z, inv), __fmul_rn(v.w, inv)));
-        }
-        if (column == 0 && p.lse) {
-          p.lse[row] = none ? -INFINITY : __fmaf_rn(from, kLn2, logf(__fmul_rn(sum_l, kUnshift)));
-        }
+      if (whole && p.cluster <= 1) {
+        results_out(h, column, v, from, sum_l);
       } else {
         *reinterpret_cast<float4*>(part + 2 * S::kHeads + h * S::DP + column) = v;
         if (column == 0) {
@@ -1119,8 +1149,33 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
         }
       }
     }
+    if (p.cluster > 1) {  // the blocks' results, each block a share of the columns
+      cluster_sync();
+      const uint32_t mine = (uint32_t)__cvta_generic_to_shared(part);
+      for (int n = tid + rank * kThreads; n < heads * (S::DP / 4); n += p.cluster * kThreads) {
+        const int h = n / (S::DP / 4), column = n % (S::DP / 4) * 4;
+        float top = -INFINITY;
+        for (int r = 0; r < p.cluster; ++r) {
+          top = fmaxf(top, load_remote(in_block(mine + 4 * h, r)));
+        }
+        const float from = top == -INFINITY ? 0.f : top;
+        float sum_l = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int r = 0; r < p.cluster; ++r) {
+          const float f = exp2_of(load_remote(in_block(mine + 4 * h, r)) - from);
+          const float4 x = load_remote4(in_block(mine + 4 * (2 * S::kHeads + h * S::DP + column), r));
+          sum_l = __fmaf_rn(f, load_remote(in_block(mine + 4 * (S::kHeads + h), r)), sum_l);
+          v.x = __fmaf_rn(f, x.x, v.x);
+          v.y = __fmaf_rn(f, x.y, v.y);
+          v.z = __fmaf_rn(f, x.z, v.z);
+          v.w = __fmaf_rn(f, x.w, v.w);
+        }
+        results_out(h, column, v, from, sum_l);
+      }
+      cluster_sync();  // (a block's memory is there until all have read it)
+    }
     if (!whole) {  // the other workers' parts: nothing
-      for (int n = tid; n < (active - 1) * S::kHeads; n += kThreads) {
+      for (int n = tid; n < (block_active - 1) * S::kHeads; n += kThreads) {
         float* const other = p.parts + 2 * ((int64_t)blockIdx.x * S::kWorkers + 1 + n / S::kHeads) * S::kPartFloats;
         other[n % S::kHeads] = -INFINITY;
         other[S::kHeads + n % S::kHeads] = 0.f;
@@ -1368,18 +1423,21 @@ cudaError_t launch_of(const PagedAttentionPlan& plan, const PagedAttentionParams
     return e;
   }
   // Blocks come to their SM while the launch before ends, and wait there for its results.
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = (unsigned)p.cluster;
+  attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)(p.block_per_item ? (int64_t)p.batch * p.kv_heads * p.head_tiles
-                                   : p.two          ? 2 * plan.blocks
-                                                    : plan.blocks));
+  config.gridDim = dim3((unsigned)(p.cluster ? (int64_t)p.batch * p.kv_heads * p.head_tiles * p.cluster
+                                   : p.two   ? 2 * plan.blocks
+                                             : plan.blocks));
   config.blockDim = dim3(kThreads);
   config.dynamicSmemBytes = S::kShared;
   config.stream = stream;
-  config.attrs = &attr;
-  config.numAttrs = 1;
+  config.attrs = attrs;
+  config.numAttrs = p.cluster > 1 ? 2 : 1;
   e = cudaLaunchKernelEx(&config, paged_attention_kernel<S, BF16, FAST>, p, maps[0], maps[1]);
   g_launch_count.fetch_add(1, std::memory_order_relaxed);
   if (e != cudaSuccess || !split) {
@@ -1387,6 +1445,7 @@ cudaError_t launch_of(const PagedAttentionPlan& plan, const PagedAttentionParams
   }
   const int64_t items = (int64_t)p.batch * p.kv_heads * p.head_tiles;
   config.dynamicSmemBytes = 0;
+  config.numAttrs = 1;
   // (all kernels with the same share of the SM for shared memory: it is not changed between them)
   if (items <= plan.workers) {
     config.gridDim = dim3((unsigned)items, (unsigned)(p.group < S::kHeads ? p.group : S::kHeads));

@@ -72,6 +72,17 @@ FBGEMM_B200_HD UnitSplit split_units(int64_t total, int64_t workers, bool two) {
   return s;
 }
 
+// Blocks that take an item, as far as the host knows its length: enough for 512 rows each, as long as all of them are on the
+// chip at once; more, up to eight, down to 64 rows each, while every one has an SM to itself.  0: the units are shared by the
+// whole chip, which takes a second launch and a workspace.
+FBGEMM_B200_HD int32_t blocks_of_item(int64_t most_rows, int64_t items, int64_t blocks) {
+  int32_t n = 1;
+  while (n < 8 && ((most_rows > 512 * n && items * 2 * n <= blocks) || (most_rows >= 128 * n && items * 2 * n <= blocks / 3))) {
+    n *= 2;
+  }
+  return most_rows <= 512 * n ? n : 0;
+}
+
 // ---- kernel parameters ------------------------------------------------------------------------------------------------
 
 struct PagedSlotsParams {
@@ -131,7 +142,7 @@ struct PagedAttentionParams {
   bool aligned;                                   // rows are 16-byte aligned
   bool tall;                                      // pages of 32 rows or more
   bool two;                                       // there are workers of either size
-  bool block_per_item;                            // items are short: a block takes one, and joins its warps' results
+  int32_t cluster;                                // 0: the chip shares all units; else blocks that take an item
 };
 
 // Which kernel a cache takes (paged_attention_kernels.cu).

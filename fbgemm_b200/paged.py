@@ -82,7 +82,7 @@ class PagedKVCache:
             slot_stride=strides[1] * size, head_stride=strides[2] * size, page_size=self.page_size, kv_heads=self.kv_heads,
             head_dim=head_dim, in_dtype=0 if bit_rate else _IN_DTYPE[k.dtype], bit_rate=bit_rate or 0)
         self._address = C.addressof(self._struct)
-        self._workspace = {}   # (query heads, type, width, window) -> bytes
+        self._workspace = {}   # (batch, query heads, type, width, window) -> bytes
         E._capi.check(E._capi.lib().fbgemm_b200_paged_cache_check(C.byref(self._struct)), "PagedKVCache")
 
     @classmethod
@@ -111,14 +111,14 @@ class PagedKVCache:
     def __reduce__(self):   # a copy describes its own tensors
         return PagedKVCache, (self._k, self._v, self.bit_rate)
 
-    def _workspace_bytes(self, heads: int, dtype, width: int, window: int) -> int:
-        key = heads, dtype, width, window
+    def _workspace_bytes(self, batch: int, heads: int, dtype, width: int, window: int) -> int:
+        key = batch, heads, dtype, width, window
         n = self._workspace.get(key)
         if n is None:
             if dtype not in _DTYPE or self._index < 0:
                 return 0    # (the call itself refuses)
             rc = E._capi.lib().fbgemm_b200_paged_attention_workspace(
-                _context(self._index), C.byref(self._struct), heads, _DTYPE[dtype], width, window)
+                _context(self._index), C.byref(self._struct), batch, heads, _DTYPE[dtype], width, window)
             n = E._capi.check(rc, "fbgemm_b200_paged_attention_workspace")
             if len(self._workspace) >= 1024:    # (a width for every step of long generations)
                 self._workspace.clear()
@@ -240,7 +240,7 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, block_tables: torch.Te
     batch, heads = q.shape[:2]
     lse = lengths.new_empty((batch, heads), dtype=torch.float32) if return_lse else None
     # The call's own workspace: calls on several streams, captured ones too, share nothing.
-    workspace, n = None, cache._workspace_bytes(heads, q.dtype, block_tables.shape[-1], window)
+    workspace, n = None, cache._workspace_bytes(batch, heads, q.dtype, block_tables.shape[-1], window)
     if n:
         workspace = torch.empty(n, dtype=torch.uint8, device=cache.device)
     dev = cache._index

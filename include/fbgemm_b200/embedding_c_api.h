@@ -983,11 +983,12 @@ FBGEMM_B200_API int fbgemm_b200_rotary_append(
     void* stream);
 
 /* Bytes of workspace (16-byte aligned, device memory, contents irrelevant before and after) of one paged_attention call
- * with `q_heads` query heads and these `width` and `window`, 0: none; calls that overlap on the GPU need one each.
- * Negative: an error code. */
+ * with these `batch`, `q_heads`, `width` and `window`, 0: none; calls that overlap on the GPU need one each.  Negative: an
+ * error code. */
 FBGEMM_B200_API int64_t fbgemm_b200_paged_attention_workspace(
     fbgemm_b200_ctx* ctx,
     const fbgemm_b200_paged_cache* cache,
+    int32_t batch,
     int32_t q_heads,
     int32_t dtype,
     int32_t width,

@@ -162,11 +162,11 @@ def test_c_cache_check_takes():
     dict(window=-1), dict(out=0), dict(out=8), dict(workspace=0), dict(workspace_bytes=100),
 ])
 def test_c_attention_refuses(bad):
-    a = dict(ctx=Stand.handle, batch=2, q_heads=4, dtype=1, q=1 << 20, q_token=256, tables=1 << 20, width=100, lengths=1 << 20,
+    a = dict(ctx=Stand.handle, batch=2, q_heads=4, dtype=1, q=1 << 20, q_token=256, tables=1 << 20, width=1000, lengths=1 << 20,
              window=0, out=1 << 20, workspace=1 << 20, workspace_bytes=1 << 30, slot=0)
     a.update(bad)
     rc = _capi.lib().fbgemm_b200_paged_attention(
-        a["ctx"], C.byref(c_cache()), a["batch"], a["q_heads"], a["dtype"], a["q"], a["q_token"], 64, a["tables"], a["width"], 100,
+        a["ctx"], C.byref(c_cache()), a["batch"], a["q_heads"], a["dtype"], a["q"], a["q_token"], 64, a["tables"], a["width"], 1000,
         a["lengths"], 0.125, a["window"], a["out"], None, a["workspace"], a["workspace_bytes"], a["slot"], None)
     assert rc == _capi.EINVAL and _capi.last_error() != ""
 
