@@ -94,6 +94,17 @@ bool good_rows(const void* p, int64_t token, int64_t head) {
   return p && aligned(p, 16) && token % 8 == 0 && head % 8 == 0;
 }
 
+// Whether [tokens, heads, dim] 16-bit values behind one another at `out` share memory with rows that strides (elements)
+// place at p: what one block writes others may not have read yet.
+bool overlaps(const void* out, const void* p, int64_t tokens, int64_t heads, int64_t dim, int64_t p_heads, int64_t token,
+              int64_t head) {
+  const int64_t t = (tokens - 1) * token, h = (p_heads - 1) * head;
+  const intptr_t at = reinterpret_cast<intptr_t>(p), to = reinterpret_cast<intptr_t>(out);
+  const intptr_t from = at + 2 * ((t < 0 ? t : 0) + (h < 0 ? h : 0));
+  const intptr_t end = at + 2 * ((t > 0 ? t : 0) + (h > 0 ? h : 0) + dim);
+  return from < to + 2 * tokens * heads * dim && to < end;
+}
+
 bool rows_aligned(const fbgemm_b200_paged_cache& c) {
   return aligned(c.k, 16) && aligned(c.v, 16) && (c.page_stride | c.slot_stride | c.head_stride) % 16 == 0;
 }
@@ -243,6 +254,18 @@ int fbgemm_b200_rotary_append(
   if (!good_rows(k, k_token_stride, k_head_stride) || !good_rows(v, v_token_stride, v_head_stride) || !slots) {
     return refuse("rotary_append: k, v or slots is null or not aligned to 16 bytes");
   }
+  if (cache->k == cache->v) {
+    return refuse("rotary_append: keys and values in the same memory");
+  }
+  if (q_out) {
+    const int64_t dim = cache->head_dim;
+    const bool in_place = q_out == q && (tokens == 1 || q_token_stride == q_heads * dim) && (q_heads == 1 || q_head_stride == dim);
+    if ((!in_place && overlaps(q_out, q, tokens, q_heads, dim, q_heads, q_token_stride, q_head_stride)) ||
+        overlaps(q_out, k, tokens, q_heads, dim, cache->kv_heads, k_token_stride, k_head_stride) ||
+        overlaps(q_out, v, tokens, q_heads, dim, cache->kv_heads, v_token_stride, v_head_stride)) {
+      return refuse("rotary_append: q_out overlaps the memory of k, v or, unless it is q itself, q");
+    }
+  }
   RotaryAppendParams p = {};
   if (rotary) {
     const fbgemm_b200_rotary& r = *rotary;
@@ -359,6 +382,9 @@ int fbgemm_b200_paged_attention(
   if (!good_rows(q, q_token_stride, q_head_stride) || !lengths || !out || !aligned(out, 16) ||
       (width > 0 && !block_tables)) {
     return refuse("paged_attention: q, block_tables, lengths or out is null, or q or out not aligned to 16 bytes");
+  }
+  if (overlaps(out, q, batch, q_heads, cache->head_dim, q_heads, q_token_stride, q_head_stride)) {
+    return refuse("paged_attention: out overlaps the memory of q");
   }
   const PagedAttentionShape shape = shape_of(*cache, q_heads, dtype);
   DeviceGuard guard(ctx->device);

@@ -17,9 +17,9 @@ fbgemm_gpu/experimental/gen_ai/src/kv_cache; layouts and arithmetic are this
 library's own.
 
 All calls are asynchronous on torch's current stream of the tensors' device,
-allocate through torch only, and may be captured into a CUDA graph.  What they
-find wrong in the tensors' contents shows in status slot ``slot``
-(``fbgemm_b200.status_read``).
+allocate through torch only, and may be captured into a CUDA graph.  They are
+for serving: no result carries a gradient.  What they find wrong in the
+tensors' contents shows in status slot ``slot`` (``fbgemm_b200.status_read``).
 """
 from __future__ import annotations
 
@@ -50,7 +50,8 @@ class PagedKVCache:
     kv_heads, row], laid out alike and in any order of memory with whole rows.
     ``bit_rate`` None: rows of head_dim float16 or bfloat16 values, 16-byte
     aligned.  8 or 4: uint8, fused quantized rows, 4-byte aligned (a multiple of
-    16 bytes apart they are read fastest).  Holds the tensors, not a copy."""
+    16 bytes apart they are read fastest).  ``k`` and ``v`` do not overlap.  Holds
+    the tensors, not a copy."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, bit_rate: int | None = None):
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
@@ -188,7 +189,8 @@ def rotary_append(cache: PagedKVCache, q: torch.Tensor | None, k: torch.Tensor, 
     tokens] with ``sections``, the number of pairs of each axis in turn (time,
     height, width).  The arithmetic is fp32 with one rounding: to 16 bits, or to
     the codes, scale and bias that ``FloatToFused...Quantized...`` give for the
-    same fp32 row, byte for byte.
+    same fp32 row, byte for byte.  ``q_out``, contiguous, takes the turned queries; it
+    may be ``q`` itself, and overlaps nothing else that is read.
 
     A position outside the table leaves its token's query unturned and its rows
     unstored (status {1, token, 0, position}); a slot outside the cache stores
@@ -229,7 +231,8 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, block_tables: torch.Te
     last ones (0: all).  Returns [batch, heads, head_dim] in q's type, and with
     ``return_lse`` the float32 [batch, heads] logarithms of the sums of
     exp(scale * q.k), by which results over parts of the rows are joined.  A
-    request without rows gets zeros and -inf.
+    request without rows gets zeros and -inf.  ``out``, contiguous, takes the
+    result; it does not overlap ``q``.
 
     Scores, sums and the output are fp32 until the output's one rounding; the
     weights enter the sum over rows as 16-bit numbers.  A page outside the cache

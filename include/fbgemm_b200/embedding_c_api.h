@@ -957,7 +957,8 @@ typedef struct fbgemm_b200_rotary {
  * unturned and its rows unstored and is recorded (BAD_INDEX, token, 0,
  * position); so is a slot outside the cache (BAD_PAGE, token, 0, slot).
  * Slots of one call are distinct: a row that two tokens name may get parts of
- * either.  One launch, nothing allocated.
+ * either.  q_out may be q itself; else it does not overlap q, k or v, and the
+ * cache's k and v do not overlap.  One launch, nothing allocated.
  */
 FBGEMM_B200_API int fbgemm_b200_rotary_append(
     fbgemm_b200_ctx* ctx,
@@ -1006,7 +1007,8 @@ FBGEMM_B200_API int64_t fbgemm_b200_paged_attention_workspace(
  * A page outside the cache is recorded (BAD_PAGE, request, row, page) and its
  * rows are left out; a negative length, or one beyond the table, is recorded
  * (SIZE_MISMATCH, request, 0, length) and brought within it.  width *
- * page_size <= 2^31 - 256.  At most two launches, nothing allocated.
+ * page_size <= 2^31 - 256.  out does not overlap q.  At most two launches,
+ * nothing allocated.
  */
 FBGEMM_B200_API int fbgemm_b200_paged_attention(
     fbgemm_b200_ctx* ctx,

@@ -163,7 +163,7 @@ def test_c_cache_check_takes():
 ])
 def test_c_attention_refuses(bad):
     a = dict(ctx=Stand.handle, batch=2, q_heads=4, dtype=1, q=1 << 20, q_token=256, tables=1 << 20, width=1000, lengths=1 << 20,
-             window=0, out=1 << 20, workspace=1 << 20, workspace_bytes=1 << 30, slot=0)
+             window=0, out=1 << 24, workspace=1 << 20, workspace_bytes=1 << 30, slot=0)
     a.update(bad)
     rc = _capi.lib().fbgemm_b200_paged_attention(
         a["ctx"], C.byref(c_cache()), a["batch"], a["q_heads"], a["dtype"], a["q"], a["q_token"], 64, a["tables"], a["width"], 1000,
@@ -184,8 +184,38 @@ def test_c_append_refuses(bad):
                      section_end=(C.c_int32 * 4)(*a["ends"]))
     rc = _capi.lib().fbgemm_b200_rotary_append(
         a["ctx"], C.byref(c_cache()), a["tokens"], a["q_heads"], a["dtype"], a["q"], a["token"], 64, a["k"], 128, 64, a["v"], 128, 64,
-        1 << 20, a["slots"], a["positions"], 0, C.byref(r), 0, None)
+        1 << 24, a["slots"], a["positions"], 0, C.byref(r), 0, None)
     assert rc == _capi.EINVAL and _capi.last_error() != ""
+
+
+def overlapping(rc):
+    return rc == _capi.EINVAL and "overlap" in _capi.last_error()
+
+
+# Two rows of four heads of 64 16-bit values: 1024 bytes at 1 << 20, or with rows 1024 elements apart 2560.
+@pytest.mark.parametrize("token,out", [(256, 0), (256, 1008), (256, -1008), (1024, 0), (1024, 2544), (-256, -512)])
+def test_c_attention_refuses_results_over_queries(token, out):
+    call = _capi.lib().fbgemm_b200_paged_attention
+    assert overlapping(call(Stand.handle, C.byref(c_cache()), 2, 4, 1, 1 << 20, token, 64, 1 << 22, 8, 8, 1 << 22, 0.125, 0,
+                            (1 << 20) + out, None, None, 0, 0, None))
+
+
+@pytest.mark.parametrize("q,token,head,k,v", [
+    (-16, 256, 64, 1 << 23, 1 << 23), (1008, 256, 64, 1 << 23, 1 << 23),
+    (0, 264, 64, 1 << 23, 1 << 23), (0, 256, 72, 1 << 23, 1 << 23), (0, 0, 64, 1 << 23, 1 << 23),   # not the same rows
+    (0, 256, 64, 1008, 1 << 23), (0, 256, 64, 1 << 23, -496), (1 << 23, 256, 64, 0, 1 << 23)])
+def test_c_append_refuses_results_over_what_it_reads(q, token, head, k, v):
+    r = _capi.Rotary(cos_sin=1 << 22, max_pos=4, rot_dim=64, axes=1, section_end=(C.c_int32 * 4)(32, 0, 0, 0))
+    at = 1 << 20
+    assert overlapping(_capi.lib().fbgemm_b200_rotary_append(
+        Stand.handle, C.byref(c_cache()), 2, 4, 1, at + q, token, head, at + k, 128, 64, at + v, 128, 64, at, 1 << 22, 1 << 22, 0,
+        C.byref(r), 0, None))
+
+
+def test_c_append_refuses_keys_and_values_in_one_place():
+    rc = _capi.lib().fbgemm_b200_rotary_append(Stand.handle, C.byref(c_cache(v=1 << 20)), 2, 0, 1, None, 0, 0, 1 << 22, 128, 64,
+                                               1 << 22, 128, 64, None, 1 << 22, None, 0, None, 0, None)
+    assert rc == _capi.EINVAL and "same memory" in _capi.last_error()
 
 
 @pytest.mark.parametrize("bad", [

@@ -1,6 +1,7 @@
 """The paged key-value cache on the GPU, against plain implementations in 64
 bits (and, for what is stored, bit for bit against the oracle's quantizers)."""
 import math
+from concurrent.futures import ThreadPoolExecutor
 
 import numpy as np
 import pytest
@@ -751,3 +752,34 @@ def test_results_into_given_memory():
     paged.rotary_append(cache, same, q[:, :1], q[:, :1], torch.tensor([-1, -1], device=DEV),
                         torch.tensor([3, 5], dtype=torch.int32, device=DEV), angles(9, 64), q_out=same)
     assert torch.equal(same, turned_q)
+    with pytest.raises(_capi.Fbgemmb200Error, match="overlaps"):
+        paged.paged_attention(cache, same, tables, lengths, out=same)
+    big = torch.empty(3, 2, 64, device=DEV).bfloat16()
+    with pytest.raises(_capi.Fbgemmb200Error, match="overlaps"):
+        paged.rotary_append(cache, big[:2], q[:, :1], q[:, :1], torch.tensor([-1, -1], device=DEV), q_out=big[1:])
+
+
+@pytest.mark.parametrize("bits,kind", [(16, "f16"), (4, "bf16")])
+def test_attention_of_the_most_heads(bits, kind):
+    """16384 query heads over one cached head: 256 tiles of heads."""
+    cache = make_cache(40, 16, 1, 32, bits, TYPES[kind])
+    fill(cache)
+    tables = torch.randperm(40, device=DEV).to(torch.int32).view(2, 20)
+    q = torch.randn(2, 16384, 32, device=DEV).to(TYPES[kind])
+    check_attention(cache, q, tables, torch.tensor([100, 311], dtype=torch.int32, device=DEV))
+
+
+def test_slots_from_several_threads():
+    """Batches of several sizes at once, each with another need of shared memory."""
+    def work(i):
+        torch.cuda.set_device(0)
+        batch, ok = 16384 - 2500 * i, True
+        lengths = torch.full((batch,), 3, dtype=torch.int32, device=DEV)
+        for _ in range(50):
+            out = paged.paged_slots(lengths, torch.ones_like(lengths), torch.zeros(batch, 1, dtype=torch.int32, device=DEV),
+                                    lengths[:0], torch.zeros(1, dtype=torch.int32, device=DEV), 16, batch)
+            ok &= bool((out.slots == 3).all())
+        return ok
+
+    with ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(work, range(4)))
