@@ -40,6 +40,12 @@
 // left as partial results, and a second launch (paged_attention_join) adds them up in a fixed order; a block whose workers
 // all work on one item joins theirs first.  Short items are left to a block each, or to a cluster of two, four or eight that
 // joins its results through distributed shared memory: one launch.
+//
+// Measured over 32 requests of 16384 rows of 8 heads of 128 columns: 16-bit rows 323 us, 6.65 TB/s, what a plain copy
+// reaches.  8-bit rows 207 us, 0.84 of that rate, and 4-bit ones 154, 0.57: a tile is half or a quarter of the bytes and
+// no fewer instructions (about 700 of a warp for 32 4-bit rows, three warps a scheduler, one instruction in two cycles),
+// whose chain from the scores through the weights to the sums is what a tile takes.  Below some 100 us a fixed 15 us shows:
+// 4 until the first rows are there, the slowest SM's 10 behind the mean one, and the join.
 #pragma once
 
 #include <cuda.h>
@@ -140,19 +146,32 @@ __device__ __forceinline__ void barrier_init(uint32_t bar) {
 __device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// Waits for a phase of the barrier, for a second or so at most; false: it did not come.
-__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
-  for (int i = 0; i < (1 << 24); ++i) {
-    uint32_t done;
-    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
-                 : "=r"(done)
-                 : "r"(bar), "r"(parity)
-                 : "memory");
-    if (done) {
-      return true;
+__device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+               : "=r"(done)
+               : "r"(bar), "r"(parity)
+               : "memory");
+  return done;
+}
+__device__ __forceinline__ uint64_t nanoseconds() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+// Waits for a phase of the barrier, for a second at most, and once one has not come in time for a millisecond: so that a
+// warp meets all its copies, late ones too, and still ends.  False: it did not come.
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, uint32_t& limit) {
+  if (!barrier_try(bar, parity)) {
+    const uint64_t since = nanoseconds();
+    while (!barrier_try(bar, parity)) {
+      if (nanoseconds() - since > limit) {
+        limit = 1000000;
+        return false;
+      }
     }
   }
-  return false;
+  return true;
 }
 __device__ __forceinline__ void copy_box(uint32_t to, const CUtensorMap* map, int column, int head, int slot, int page,
                                          uint32_t bar) {
@@ -228,7 +247,8 @@ struct Shape {
   static constexpr int kHeads = kWarpHeads * HW;
   static constexpr int kPartFloats = kHeads * (DP + 2);
   // Blocks of an SM by registers (output 4 NT MT, queries 2 NT KSTEPS, scores, and about 70 more), and ring slots of a warp
-  // by shared memory.
+  // by shared memory.  (128 requests of up to 4096 4-bit rows: 68 us with three blocks; 79 with two, 77 with four, whose
+  // registers do not suffice.)
   static constexpr int kRegisters = 4 * NT * MT + 2 * NT * KSTEPS + 4 * NT * SUB;
   static constexpr int kBlocks = kRegisters <= 90 ? 3 : 2;
   static constexpr int kFit = 222 * 1024 / (kBlocks * kWarps * SLOT);
@@ -299,57 +319,57 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     }
     __syncthreads();
   } else {
-  // -- the units of this block's workers, and the requests that their first ones belong to
-  const int chunk = (p.batch + kThreads - 1) / kThreads;
-  const int b0 = min(tid * chunk, p.batch), b1 = min(b0 + chunk, p.batch);
-  auto units_of_request = [&](int b) {
-    return (int64_t)units_of(span_of(p.lengths[b], p.window, p.most_rows), S::UNIT) * per_request;
-  };
-  int64_t sum = 0;
-  for (int b = b0; b < b1; ++b) {
-    sum += units_of_request(b);
-  }
-  int64_t before = sum;
+    // -- the units of this block's workers, and the requests that their first ones belong to
+    const int chunk = (p.batch + kThreads - 1) / kThreads;
+    const int b0 = min(tid * chunk, p.batch), b1 = min(b0 + chunk, p.batch);
+    auto units_of_request = [&](int b) {
+      return (int64_t)units_of(span_of(p.lengths[b], p.window, p.most_rows), S::UNIT) * per_request;
+    };
+    int64_t sum = 0;
+    for (int b = b0; b < b1; ++b) {
+      sum += units_of_request(b);
+    }
+    int64_t before = sum;
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t up = __shfl_up_sync(kAll, before, d);
-    before += lane >= d ? up : 0;
-  }
-  if (lane == 31) {
-    sm_sums[warp] = before;
-  }
-  if (tid < S::kWorkers) {
-    sm_request[tid] = 0;
-    sm_unit[tid] = 0;
-  }
-  __syncthreads();
-  before -= sum;
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t up = __shfl_up_sync(kAll, before, d);
+      before += lane >= d ? up : 0;
+    }
+    if (lane == 31) {
+      sm_sums[warp] = before;
+    }
+    if (tid < S::kWorkers) {
+      sm_request[tid] = 0;
+      sm_unit[tid] = 0;
+    }
+    __syncthreads();
+    before -= sum;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    before += w < warp ? sm_sums[w] : 0;
-    total += sm_sums[w];
-  }
-  split = split_units(total, p.workers, p.two);
+    for (int w = 0; w < kWarps; ++w) {
+      before += w < warp ? sm_sums[w] : 0;
+      total += sm_sums[w];
+    }
+    split = split_units(total, p.workers, p.two);
 #pragma unroll
-  for (int w = 0; w < S::kWorkers; ++w) {
-    const int64_t first = split.first((int64_t)blockIdx.x * S::kWorkers + w);
-    if (first >= before && first < before + sum) {
-      int64_t from = before;
-      for (int b = b0; b < b1; ++b) {
-        const int64_t n = units_of_request(b);
-        if (first < from + n) {
-          sm_request[w] = b;
-          sm_unit[w] = first - from;
-          break;
+    for (int w = 0; w < S::kWorkers; ++w) {
+      const int64_t first = split.first((int64_t)blockIdx.x * S::kWorkers + w);
+      if (first >= before && first < before + sum) {
+        int64_t from = before;
+        for (int b = b0; b < b1; ++b) {
+          const int64_t n = units_of_request(b);
+          if (first < from + n) {
+            sm_request[w] = b;
+            sm_unit[w] = first - from;
+            break;
+          }
+          from += n;
         }
-        from += n;
       }
     }
-  }
-  __syncthreads();
-  const int64_t first_unit = split.first(worker);
-  last_unit = min(first_unit + split.units_of(worker), total);
-  left = (int)max(last_unit - first_unit, (int64_t)0);
+    __syncthreads();
+    const int64_t first_unit = split.first(worker);
+    last_unit = min(first_unit + split.units_of(worker), total);
+    left = (int)max(last_unit - first_unit, (int64_t)0);
   }
 
   const int row_bytes = p.dim * BITS / 8 + S::kTail;
@@ -374,7 +394,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   // The ring: what is filled next and what is worked on.
   uint32_t fill_at = ring_at, at = ring_at;
   int fill_slot = 0, slot = 0;
-  uint32_t phase = 0;
+  uint32_t phase = 0, limit = 1000000000;
 
   // A place in the line of units: tile u of an item (a cached head and a tile of its query heads) of a request.
   struct Place {
@@ -531,25 +551,25 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
               copy_box(fill_at, map, 0, head_fill, row_fill & page_mask, page[0], bar);
             }
           } else {
-          int steps = SUB;
-          if (seen != kFull) {
-            steps = 0;
+            int steps = SUB;
+            if (seen != kFull) {
+              steps = 0;
 #pragma unroll
-            for (int s = 0; s < SUB; ++s) {
-              steps += ((seen >> (16 * s)) & 0xffffu) != 0;
-            }
-          }
-          barrier_expect(bar, steps * (S::kBoxes * S::kBoxBytes));
-#pragma unroll
-          for (int s = 0; s < SUB; ++s) {
-            if ((seen >> (16 * s)) & 0xffffu) {
-#pragma unroll
-              for (int x = 0; x < S::kBoxes; ++x) {
-                copy_box(fill_at + (s * S::kBoxes + x) * S::kBoxBytes, map, 64 * x, head_fill, (row_fill + 16 * s) & page_mask,
-                         page[s], bar);
+              for (int s = 0; s < SUB; ++s) {
+                steps += ((seen >> (16 * s)) & 0xffffu) != 0;
               }
             }
-          }
+            barrier_expect(bar, steps * (S::kBoxes * S::kBoxBytes));
+#pragma unroll
+            for (int s = 0; s < SUB; ++s) {
+              if ((seen >> (16 * s)) & 0xffffu) {
+#pragma unroll
+                for (int x = 0; x < S::kBoxes; ++x) {
+                  copy_box(fill_at + (s * S::kBoxes + x) * S::kBoxBytes, map, 64 * x, head_fill, (row_fill + 16 * s) & page_mask,
+                           page[s], bar);
+                }
+              }
+            }
           }
         }
       } else {
@@ -586,7 +606,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   // The half tile that is worked on next is there, and the one before has been read by all lanes.
   auto arrived = [&] {
     if constexpr (FAST) {
-      if (!barrier_wait(bars + 8 * slot, phase) && atomicCAS(p.status, 0, FBGEMM_B200_STATUS_COPY_TIMEOUT) == 0) {
+      if (!barrier_wait(bars + 8 * slot, phase, limit) && atomicCAS(p.status, 0, FBGEMM_B200_STATUS_COPY_TIMEOUT) == 0) {
         p.status[1] = now.request;
       }
     } else {
@@ -1186,7 +1206,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
 
 // Adds up the parts of items that several workers share, in their order: a block takes a few heads of an item, TEAM warps a
 // head.  BY_ITEM: block x takes item x, whose workers follow from the lengths as in the kernel before (few items, many
-// workers each: 64 blocks and 4 us for one request of 131072 rows; a pass over all workers' records took 38).
+// workers each: 4 us for one request of 131072 rows of four heads; a pass over all workers' records took 38).
 // Otherwise block x takes the item that worker x began, if others end it (many items, most of them whole).
 template <typename S, bool BF16, bool BY_ITEM, int TEAM>
 __global__ void __launch_bounds__(kThreads) paged_attention_join(const PagedAttentionParams p) {

@@ -46,8 +46,10 @@ FBGEMM_B200_HD int32_t units_of(RowSpan s, int32_t unit) {
 
 // Who takes which units.  The first `workers` take `big` units each.  SMs are not equally fast (three quarters to one and
 // an eighth of the mean rate, by where they lie), so with enough to do the last quarter of the line is left to as many
-// workers again, `small` units each, whose blocks start where others have ended: 93 us instead of 99 for 64 requests of up
-// to 8192 16-bit rows.
+// workers again, `small` units each, whose blocks start where others have ended: over 32 requests of 16384 rows 320 us
+// instead of 332 (16-bit rows), 206 instead of 218 (8-bit).  Fewer units than kUnitsForTwo lose more by more parts and a second
+// start than they gain: at 35 a worker (64 requests of up to 8192 rows) nothing, at 37 (one of 131072) 107 us instead of 98, at
+// 17 (48 requests of one head of 256 columns) 52 instead of 41; the two above have 148.
 struct UnitSplit {
   int64_t big, small, workers;
   FBGEMM_B200_HD int64_t first(int64_t worker) const {
@@ -74,7 +76,9 @@ FBGEMM_B200_HD UnitSplit split_units(int64_t total, int64_t workers, bool two) {
 
 // Blocks that take an item, as far as the host knows its length: enough for 512 rows each, as long as all of them are on the
 // chip at once; more, up to eight, down to 64 rows each, while every one has an SM to itself.  0: the units are shared by the
-// whole chip, which takes a second launch and a workspace.
+// whole chip, which takes a second launch and a workspace.  One request of 8 heads, us by one block a head, by two, by
+// eight, shared by the chip: 1000 rows 18.7, 13.3, 8.2, 11.2; 2000 rows 33.2, -, 10.1, 11.5.  (A block an item up to 2048 rows
+// with the chip full: 90 us instead of 101 for 128 requests of 1000 rows, but 42 instead of 32 for 64 of 64 to 2000.)
 FBGEMM_B200_HD int32_t blocks_of_item(int64_t most_rows, int64_t items, int64_t blocks) {
   int32_t n = 1;
   while (n < 8 && ((most_rows > 512 * n && items * 2 * n <= blocks) || (most_rows >= 128 * n && items * 2 * n <= blocks / 3))) {
@@ -145,7 +149,7 @@ struct PagedAttentionParams {
   int32_t cluster;                                // 0: the chip shares all units; else blocks that take an item
 };
 
-// Which kernel a cache takes (paged_attention_kernels.cu).
+// Which kernel a cache takes (paged_attention_variants.cuh).
 struct PagedAttentionShape {
   int32_t bits;       // 16, 8, 4
   bool bf16;          // of q, the output and 16-bit rows

@@ -8,7 +8,9 @@
 // One launch, bound by its latency: a few kilobytes are read and 16 bytes written per row.  Every block scans the
 // requests' counts itself into shared memory (8 bytes a request; a scan of its own launch costs more than reading them
 // again from L2) and then fills its stretch of the maps, each row finding its request by bisection.  What a block reads
-// no block writes: fresh pages are looked up in the stack, not in the table that they are being written to.
+// no block writes: fresh pages are looked up in the stack, not in the table that they are being written to.  256 requests
+// of one new row take 3.7 us, 71 thousand rows of 64 requests 5.4, of which their bytes would take 0.2: the launch, the scan's
+// reads and barriers, the bisection and the reads of length and page behind it, one after the other.
 #include "internal.h"
 #include "paged_cache.h"
 
@@ -172,8 +174,9 @@ __global__ void __launch_bounds__(kThreads) paged_slots_kernel(const PagedSlotsP
 cudaError_t launch_paged_slots(const PagedSlotsParams& p, cudaStream_t stream) {
   const int64_t blocks = p.capacity > kRowsPerBlock ? ((int64_t)p.capacity + kRowsPerBlock - 1) / kRowsPerBlock : 1;
   const int smem = (2 * p.batch + 1) * 4;
-  if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(paged_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (smem > 40 * 1024) {  // (always to the most there can be: calls from several threads would undercut each other)
+    constexpr int kMost = (2 * FBGEMM_B200_PAGED_MAX_BATCH + 1) * 4;
+    const cudaError_t e = cudaFuncSetAttribute(paged_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
     if (e != cudaSuccess) {
       return e;
     }
