@@ -340,7 +340,13 @@ def check_attention(cache, q, tables, lengths, scale=None, window=0, requests=No
         # fp16 numbers below 2^-14 are 2^-24 apart, so a small weight is off by 2^-25; weights are 2^10 times their size
         # relative to a row's that is not above the largest (and beside quantized rows to the largest scale): 2^-35 each.
         small = len(t) * 2.0 ** -35 * (vd.abs().max() if vq is None else vq[0].abs().max() * 128)
-        most = HALF_STEP[q.dtype] * o.abs() + weight * heavy + (2 * off[..., None] + steps) * both + small + 2.0 ** -25
+        # Beside quantized rows the sums are of whole codes, sum w c and middle * sum w, and only their difference is of centred
+        # ones: where that is 0 (codes 8 and 8, w s = 0.29: 2.3 - 2.3, off by 1.2e-7) their own roundings stay.  Each is at most
+        # held = sum p s 2^bits.  A step of 16 rows rounds its sum, by 2^-22 held, and drops what lies 2^-22 below its largest
+        # term, a subnormal code being aligned as 64 (4-bit) or 1024 (8-bit) would be, 4 * 2^bits: over all steps 4 * 2^-22
+        # held; the products with the middle and the unit, the difference and its sum with the biases: 4 * 2^-24 held each side.
+        held = 0 if vq is None else torch.einsum("kgt,tkd->kgd", p, vq[0].abs()) * 2.0 ** bits * (len(t) / 16 + 6) * 2.0 ** -22
+        most = HALF_STEP[q.dtype] * o.abs() + weight * heavy + (2 * off[..., None] + steps) * both + held + small + 2.0 ** -25
         bad = (got - o).abs() - most
         assert (bad <= 0).all(), (b, n, (got - o).abs().max(), bad.max())
         assert ((got_lse - full_lse).abs() <= 2 * off + steps + full_lse.abs() * 2.0 ** -22).all(), (b, n)
@@ -757,6 +763,19 @@ def test_results_into_given_memory():
     big = torch.empty(3, 2, 64, device=DEV).bfloat16()
     with pytest.raises(_capi.Fbgemmb200Error, match="overlaps"):
         paged.rotary_append(cache, big[:2], q[:, :1], q[:, :1], torch.tensor([-1, -1], device=DEV), q_out=big[1:])
+
+
+@pytest.mark.parametrize("bits,kind,kv", [(16, "bf16", 2), (8, "f16", 2), (4, "bf16", 8)])
+def test_attention_of_more_short_items_than_blocks(bits, kind, kv):
+    """Warps take several whole items each, or share one with the next; some have no rows."""
+    rng = np.random.default_rng(bits)
+    lengths = rng.integers(0, 130, 250).tolist()
+    lengths[:4] = [0, 0, 130, 1]
+    tables, pages = place(lengths, 16, rng)
+    cache = make_cache(pages, 16, kv, 128, bits, TYPES[kind])
+    fill(cache)
+    q = torch.randn(len(lengths), 3 * kv, 128, device=DEV).to(TYPES[kind])
+    check_attention(cache, q, torch.from_numpy(tables).to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV))
 
 
 @pytest.mark.parametrize("bits,kind", [(16, "f16"), (4, "bf16")])
