@@ -37,7 +37,8 @@ int main() {
   CHECK(split_units(444 * 39, 444, true).small == 0 && split_units(444 * 40, 444, true).small == 10);
   CHECK(split_units(444 * 40, 444, false).small == 0);
 
-  CHECK(blocks_of_item(0, 1, 444) == 1 && blocks_of_item(127, 1, 444) == 1 && blocks_of_item(512, 1 << 20, 444) == 1);
+  CHECK(blocks_of_item(0, 1, 444) == 1 && blocks_of_item(127, 1, 444) == 1 && blocks_of_item(512, 444, 444) == 1);
+  CHECK(blocks_of_item(512, 445, 444) == 0 && blocks_of_item(1, 1 << 20, 444) == 0);
   CHECK(blocks_of_item(128, 1, 444) == 2 && blocks_of_item(512, 1, 444) == 8 && blocks_of_item(512, 37, 444) == 4);
   CHECK(blocks_of_item(513, 222, 444) == 2 && blocks_of_item(513, 223, 444) == 0);
   CHECK(blocks_of_item(4096, 55, 444) == 8 && blocks_of_item(4096, 56, 444) == 0 && blocks_of_item(4097, 1, 444) == 0);
