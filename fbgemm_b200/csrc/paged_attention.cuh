@@ -41,8 +41,8 @@
 // all work on one item joins theirs first.  Short items are left to a block each, or to a cluster of two, four or eight that
 // joins its results through distributed shared memory: one launch.
 //
-// Measured over 32 requests of 16384 rows of 8 heads of 128 columns: 16-bit rows 323 us, 6.65 TB/s, what a plain copy
-// reaches.  8-bit rows 207 us, 0.84 of that rate, and 4-bit ones 154, 0.57: a tile is half or a quarter of the bytes and
+// Measured over 32 requests of 16384 rows of 8 heads of 128 columns: 16-bit rows 319 to 323 us, 6.7 TB/s, what a plain copy
+// reaches.  8-bit rows 205 us, 0.85 of that rate, and 4-bit ones 150, 0.58: a tile is half or a quarter of the bytes and
 // no fewer instructions (about 700 of a warp for 32 4-bit rows, three warps a scheduler, one instruction in two cycles),
 // whose chain from the scores through the weights to the sums is what a tile takes.  Below some 100 us a fixed 15 us shows:
 // 4 until the first rows are there, the slowest SM's 10 behind the mean one, and the join.
@@ -248,8 +248,8 @@ struct Shape {
   static constexpr int kHeads = kWarpHeads * HW;
   static constexpr int kPartFloats = kHeads * (DP + 2);
   // Blocks of an SM by registers (output 4 NT MT, queries 2 NT KSTEPS, scores, and about 70 more), and ring slots of a warp
-  // by shared memory.  (128 requests of up to 4096 4-bit rows: 68 us with three blocks; 79 with two, 77 with four, whose
-  // registers do not suffice.)
+  // by shared memory.  (128 requests of up to 4096 4-bit rows, before the join went by workers there: 68 us with three blocks, 79
+  // with two, 77 with four, whose registers do not suffice.)
   static constexpr int kRegisters = 4 * NT * MT + 2 * NT * KSTEPS + 4 * NT * SUB;
   static constexpr int kBlocks = kRegisters <= 90 ? 3 : 2;
   static constexpr int kFit = 222 * 1024 / (kBlocks * kWarps * SLOT);

@@ -79,8 +79,8 @@ FBGEMM_B200_HD UnitSplit split_units(int64_t total, int64_t workers, bool two) {
 // units are shared by the whole chip, which takes a second launch and a workspace.  Us by one block a head, by two, by
 // eight, shared by the chip, one request of 8 heads: 1000 rows 18.7, 13.3, 8.2, 11.2; 2000 rows 33.2, -, 10.1, 11.5.  With more
 // items than blocks, a block each and shared: 208 requests of up to 30 16-bit rows 20.2 and 12.3, 128 of 100 17.1 and 14.1, 208
-// of 500 45.5 and 50.1, of 8-bit rows 40.8 and 38.4.  (A block an item up to 2048 rows: 90 instead of 93 for 128 requests of 1000
-// 16-bit rows, but 42 instead of 32 for 64 of 64 to 2000.)
+// of 500 45.5 and 50.1, of 8-bit rows 40.8 and 38.4.  (A block an item up to 2048 rows: 42 instead of 32 for 64 requests of 64 to
+// 2000 rows.)
 FBGEMM_B200_HD int32_t blocks_of_item(int64_t most_rows, int64_t items, int64_t blocks) {
   int32_t n = 1;
   while (n < 8 && ((most_rows > 512 * n && items * 2 * n <= blocks) || (most_rows >= 128 * n && items * 2 * n <= blocks / 3))) {
