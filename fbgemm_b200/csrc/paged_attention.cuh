@@ -131,7 +131,8 @@ __device__ __forceinline__ void load_turned(uint32_t (&r)[4], uint32_t at) {
                : "memory");
 }
 
-// 16 or 4 bytes to shared memory, past the first cache where that is possible; `bytes` 0: zeros instead.
+// 16 or 4 bytes to shared memory, past the first cache where that is possible; only `bytes` of them are read, zeros for the
+// others.
 __device__ __forceinline__ void copy16(uint32_t to, const uint8_t* from, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
@@ -581,9 +582,9 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
           for (int j = 0; j < kRounds; ++j) {
             const int n = lane + 32 * j, r = n / S::kPieces, piece = n - r * S::kPieces;
             const int64_t row = __shfl_sync(kAll, off, min(r, S::ROWS - 1));
-            if (r < S::ROWS) {  // (pieces behind the row's: zeros)
-              copy16(fill_at + r * S::PITCH + piece * 16, rows + row + (piece * 16 < row_bytes ? piece * 16 : 0),
-                     ((seen >> r) & 1) && piece * 16 < row_bytes ? 16 : 0);
+            if (r < S::ROWS) {  // (zeros behind the row's end)
+              const int bytes = (seen >> r) & 1 ? piece_bytes(row_bytes, piece) : 0;
+              copy16(fill_at + r * S::PITCH + piece * 16, rows + row + (bytes ? piece * 16 : 0), bytes);
             }
           }
         } else if (lane < S::ROWS) {

@@ -89,6 +89,13 @@ FBGEMM_B200_HD int32_t blocks_of_item(int64_t most_rows, int64_t items, int64_t 
   return items <= blocks && most_rows <= 512 * n ? n : 0;
 }
 
+// Bytes of a row's 16-byte piece `piece`: what the copies of pages below 16 rows read, so that nothing behind a row is read
+// (strides may be padded without padding behind the last row).
+FBGEMM_B200_HD int32_t piece_bytes(int32_t row_bytes, int32_t piece) {
+  const int32_t n = row_bytes - 16 * piece;
+  return n < 0 ? 0 : n < 16 ? n : 16;
+}
+
 // ---- kernel parameters ------------------------------------------------------------------------------------------------
 
 struct PagedSlotsParams {
