@@ -20,6 +20,7 @@ STATUS_SIZE_MISMATCH = 3
 STATUS_PEER_TIMEOUT = 5
 STATUS_NO_PAGES = 6
 STATUS_BAD_PAGE = 7
+STATUS_COPY_TIMEOUT = 8
 PAGED_MAX_BATCH = 16384
 IPC_HANDLE_BYTES = 64
 NOALLOC_MAX_BAGS = 1 << 20
@@ -191,6 +192,7 @@ SIGNATURES = {
     "fbgemm_b200_paged_attention_workspace": (_i64, [_p, _cachep, _i32, _i32, _i32, _i32, _i32]),
     "fbgemm_b200_paged_attention": (C.c_int, [_p, _cachep, _i32, _i32, _i32, _p, _i64, _i64, _p, _i32, _i64, _p, C.c_float,
                                               _i32, _p, _p, _p, _i64, C.c_int, _p]),
+    "fbgemm_b200_set_copy_limit": (_i64, [_i64]),
     "fbgemm_b200_float_to_fused_8bit_rowwise": (C.c_int, [_p, _i64, C.c_int32, _p, _p]),
     "fbgemm_b200_float_to_fused_nbit_rowwise": (C.c_int, [C.c_int32, _p, _i64, C.c_int32, _p, _p]),
 }

@@ -1,4 +1,6 @@
 // The C ABI of the paged key-value cache: argument checks and launches (include/fbgemm_b200/embedding_c_api.h).
+#include <atomic>
+
 #include "context.h"
 #include "paged_cache.h"
 
@@ -7,6 +9,8 @@ using namespace fbgemm_b200;
 namespace {
 
 constexpr int64_t kMostRows = 0x7fffff00LL;  // of a request, as far as its block table goes
+constexpr int64_t kMostWait = 1000000000;
+std::atomic<int64_t> g_copy_limit{kMostWait};
 
 bool aligned(const void* p, uintptr_t to) {
   return reinterpret_cast<uintptr_t>(p) % to == 0;
@@ -147,6 +151,15 @@ extern "C" {
 
 int fbgemm_b200_paged_cache_check(const fbgemm_b200_paged_cache* cache) try {
   return check_cache(cache);
+} catch (...) {
+  return thrown();
+}
+
+int64_t fbgemm_b200_set_copy_limit(int64_t nanoseconds) try {
+  if (nanoseconds < 0 || nanoseconds > kMostWait) {
+    return refuse("a copy is waited for 0 to 1e9 nanoseconds");
+  }
+  return g_copy_limit.exchange(nanoseconds, std::memory_order_relaxed);
 } catch (...) {
   return thrown();
 }
@@ -417,6 +430,7 @@ int fbgemm_b200_paged_attention(
     p.open = reinterpret_cast<int4*>(p.parts + 2 * plan.part_floats * 2 * plan.workers);
   }
   p.status = ctx->status + 4 * slot;
+  p.copy_limit = (uint32_t)g_copy_limit.load(std::memory_order_relaxed);
   p.most_rows = most;
   p.scale_log2 = (float)((double)scale * 1.4426950408889634);
   p.num_pages = (int32_t)cache->num_pages;

@@ -67,6 +67,7 @@ namespace paged {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
+constexpr uint32_t kLateCopy = 1000000;  // nanoseconds that a copy which is late gets once more
 constexpr int kByItem = 6;  // workers to an item from which on the join goes by items
 
 // Weights are 2^kShift times as large as in the formula and at most 2^kSlack above their reference: 2^14 at most, and with
@@ -161,14 +162,12 @@ __device__ __forceinline__ uint64_t nanoseconds() {
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
   return t;
 }
-// Waits for a phase of the barrier, for a second at most, and once one has not come in time for a millisecond: so that a
-// warp meets all its copies, late ones too, and still ends.  False: it did not come.
-__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, uint32_t& limit) {
+// Waits for a phase of the barrier, for `limit` nanoseconds at most.  False: it did not come.
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, uint32_t limit) {
   if (!barrier_try(bar, parity)) {
     const uint64_t since = nanoseconds();
     while (!barrier_try(bar, parity)) {
       if (nanoseconds() - since > limit) {
-        limit = 1000000;
         return false;
       }
     }
@@ -396,7 +395,8 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   // The ring: what is filled next and what is worked on.
   uint32_t fill_at = ring_at, at = ring_at;
   int fill_slot = 0, slot = 0;
-  uint32_t phase = 0, limit = 1000000000;
+  uint32_t phase = 0;
+  bool lost = false;  // a copy did not come in time: the warp leaves
 
   // A place in the line of units: tile u of an item (a cached head and a tile of its query heads) of a request.
   struct Place {
@@ -605,15 +605,36 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
   };
-  // The half tile that is worked on next is there, and the one before has been read by all lanes.
+  // The half tile that is worked on next is there, and the one before has been read by all lanes.  False: it did not come in
+  // time, as far as this lane can tell.
   auto arrived = [&] {
+    bool came = true;
     if constexpr (FAST) {
-      if (!barrier_wait(bars + 8 * slot, phase, limit) && atomicCAS(p.status, 0, FBGEMM_B200_STATUS_COPY_TIMEOUT) == 0) {
-        p.status[1] = now.request;
-      }
+      came = barrier_wait(bars + 8 * slot, phase, p.copy_limit);
     } else {
       asm volatile("cp.async.wait_group %0;" ::"n"(S::SLOTS - 2) : "memory");
     }
+    __syncwarp();
+    return came;
+  };
+  // A half tile did not come in time, the one at `from` or one behind it.  No copy is asked for any more, so that no barrier is
+  // armed again whose phase has not ended, and those that were asked for are waited for once more: one that comes up to
+  // kLateCopy later still finds its memory there.
+  auto give_up = [&](int from, uint32_t parity) {
+    if (lane == 0 && atomicCAS(p.status, 0, FBGEMM_B200_STATUS_COPY_TIMEOUT) == 0) {
+      p.status[1] = now.request;
+      p.status[2] = p.status[3] = 0;
+    }
+    lost = true;
+    fill_more = false;
+    to_read = 0;
+    do {  // (at least one, at most all)
+      barrier_wait(bars + 8 * from, parity, kLateCopy);
+      if (++from == S::SLOTS) {
+        from = 0;
+        parity ^= 1;
+      }
+    } while (from != fill_slot);
     __syncwarp();
   };
   read_pages();
@@ -623,12 +644,15 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   }
   int4 opened = make_int4(0, 0, 0, 0);
   const bool idle = left == 0;
+  if (FAST && p.copy_limit == 0 && !idle) {
+    give_up(slot, phase);
+  }
 
   // -- item after item
   while (left > 0) {
     const int request = now.request, item = now.item;
     const bool begins = now.u == 0, ends = now.units - now.u <= left, none = now.span.end == now.span.first;
-    const int tiles = ends ? now.units - now.u : left;
+    const int tiles = lost ? 0 : ends ? now.units - now.u : left;
     const int kv_head = item / p.head_tiles, first_head = (item - kv_head * p.head_tiles) * S::kHeads + head_warp * S::kWarpHeads;
     const int heads = min(p.group - first_head, S::kWarpHeads);  // of this warp, may be none
     const int q_head0 = kv_head * p.group + first_head;
@@ -781,8 +805,8 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
 
     for (int i = 0; i < tiles; ++i) {
       // -- scores
-      arrived();
-      fill(S::SLOTS % 2 == 0);
+      bool late = !arrived();
+      fill(S::SLOTS % 2 == 0);  // (into the half before, which has come)
       float sc[NT][SUB][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -863,8 +887,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
       advance();
 
       // -- weights
-      arrived();
-      fill(S::SLOTS % 2 != 0);
+      late |= !arrived();
       if (kSwizzled && rows_seen != kFull) {  // whatever else the page holds: weights of 0 do not make up for infinities
         for (int n = lane; n < S::SLOT_FAST / 16; n += 32) {
           const int row = (n / 8) % 16 + 16 * (n / (S::kBoxes * 128));
@@ -875,7 +898,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
-      bool more = false;
+      bool more = FAST && late;
       float top[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -917,6 +940,10 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
         more |= largest >= scale_limit;
       }
       if (__any_sync(kAll, more)) {
+        if (FAST && __any_sync(kAll, late)) {  // (this tile's halves from K's on: V's is at `slot`)
+          give_up(slot == 0 ? S::SLOTS - 1 : slot - 1, slot == 0 ? phase ^ 1 : phase);
+          break;
+        }
         float fade_scale = 1.f;
         if constexpr (kQuantized) {
           const int to = (int)min(__reduce_max_sync(kAll, __float_as_uint(largest) >> 23), 253u);
@@ -955,6 +982,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
           }
         }
       }
+      fill(S::SLOTS % 2 != 0);  // (into K's half, which has come, as that question has shown)
       uint32_t wt[NT][SUB][2];
 #pragma unroll
       for (int s = 0; s < SUB; ++s) {
@@ -1109,7 +1137,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
       const int64_t last = last_unit - left + now.units - 1;
       opened = make_int4((int)(split.worker_of(last) - worker), request, item, 0);
     }
-    left -= tiles;
+    left = lost ? 0 : left - tiles;
     if (left > 0) {
       next_item(now);
     }

@@ -149,6 +149,7 @@ struct PagedAttentionParams {
   float* parts;                                   // partial results, two per worker
   int4* open;                                     // per worker: the item that it began and others end
   int32_t* status;
+  uint32_t copy_limit;                            // nanoseconds that a copy of the kernel's own is waited for
   int64_t most_rows;                              // rows that a block table names
   float scale_log2;                               // softmax scale * log2(e)
   int32_t num_pages, page_shift, batch, kv_heads, group, head_tiles, dim, window, workers;  // workers of the first size

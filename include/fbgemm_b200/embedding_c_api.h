@@ -1032,6 +1032,16 @@ FBGEMM_B200_API int fbgemm_b200_paged_attention(
     int slot,
     void* stream);
 
+/*
+ * How long paged_attention's kernel waits for a copy of its own, in
+ * nanoseconds: 1e9, the most, unless set.  A copy that has not come by then is
+ * recorded (COPY_TIMEOUT, request, 0, 0) and the call's results are void; the
+ * kernel asks for no more copies, gives those under way another millisecond
+ * each, and ends.  0: as if none came in time (tests).  Process-wide, for calls
+ * from then on.  Returns the value before, or a negative code.
+ */
+FBGEMM_B200_API int64_t fbgemm_b200_set_copy_limit(int64_t nanoseconds);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -1,8 +1,11 @@
 """The paged key-value cache at its edges, without a GPU."""
 import os
+import re
 import subprocess
 
-from fbgemm_b200 import build
+import pytest
+
+from fbgemm_b200 import _capi, build
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -14,3 +17,19 @@ def test_rules_at_the_edges(tmp_path):
                     os.path.join(ROOT, "tests", "cpp", "paged_edges_test.cc"), "-o", exe], check=True)
     res = subprocess.run([exe], capture_output=True, text=True, timeout=60)
     assert res.returncode == 0, res.stdout
+
+
+def test_status_codes_are_the_headers():
+    header = open(os.path.join(build.INCLUDE, "fbgemm_b200", "embedding_c_api.h")).read()
+    codes = dict(re.findall(r"#define FBGEMM_B200_(STATUS_[A-Z_]+) (\d+) ", header))
+    assert codes["STATUS_COPY_TIMEOUT"] == "8"
+    for name, value in codes.items():
+        assert getattr(_capi, name, int(value)) == int(value), name
+    assert _capi.STATUS_COPY_TIMEOUT == 8
+
+
+@pytest.mark.parametrize("wrong", [-1, 10 ** 9 + 1, 2 ** 32])
+def test_copy_limit_refuses(wrong):
+    lib = _capi.lib()
+    assert lib.fbgemm_b200_set_copy_limit(wrong) == _capi.EINVAL and "nanoseconds" in _capi.last_error()
+    assert lib.fbgemm_b200_set_copy_limit(10 ** 9) == 10 ** 9
