@@ -425,15 +425,14 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   if (p.cluster) {
     together = block_begins = block_ends = true;
   } else if constexpr (S::kWorkers > 1) {
-    const int64_t block_first = split.first((int64_t)blockIdx.x * S::kWorkers), per = split.units_of(blockIdx.x * S::kWorkers);
-    const int64_t block_units = min(block_first + S::kWorkers * per, total) - block_first;
+    const BlockShare share = block_share(split, blockIdx.x, S::kWorkers, total);
     const int units = units_of(span_of(p.lengths[sm_request[0]], p.window, p.most_rows), S::UNIT);
     const int u = (int)(sm_unit[0] % units);
-    together = block_units > per && u + block_units <= units;
+    together = share.active > 1 && u + share.units <= units;
     block_begins = u == 0;
-    block_ends = u + block_units == units;
+    block_ends = u + share.units == units;
     block_item = (int)(sm_unit[0] / units);
-    block_active = (int)((block_units + per - 1) / per);
+    block_active = share.active;
   }
 
   // -- half tiles come in turn: K and V of a tile, then of the next.  SLOTS - 1 are on their way, and the pages of the tile

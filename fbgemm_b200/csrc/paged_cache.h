@@ -74,6 +74,23 @@ FBGEMM_B200_HD UnitSplit split_units(int64_t total, int64_t workers, bool two) {
   return s;
 }
 
+// What a block's neighbouring workers have together, and how many of them have any; nothing behind the last unit (a block of the
+// second set where there is none).
+struct BlockShare {
+  int64_t units;
+  int32_t active;
+};
+FBGEMM_B200_HD BlockShare block_share(const UnitSplit& s, int64_t block, int32_t workers, int64_t total) {
+  const int64_t first = s.first(block * workers), per = s.units_of(block * workers);
+  const int64_t end = first + workers * per < total ? first + workers * per : total;
+  BlockShare r = {0, 0};
+  if (per > 0 && end > first) {
+    r.units = end - first;
+    r.active = (int32_t)((r.units + per - 1) / per);
+  }
+  return r;
+}
+
 // Blocks that take an item, as far as the host knows its length: one for 512 rows, as many as that takes for more, as long as
 // all of them are on the chip at once; and more, up to eight, down to 64 rows each, while every one has an SM to itself.  0: the
 // units are shared by the whole chip, which takes a second launch and a workspace.  Us by one block a head, by two, by

@@ -28,8 +28,37 @@ static void pieces() {
   }
 }
 
+// Blocks' shares are all units, each once; blocks of a second set that has none, or behind the last unit, have no share.
+static void blocks() {
+  for (int64_t total : {1, 5, 443, 444, 4440, 17000, 17760, 17761, 60000, 1000000}) {
+    for (int32_t of_block : {2, 4}) {
+      for (bool two : {false, true}) {
+        const int64_t blocks = 444 / of_block;
+        const UnitSplit s = split_units(total, blocks * of_block, two);
+        int64_t sum = 0;
+        for (int64_t b = 0; b < 2 * blocks; ++b) {
+          const BlockShare share = block_share(s, b, of_block, total);
+          int64_t units = 0;
+          int32_t active = 0;
+          for (int32_t w = 0; w < of_block; ++w) {  // worker by worker
+            const int64_t first = s.first(b * of_block + w), end = first + s.units_of(b * of_block + w);
+            const int64_t n = (end < total ? end : total) - first;
+            units += n > 0 ? n : 0;
+            active += n > 0;
+          }
+          CHECK(share.units == units && share.active == active);
+          CHECK(b < blocks || s.small > 0 || share.active == 0);
+          sum += share.units;
+        }
+        CHECK(sum == total);
+      }
+    }
+  }
+}
+
 int main() {
   pieces();
+  blocks();
   std::printf(failures ? "%d failures\n" : "ok\n", failures);
   return failures != 0;
 }
