@@ -52,6 +52,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cfloat>
+
 #include "internal.h"
 #include "paged_cache.h"
 
@@ -650,7 +652,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   // -- item after item
   while (left > 0) {
     const int request = now.request, item = now.item;
-    const bool begins = now.u == 0, ends = now.units - now.u <= left, none = now.span.end == now.span.first;
+    const bool begins = now.u == 0, ends = now.units - now.u <= left;
     const int tiles = lost ? 0 : ends ? now.units - now.u : left;
     const int kv_head = item / p.head_tiles, first_head = (item - kv_head * p.head_tiles) * S::kHeads + head_warp * S::kWarpHeads;
     const int heads = min(p.group - first_head, S::kWarpHeads);  // of this warp, may be none
@@ -802,6 +804,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
       }
     };
 
+    unsigned any_seen = 0;
     for (int i = 0; i < tiles; ++i) {
       // -- scores
       bool late = !arrived();
@@ -869,6 +872,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
         }
       }
       const unsigned rows_seen = sm_seen[warp][slot];
+      any_seen |= rows_seen;
       if (rows_seen != kFull) {
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
@@ -1052,7 +1056,10 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
       advance();
     }
 
-    // -- this warp's result: whole, or a part of one
+    // -- this warp's result: whole, or a part of one.  No row at all, or none on a page of the cache: zeros, and -inf as the
+    // maximum.  Rows whose scores are all -inf: 0 / 0, as in the formula; the lowest finite maximum tells other parts that there
+    // are such.
+    const bool none = any_seen == 0;
     float scale_l[NT][2], scale_o[NT][2], add_o[NT][2];
     const bool whole = begins && ends && !together;
     const float unit = kQuantized ? __uint_as_float((uint32_t)exponent << 23) : 1.f;
@@ -1071,7 +1078,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
             sum_b += __shfl_xor_sync(kAll, sum_b, d);
           }
         }
-        const float inv = !whole ? 1.f : none ? 0.f : __fdiv_rn(1.f, sum_l);  // no row at all: zeros
+        const float inv = !whole ? 1.f : none ? 0.f : __fdiv_rn(1.f, sum_l);
         scale_l[n][x] = sum_l;
         scale_o[n][x] = inv;
         add_o[n][x] = sum_b;
@@ -1095,7 +1102,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
         const int in_part = head_warp * S::kWarpHeads + h;
         if (g == 0) {
           if (!whole) {
-            part[in_part] = m[n][x];
+            part[in_part] = m[n][x] == -INFINITY && !none ? -FLT_MAX : m[n][x];
             part[S::kHeads + in_part] = scale_l[n][x];
           } else if (p.lse) {
             const float from = m[n][x] == -INFINITY ? 0.f : m[n][x];
@@ -1149,13 +1156,12 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
       __syncthreads();
     }
     __syncthreads();
-    const RowSpan span = span_of(p.lengths[sm_request[0]], p.window, p.most_rows);
-    const bool none = span.end == span.first;
     const int kv_head = block_item / p.head_tiles, first_head = (block_item - kv_head * p.head_tiles) * S::kHeads;
     const int heads = min(p.group - first_head, S::kHeads);
     const float* const parts = reinterpret_cast<const float*>(smem);
-    auto results_out = [&](int h, int column, float4 v, float from, float sum_l) {
-      const float inv = none ? 0.f : __fdiv_rn(1.f, sum_l);  // no row at all: zeros
+    auto results_out = [&](int h, int column, float4 v, float top, float sum_l) {
+      const bool none = top == -INFINITY;
+      const float inv = none ? 0.f : __fdiv_rn(1.f, sum_l);
       const int64_t row = ((int64_t)sm_request[0] * p.kv_heads + kv_head) * p.group + first_head + h;
       if (column < p.dim) {
         *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + (row * p.dim + column) * 2) =
@@ -1163,7 +1169,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
                        pack<BF16>(__fmul_rn(v.z, inv), __fmul_rn(v.w, inv)));
       }
       if (column == 0 && p.lse) {
-        p.lse[row] = none ? -INFINITY : __fmaf_rn(from, kLn2, logf(__fmul_rn(sum_l, kUnshift)));
+        p.lse[row] = none ? -INFINITY : __fmaf_rn(top, kLn2, logf(__fmul_rn(sum_l, kUnshift)));
       }
     };
     const bool whole = block_begins && block_ends;
@@ -1189,7 +1195,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
         v.w = __fmaf_rn(f, x.w, v.w);
       }
       if (whole && p.cluster <= 1) {
-        results_out(h, column, v, from, sum_l);
+        results_out(h, column, v, top, sum_l);
       } else {
         *reinterpret_cast<float4*>(part + 2 * S::kHeads + h * S::DP + column) = v;
         if (column == 0) {
@@ -1219,7 +1225,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
           v.z = __fmaf_rn(f, x.z, v.z);
           v.w = __fmaf_rn(f, x.w, v.w);
         }
-        results_out(h, column, v, from, sum_l);
+        results_out(h, column, v, top, sum_l);
       }
       cluster_sync();  // (a block's memory is there until all have read it)
     }
@@ -1397,7 +1403,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join(const PagedAtte
         top = all;
       }
       const int64_t row = ((int64_t)request * p.kv_heads + kv_head) * p.group + first_head + h;
-      const float inv = __fdiv_rn(1.f, sum_l);
+      const float inv = top == -INFINITY ? 0.f : __fdiv_rn(1.f, sum_l);  // (no row on a page of the cache: zeros)
 #pragma unroll
       for (int j = 0; j < kCols; j += 2) {
         const int column = 32 * j + 2 * lane;

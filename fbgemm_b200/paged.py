@@ -236,7 +236,8 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, block_tables: torch.Te
 
     Scores, sums and the output are fp32 until the output's one rounding; the
     weights enter the sum over rows as 16-bit numbers.  A page outside the cache
-    is left out (status {7, request, row, page}); a length that is negative or
+    is left out (status {7, request, row, page}; all of a request's pages: a
+    request without rows); a length that is negative or
     beyond the table is brought within it (status {3, request, 0, length})."""
     if out is None:
         out = torch.empty_like(q, memory_format=_CONTIGUOUS)

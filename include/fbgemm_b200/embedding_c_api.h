@@ -1005,7 +1005,7 @@ FBGEMM_B200_API int64_t fbgemm_b200_paged_attention_workspace(
  * seen does not matter.  q and out are dtype (FBGEMM_B200_OUT_F16 or _BF16, a
  * 16-bit cache's own); q strides in elements are multiples of 8.
  * A page outside the cache is recorded (BAD_PAGE, request, row, page) and its
- * rows are left out; a negative length, or one beyond the table, is recorded
+ * rows are left out, all of them as if there were none; a negative length, or one beyond the table, is recorded
  * (SIZE_MISMATCH, request, 0, length) and brought within it.  width *
  * page_size <= 2^31 - 256.  out does not overlap q.  At most two launches,
  * nothing allocated.

@@ -1,6 +1,8 @@
 """The paged key-value cache on the GPU at its edges: memory that ends with the
 last row, tables without a good page, numbers at the ends of their ranges, the
 forms that only large calls take."""
+import math
+
 import pytest
 import torch
 
@@ -72,3 +74,81 @@ def test_a_copy_that_does_not_come_in_time(no_copy_in_time, bits, batch, rows, h
     assert not ok and info[0] == _capi.STATUS_COPY_TIMEOUT and 0 <= info[1] < batch and info[2:] == [0, 0]
     assert no_copy_in_time(10 ** 9) == 0
     assert torch.equal(paged.paged_attention(cache, q, tables, lengths), want) and F.status_read(0)[0]
+
+
+# ---- nothing left of a request -----------------------------------------------
+
+# items that are whole ones of a warp, of a block, of a cluster; that neighbours share; that the chip shares
+LEFT = [(1, 16, 2, 1), (3, 60, 4, 1), (2, 1500, 8, 2), (1, 20_000, 8, 2), (300, 100, 8, 2), (300, 700, 16, 2), (60, 2500, 24, 1)]
+
+
+@pytest.mark.parametrize("batch,rows,heads,kv", LEFT)
+@pytest.mark.parametrize("bits,page", [(16, 16), (16, 8), (8, 64), (8, 4), (4, 32)])
+def test_a_request_whose_pages_are_all_bad(batch, rows, heads, kv, bits, page):
+    """Its rows are left out, so there are none: zeros and -inf.  The other requests are as they were."""
+    pages = 3200 // page
+    cache = paged.PagedKVCache.allocate(pages, page, kv, 64, dtype=torch.bfloat16, bit_rate=None if bits == 16 else bits, device=DEV)
+    fill(cache)
+    q = torch.randn(batch, heads, 64, device=DEV).bfloat16()
+    tables = torch.randint(0, pages, (batch, -(-rows // page)), device=DEV, dtype=torch.int32)
+    lengths = torch.full((batch,), rows, dtype=torch.int32, device=DEV)
+    want, want_lse = paged.paged_attention(cache, q, tables, lengths, return_lse=True)
+    assert F.status_read(0)[0]
+    hit = torch.zeros(batch, dtype=torch.bool)
+    hit[::7] = True
+    hit = hit.to(DEV)
+    for value in (-1, pages):
+        bad = torch.where(hit[:, None], value, tables)
+        got, lse = paged.paged_attention(cache, q, bad, lengths, return_lse=True)
+        ok, info = F.status_read(0)
+        assert not ok and info[0] == _capi.STATUS_BAD_PAGE and info[1] % 7 == 0 and info[3] == value
+        assert (got[hit] == 0).all() and (lse[hit] == -math.inf).all()
+        assert torch.equal(got[~hit], want[~hit]) and torch.equal(lse[~hit], want_lse[~hit])
+    # one row left: its value
+    bad[0, -1] = tables[0, -1]
+    last = (rows - 1) % page
+    lengths[0] = rows - last
+    got, lse = paged.paged_attention(cache, q[:1], bad[:1], lengths[:1], return_lse=True)
+    F.status_read(0)
+    one, one_lse = paged.paged_attention(cache, q[:1], tables[:1, -1:].contiguous(), torch.ones_like(lengths[:1]), return_lse=True)
+    assert torch.equal(got, one) and torch.equal(lse, one_lse)
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+def test_a_window_over_bad_pages_alone(bits):
+    cache = paged.PagedKVCache.allocate(8, 16, 2, 64, bit_rate=None if bits == 16 else bits, device=DEV)
+    fill(cache)
+    q = torch.randn(2, 4, 64, device=DEV).bfloat16()
+    tables = torch.tensor([[0, 1, 8, -1], [2, 3, 4, 5]], dtype=torch.int32, device=DEV)
+    lengths = torch.tensor([60, 60], dtype=torch.int32, device=DEV)
+    for window in (1, 12, 13, 28):
+        got, lse = paged.paged_attention(cache, q, tables, lengths, window=window, return_lse=True)
+        ok, info = F.status_read(0)
+        assert not ok and info[:2] == [_capi.STATUS_BAD_PAGE, 0] and 60 - window <= info[2] < 60
+        assert (got[0] == 0).all() and (lse[0] == -math.inf).all()
+        want = paged.paged_attention(cache, q[1:], tables[1:], lengths[1:], window=window)
+        assert F.status_read(0)[0] and (got[1].float() - want[0].float()).abs().max() <= 5 * 2 * 2.0 ** -8   # (another split)
+
+
+@pytest.mark.parametrize("rows", [10, 60, 1500, 20_000])
+def test_scores_that_are_all_minus_infinity(rows):
+    """Rows that are there, unlike none: 0 / 0, as in the formula; with one finite score among them that row's value."""
+    cache = paged.PagedKVCache.allocate(1250, 16, 1, 64, dtype=torch.bfloat16, device=DEV)
+    fill(cache)
+    cache.k.zero_()
+    cache.k[..., 0] = -math.inf
+    q = torch.ones(1, 4, 64, device=DEV).bfloat16()
+    tables = torch.arange(1250, dtype=torch.int32, device=DEV)[None]
+    tables = tables[:, :-(-rows // 16)].contiguous()
+    lengths = torch.tensor([rows], dtype=torch.int32, device=DEV)
+    got, lse = paged.paged_attention(cache, q, tables, lengths, return_lse=True)
+    assert got.isnan().all() and (lse == -math.inf).all()
+    if rows > 100:
+        tables[0, :3] = -1                     # some rows left out, the others as before
+        got, lse = paged.paged_attention(cache, q, tables, lengths, return_lse=True)
+        assert got.isnan().all() and (lse == -math.inf).all() and not F.status_read(0)[0]
+    at = rows - 2
+    cache.k[at // 16, at % 16, 0, 0] = 0
+    got, lse = paged.paged_attention(cache, q, tables, lengths, return_lse=True)
+    F.status_read(0)
+    assert torch.equal(got[0], cache.v[at // 16, at % 16].expand(4, 64)) and (lse.abs() <= 2.0 ** -20).all()
