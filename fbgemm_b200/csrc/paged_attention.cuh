@@ -76,6 +76,7 @@ constexpr int kByItem = 6;  // workers to an item from which on the join goes by
 // a scale of less than 2 below 2^15.
 constexpr float kShift = 10.f, kSlack = 4.f;
 constexpr float kUnshift = 1.f / 1024.f;
+constexpr float kFar = 1152921504606846976.f;  // 2^60
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -702,6 +703,9 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     }
 
     float factor[NT][2], q_sum[NT][2];  // heads 2c and 2c + 1
+    // Heads (a bit of 2 n + x each) of queries so large that their factor is no fp32 number: 2^-60 of it is kept, and their
+    // scores are multiplied twice.
+    unsigned far = 0;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float scale_head = 1.f, sum_head = 0.f;
@@ -753,14 +757,20 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int from = 4 * (2 * c + x);
-        factor[n][x] = __fmul_rn(__shfl_sync(kAll, scale_head, from), p.scale_log2);
+        const float scale_x = __shfl_sync(kAll, scale_head, from);
+        factor[n][x] = __fmul_rn(scale_x, p.scale_log2);
         if constexpr (kQuantized) {
           factor[n][x] = __fmul_rn(factor[n][x], 1.f / kCode);
+          if (BF16 && isinf(factor[n][x])) {
+            factor[n][x] = __fmul_rn(__fmul_rn(__fmul_rn(scale_x, 1.f / kFar), p.scale_log2), 1.f / kCode);
+            far |= 1u << (2 * n + x);
+          }
           q_sum[n][x] = __fmul_rn(__shfl_sync(kAll, sum_head, from), kCode);
         }
       }
     }
 
+    const bool any_far = kQuantized && BF16 && __any_sync(kAll, far != 0);
     float o[NT][S::MT][4];
     // m: what weights are relative to, base = m - kShift; l: their sum over this lane's rows; of the rounded weights
     // w_sum, of the weights times the rows' biases bias_sum
@@ -867,6 +877,18 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
                 v = __fmaf_rn(sb.x, v, __fmul_rn(sb.y, q_sum[n][x]));
               }
               v = __fmul_rn(v, factor[n][x]);
+            }
+          }
+        }
+      }
+      if (any_far) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int s = 0; s < SUB; ++s) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              sc[n][s][j] = __fmul_rn(sc[n][s][j], (far >> (2 * n + j % 2)) & 1 ? kFar : 1.f);
             }
           }
         }

@@ -9,7 +9,7 @@ import torch
 import fbgemm_b200 as F
 from fbgemm_b200 import _capi, paged
 
-from test_paged_gpu import DEV, TYPES, check_attention, fill
+from test_paged_gpu import DEV, TYPES, check_attention, fill, values
 
 pytestmark = pytest.mark.gpu
 
@@ -152,3 +152,48 @@ def test_scores_that_are_all_minus_infinity(rows):
     got, lse = paged.paged_attention(cache, q, tables, lengths, return_lse=True)
     F.status_read(0)
     assert torch.equal(got[0], cache.v[at // 16, at % 16].expand(4, 64)) and (lse.abs() <= 2.0 ** -20).all()
+
+
+# ---- numbers at the ends of their ranges -------------------------------------
+
+@pytest.mark.parametrize("scale", [1.0, 0.125, 2.0, 2.0 ** 20])
+@pytest.mark.parametrize("rows", [1, 77, 1500, 9000])
+def test_queries_of_the_whole_range_of_bf16(rows, scale):
+    """8-bit keys so small that the scores of queries up to 2^123 are ordinary; smaller queries beside them."""
+    cache = paged.PagedKVCache.allocate(600, 16, 1, 64, bit_rate=8, device=DEV)
+    fill(cache)
+    codes = torch.randint(0, 256, (600, 16, 1, 64), device=DEV, dtype=torch.uint8)
+    cache.k[..., :64] = codes
+    cache.k[..., 64:] = torch.tensor([2.0 ** -120, -127.0 * 2.0 ** -120], device=DEV).view(torch.uint8)
+    q = torch.randn(2, 10, 64, device=DEV)
+    q[:, :3] *= 2.0 ** 114 / scale      # scores of 114 - 120 binary places, 8 columns' worth of 73 on average: about 9
+    q[:, 3] *= 2.0 ** 118 / scale
+    q[1, 4] *= 2.0 ** -100
+    q[1, 5] *= 2.0 ** 100
+    tables = torch.randint(0, 600, (2, -(-rows // 16)), device=DEV, dtype=torch.int32)
+    out, lse = check_attention(cache, q.bfloat16(), tables, torch.tensor([rows, max(1, rows - 5)], dtype=torch.int32, device=DEV), scale=scale)
+    assert out.isfinite().all() and lse.isfinite().all()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_the_largest_queries_beside_quantized_rows(bits):
+    """Scores of 2^120 and more: the largest takes all the weight."""
+    cache = paged.PagedKVCache.allocate(4, 16, 1, 64, bit_rate=bits, device=DEV)
+    fill(cache)
+    q = torch.randn(1, 8, 64, device=DEV) * 2.0 ** 117
+    q[0, 4:] *= 2.0 ** 3
+    q = q.bfloat16()
+    tables = torch.arange(4, dtype=torch.int32, device=DEV)[None]
+    out, lse = paged.paged_attention(cache, q, tables, torch.tensor([60], dtype=torch.int32, device=DEV), scale=0.125, return_lse=True)
+    assert F.status_read(0)[0]
+    (k, _), (v, (step, code, _)) = (values(x.reshape(64, -1)[:60], bits, 64) for x in (cache.k, cache.v))
+    score = q[0].double() @ k.T * 0.125
+    top, at = score.max(-1)
+    # (a score is off by 2^-18 of the sum of its terms' sizes; the second largest is further away)
+    second = score.scatter(-1, at[:, None], -math.inf).amax(-1)
+    assert ((top - second) > 2.0 ** -18 * (q[0].double().abs() @ k.abs().T).amax(-1) * 0.125 * 4).all()
+    # One weight of 1, which enters times the row's scale as fp16: off by 2^-11 of scale * (code - middle), the rest of the value,
+    # bias + scale * middle, is added in fp32 (sums of whole codes: 2^-18 of the largest value), and the sum is rounded once.
+    weight = 2.0 ** -11 * (step * code)[at].abs()
+    assert ((out[0].double() - v[at]).abs() <= 2.0 ** -8 * v[at].abs() + weight + 2.0 ** -18 * v.abs().max()).all()
+    assert ((lse[0].double() - top).abs() <= 2.0 ** -18 * (q[0].double().abs() @ k.abs().T).amax(-1) * 0.125).all()
