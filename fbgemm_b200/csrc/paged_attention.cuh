@@ -28,7 +28,7 @@
 //
 // One pass with a running maximum and sum per head in fp32 (in registers, per warp).  A tile's largest score is looked
 // for across lanes only if one exceeds the running maximum by more than 2^kSlack.  Weights are rounded to 16 bits for
-// the second product: bf16 beside bf16 rows; fp16 (2^kShift times as large, so that weights down to 2^-24 of the largest
+// the second product: bf16 beside bf16 rows; fp16 (2^10 times as large, so that weights down to 2^-24 of the largest
 // keep all 11 bits) otherwise, with the quantized rows' scales taken relative to the largest power of two seen so far.
 // A weight's rounding is at most half a step of the output's own type, and averages out over the rows; codes are weighed
 // about the middle of their range (sum w (c - 128) = sum w c - 128 sum w, with the rounded w), which keeps it there.
@@ -72,10 +72,15 @@ constexpr int kThreads = 32 * kWarps;
 constexpr uint32_t kLateCopy = 1000000;  // nanoseconds that a copy which is late gets once more
 constexpr int kByItem = 6;  // workers to an item from which on the join goes by items
 
-// Weights are 2^kShift times as large as in the formula and at most 2^kSlack above their reference: 2^14 at most, and with
-// a scale of less than 2 below 2^15.
-constexpr float kShift = 10.f, kSlack = 4.f;
-constexpr float kUnshift = 1.f / 1024.f;
+// Weights are at most 2^kSlack above their reference, and as fp16 numbers 2^10 times as large as in the formula: 2^14 at most,
+// and with a scale of less than 2 below 2^15.  16-bit rows take the power of two into the reference (kShift), quantized ones
+// into their scales.
+constexpr float kSlack = 4.f;
+template <typename S>
+struct Weights {
+  static constexpr float kShift = S::BITS == 16 ? 10.f : 0.f;
+  static constexpr float kUnshift = S::BITS == 16 ? 1.f / 1024.f : 1.f;
+};
 constexpr float kFar = 1152921504606846976.f;  // 2^60
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr unsigned kAll = 0xffffffffu;
@@ -273,6 +278,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   constexpr int BITS = S::BITS, NT = S::NT, SUB = S::SUB;
   constexpr bool kQuantized = BITS != 16;
   constexpr bool kMmaBf16 = !kQuantized && BF16;
+  constexpr float kShift = Weights<S>::kShift, kUnshift = Weights<S>::kUnshift;
   constexpr float kMiddle = BITS == 8 ? 128.f : 8.f;
   constexpr float kCode = BITS == 4 ? 1.f / 1048576.f : 1.f / 16777216.f;  // what a code of 1 is to the products
   constexpr unsigned kFull = S::ROWS == 32 ? kAll : (1u << (S::ROWS & 31)) - 1;
@@ -772,7 +778,8 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
 
     const bool any_far = kQuantized && BF16 && __any_sync(kAll, far != 0);
     float o[NT][S::MT][4];
-    // m: what weights are relative to, base = m - kShift; l: their sum over this lane's rows; of the rounded weights
+    // m: what weights are relative to, base = m - kShift (m itself where m - kShift is rounded by one and more: from 2^24 on
+    // scores are that far apart); l: their sum over this lane's rows; of the rounded weights
     // w_sum, of the weights times the rows' biases bias_sum
     float m[NT][2], base[NT][2], l[NT][2], w_sum[NT][2], bias_sum[NT][2];
 #pragma unroll
@@ -788,9 +795,9 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
         l[n][x] = w_sum[n][x] = bias_sum[n][x] = 0.f;
       }
     }
-    // V's scales are taken relative to 2^(exponent - 127) = 1 / v_unit, and are below scale_limit, twice that.
-    int exponent = 1;
-    float v_unit = __uint_as_float(253u << 23), scale_limit = __uint_as_float(2u << 23);
+    // V's scales are taken relative to 2^(exponent - 127) = 2^10 / v_unit, and are below scale_limit, twice that.
+    int exponent = 11;
+    float v_unit = __uint_as_float(253u << 23), scale_limit = __uint_as_float(12u << 23);
 
     auto advance = [&] {
       at += kSlot;
@@ -934,7 +941,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
           for (int s = 1; s < SUB; ++s) {
             top[n][x] = fmaxf(top[n][x], fmaxf(sc[n][s][x], sc[n][s][2 + x]));
           }
-          more |= top[n][x] > m[n][x] + kSlack;
+          more |= top[n][x] - m[n][x] > kSlack;  // (a difference of close numbers is exact)
         }
       }
       float2 v_sb[SUB][2];
@@ -976,7 +983,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
             fade_scale = to - exponent > 126 ? 0.f : __uint_as_float((uint32_t)(127 - (to - exponent)) << 23);
             exponent = to;
             scale_limit = __uint_as_float((uint32_t)(exponent + 1) << 23);
-            v_unit = __uint_as_float((uint32_t)(254 - exponent) << 23);
+            v_unit = __uint_as_float((uint32_t)(264 - exponent) << 23);
           }
         }
 #pragma unroll
@@ -990,9 +997,13 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
             t = fmaxf(t, m[n][x]);
             const float b = t == -INFINITY ? 0.f : t;  // nothing seen yet: every weight is 0
             // (a largest score of +inf: inf - inf, so that the row becomes NaN as in the formula)
-            const float fade = m[n][x] == t ? 1.f : exp2_of(m[n][x] - b);
+            float to = b - kShift;
+            if (kShift != 0.f && fabsf(b - to - kShift) >= 1.f) {
+              to = b;
+            }
+            const float fade = m[n][x] == t ? 1.f : m[n][x] == -INFINITY ? 0.f : exp2_of(base[n][x] - to);
             m[n][x] = t;
-            base[n][x] = b - kShift;
+            base[n][x] = to;
             l[n][x] = __fmul_rn(l[n][x], fade);
             const float f = __fmul_rn(fade, fade_scale);
             if constexpr (kQuantized) {
@@ -1084,7 +1095,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     const bool none = any_seen == 0;
     float scale_l[NT][2], scale_o[NT][2], add_o[NT][2];
     const bool whole = begins && ends && !together;
-    const float unit = kQuantized ? __uint_as_float((uint32_t)exponent << 23) : 1.f;
+    const float unit = kQuantized ? __uint_as_float((uint32_t)(exponent - 10) << 23) : 1.f;  // 1 / v_unit
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -1124,11 +1135,10 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
         const int in_part = head_warp * S::kWarpHeads + h;
         if (g == 0) {
           if (!whole) {
-            part[in_part] = m[n][x] == -INFINITY && !none ? -FLT_MAX : m[n][x];
+            part[in_part] = none ? -INFINITY : m[n][x] == -INFINITY ? -FLT_MAX : base[n][x];
             part[S::kHeads + in_part] = scale_l[n][x];
           } else if (p.lse) {
-            const float from = m[n][x] == -INFINITY ? 0.f : m[n][x];
-            p.lse[row] = none ? -INFINITY : __fmaf_rn(from, kLn2, logf(__fmul_rn(scale_l[n][x], kUnshift)));
+            p.lse[row] = none ? -INFINITY : __fmaf_rn(base[n][x] + kShift, kLn2, logf(__fmul_rn(scale_l[n][x], kUnshift)));
           }
         }
         uint16_t* const out = static_cast<uint16_t*>(p.out) + row * p.dim;
@@ -1191,7 +1201,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
                        pack<BF16>(__fmul_rn(v.z, inv), __fmul_rn(v.w, inv)));
       }
       if (column == 0 && p.lse) {
-        p.lse[row] = none ? -INFINITY : __fmaf_rn(top, kLn2, logf(__fmul_rn(sum_l, kUnshift)));
+        p.lse[row] = none ? -INFINITY : __fmaf_rn(top + kShift, kLn2, logf(__fmul_rn(sum_l, kUnshift)));
       }
     };
     const bool whole = block_begins && block_ends;
@@ -1435,7 +1445,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join(const PagedAtte
         }
       }
       if (lane == 0 && p.lse) {
-        p.lse[row] = __fmaf_rn(top == -INFINITY ? 0.f : top, kLn2, logf(__fmul_rn(sum_l, kUnshift)));
+        p.lse[row] = __fmaf_rn(top == -INFINITY ? 0.f : top + Weights<S>::kShift, kLn2, logf(__fmul_rn(sum_l, Weights<S>::kUnshift)));
       }
     }
     if constexpr (TEAM > 1) {

@@ -197,3 +197,67 @@ def test_the_largest_queries_beside_quantized_rows(bits):
     weight = 2.0 ** -11 * (step * code)[at].abs()
     assert ((out[0].double() - v[at]).abs() <= 2.0 ** -8 * v[at].abs() + weight + 2.0 ** -18 * v.abs().max()).all()
     assert ((lse[0].double() - top).abs() <= 2.0 ** -18 * (q[0].double().abs() @ k.abs().T).amax(-1) * 0.125).all()
+
+
+def rows_of(cache, n, k, v):
+    """Stores n rows of single keys and values one behind another; the block table that names them."""
+    paged.rotary_append(cache, None, k, v, torch.arange(n, device=DEV))
+    assert F.status_read(0)[0]
+    return torch.arange(-(-n // cache.page_size), dtype=torch.int32, device=DEV)[None]
+
+
+@pytest.mark.parametrize("page", [16, 8])
+@pytest.mark.parametrize("rows", [1, 50, 700, 5000])
+@pytest.mark.parametrize("bits,kind", [(16, "f16"), (16, "bf16"), (8, "f16"), (4, "bf16")])
+def test_equal_scores_far_from_zero(bits, kind, rows, page):
+    """Scores of 2^20 to 2^30, all the same: the mean of the values, for every size of the scores' last place."""
+    dtype = TYPES[kind]
+    cache = paged.PagedKVCache.allocate(-(-rows // page), page, 1, 64, dtype=dtype, bit_rate=None if bits == 16 else bits, device=DEV)
+    v = (torch.rand(rows, 1, 64, device=DEV) + 1).to(dtype)
+    tables = rows_of(cache, rows, torch.full_like(v, 32.0), v)
+    stored, parts = values(cache.v.reshape(-1, cache.v.shape[-1])[:rows], bits, 64)
+    mean = stored.mean(0)
+    # Equal weights of powers of two, exact, beside 16-bit rows; beside quantized ones times the row's scale as fp16 (2^-11 of scale *
+    # (code - middle)).  Sums of rows / 16 steps and of joins, of whole codes beside quantized rows: 2^-22 each of what is summed.
+    most = stored.abs().mean(0) if parts is None else (parts[0] * 2 ** bits + parts[2].abs()).mean(0)
+    rounded = 0 if parts is None else 2.0 ** -11 * (parts[0] * parts[1].abs()).mean(0)
+    bound = 2.0 ** -8 * mean.abs() + (rows / 16 + 64) * 2.0 ** -22 * most + rounded
+    lengths = torch.tensor([rows], dtype=torch.int32, device=DEV)
+    for power in range(20, 31):
+        for sign in (1.0, -1.0):
+            q = torch.full((1, 3, 64), 32.0 * sign, device=DEV).to(dtype)
+            scale = 2.0 ** (power - 16)          # 64 columns of 2^10 each
+            out, lse = paged.paged_attention(cache, q, tables, lengths, scale=scale, return_lse=True)
+            assert ((out[0].double() - mean).abs() <= bound).all(), (power, sign)
+            want = sign * 2.0 ** power + math.log(rows)
+            assert ((lse.double() - want).abs() <= 2.0 ** -21 * abs(want)).all(), (power, sign)
+
+
+@pytest.mark.parametrize("bits,kind", [(16, "f16"), (16, "bf16"), (8, "f16"), (8, "bf16")])
+def test_scores_that_rise_by_single_steps_far_from_zero(bits, kind):
+    """A running maximum whose last places are worth 2 to 32: weights stay numbers, and the result among the values."""
+    dtype, rows = TYPES[kind], 1000
+    cache = paged.PagedKVCache.allocate(63, 16, 1, 64, dtype=dtype, bit_rate=None if bits == 16 else bits, device=DEV)
+    v = (torch.rand(rows, 1, 64, device=DEV) + 1).to(dtype)
+    k = torch.zeros_like(v)
+    tables = rows_of(cache, rows, k, v)
+    lengths = torch.tensor([rows], dtype=torch.int32, device=DEV)
+    row = torch.arange(rows, device=DEV)
+    for power in range(22, 31):
+        for step in (1, 2, 3, 4, 5, 6, 8):
+            q = torch.zeros(1, 2, 64, device=DEV)
+            if bits == 16:      # column 0: the common size; column 1: the steps
+                q[..., 0], q[..., 1] = 2.0 ** 15, 1.0
+                k[:, 0, 0], k[:, 0, 1] = 2.0 ** (power - 15), (row % 256 * 4 * step).to(dtype)
+                tables = rows_of(cache, rows, k, v)
+            else:               # codes of 0 and the row's bias
+                bias = (2.0 ** power + row % 256 * 4 * step).float()
+                flat = cache.k.permute(0, 2, 1, 3)[:, 0]          # [pages, page, row]
+                flat[..., :68] = 0
+                flat[..., 68:] = torch.nn.functional.pad(bias, (0, 8)).view(63, 16, 1).view(torch.uint8)
+                q[..., 0] = 1.0
+            out, lse = paged.paged_attention(cache, q.to(dtype), tables, lengths, scale=1.0, return_lse=True)
+            # (a value of [1, 2] stored with an error of 2^-8, two roundings of 2^-8 each)
+            assert ((out >= 1 - 3 * 2.0 ** -8) & (out <= 2 + 6 * 2.0 ** -8)).all(), (power, step)
+            top = 2.0 ** power + 255 * 4 * step
+            assert ((lse - top).abs() <= 2.0 ** -16 * top).all(), (power, step)
