@@ -72,14 +72,16 @@ constexpr int kThreads = 32 * kWarps;
 constexpr uint32_t kLateCopy = 1000000;  // nanoseconds that a copy which is late gets once more
 constexpr int kByItem = 6;  // workers to an item from which on the join goes by items
 
-// Weights are at most 2^kSlack above their reference, and as fp16 numbers 2^10 times as large as in the formula: 2^14 at most,
-// and with a scale of less than 2 below 2^15.  16-bit rows take the power of two into the reference (kShift), quantized ones
-// into their scales.
+// A weight is exp2(score - maximum so far), at most 2^kSlack.  fp16 numbers are 2^10 times that, 2^14 at most, and with a scale of
+// less than 2 below 2^15 (quantized rows: V's scales hold the power of two).  Sums over 2^31 rows of bf16's or fp32's largest values
+// are to stay numbers until they are divided by the sum of the weights: bf16 weights are 2^-36 of it, and quantized rows' sums
+// are kept times as much.
 constexpr float kSlack = 4.f;
-template <typename S>
+constexpr float kSmall = 1.f / 68719476736.f;  // 2^-36
+template <typename S, bool BF16>
 struct Weights {
-  static constexpr float kShift = S::BITS == 16 ? 10.f : 0.f;
-  static constexpr float kUnshift = S::BITS == 16 ? 1.f / 1024.f : 1.f;
+  static constexpr float kWeight = BF16 ? kSmall : 1024.f;                          // beside 16-bit rows
+  static constexpr float kResult = S::BITS == 16 ? 1.f / kWeight : 1.f / kSmall;    // of what the sums are divided by
 };
 constexpr float kFar = 1152921504606846976.f;  // 2^60
 constexpr float kLn2 = 0.6931471805599453f;
@@ -278,7 +280,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   constexpr int BITS = S::BITS, NT = S::NT, SUB = S::SUB;
   constexpr bool kQuantized = BITS != 16;
   constexpr bool kMmaBf16 = !kQuantized && BF16;
-  constexpr float kShift = Weights<S>::kShift, kUnshift = Weights<S>::kUnshift;
+  constexpr float kWeight = Weights<S, BF16>::kWeight, kResult = Weights<S, BF16>::kResult;
   constexpr float kMiddle = BITS == 8 ? 128.f : 8.f;
   constexpr float kCode = BITS == 4 ? 1.f / 1048576.f : 1.f / 16777216.f;  // what a code of 1 is to the products
   constexpr unsigned kFull = S::ROWS == 32 ? kAll : (1u << (S::ROWS & 31)) - 1;
@@ -778,8 +780,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
 
     const bool any_far = kQuantized && BF16 && __any_sync(kAll, far != 0);
     float o[NT][S::MT][4];
-    // m: what weights are relative to, base = m - kShift (m itself where m - kShift is rounded by one and more: from 2^24 on
-    // scores are that far apart); l: their sum over this lane's rows; of the rounded weights
+    // m: what weights are relative to, base = m, or 0 before the first; l: their sum over this lane's rows; of the rounded weights
     // w_sum, of the weights times the rows' biases bias_sum
     float m[NT][2], base[NT][2], l[NT][2], w_sum[NT][2], bias_sum[NT][2];
 #pragma unroll
@@ -791,7 +792,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         m[n][x] = -INFINITY;
-        base[n][x] = -kShift;
+        base[n][x] = 0.f;
         l[n][x] = w_sum[n][x] = bias_sum[n][x] = 0.f;
       }
     }
@@ -997,13 +998,9 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
             t = fmaxf(t, m[n][x]);
             const float b = t == -INFINITY ? 0.f : t;  // nothing seen yet: every weight is 0
             // (a largest score of +inf: inf - inf, so that the row becomes NaN as in the formula)
-            float to = b - kShift;
-            if (kShift != 0.f && fabsf(b - to - kShift) >= 1.f) {
-              to = b;
-            }
-            const float fade = m[n][x] == t ? 1.f : m[n][x] == -INFINITY ? 0.f : exp2_of(base[n][x] - to);
+            const float fade = m[n][x] == t ? 1.f : exp2_of(m[n][x] - b);
             m[n][x] = t;
-            base[n][x] = to;
+            base[n][x] = b;
             l[n][x] = __fmul_rn(l[n][x], fade);
             const float f = __fmul_rn(fade, fade_scale);
             if constexpr (kQuantized) {
@@ -1025,7 +1022,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float vs = kQuantized ? __fmul_rn(v_sb[s][r].x, v_unit) : 1.f;
-          const float vb = kQuantized ? __fmaf_rn(kMiddle, v_sb[s][r].x, v_sb[s][r].y) : 0.f;
+          const float vb = kQuantized ? __fmul_rn(__fmaf_rn(kMiddle, v_sb[s][r].x, v_sb[s][r].y), kSmall) : 0.f;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             float e[2];
@@ -1036,6 +1033,8 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
               if constexpr (kQuantized) {
                 bias_sum[n][x] = __fmaf_rn(e[x], vb, bias_sum[n][x]);
                 e[x] = __fmul_rn(e[x], vs);
+              } else {
+                e[x] = __fmul_rn(e[x], kWeight);
               }
             }
             const uint32_t w = pack<kMmaBf16>(e[0], e[1]);
@@ -1095,14 +1094,14 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     const bool none = any_seen == 0;
     float scale_l[NT][2], scale_o[NT][2], add_o[NT][2];
     const bool whole = begins && ends && !together;
-    const float unit = kQuantized ? __uint_as_float((uint32_t)(exponent - 10) << 23) : 1.f;  // 1 / v_unit
+    const float unit = kQuantized ? __uint_as_float((uint32_t)exponent << 23) : 1.f;  // 2^10 / v_unit
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         float sum_l = l[n][x], sum_b = 0.f;
         if constexpr (kQuantized) {
-          sum_b = __fmaf_rn(__fmul_rn(w_sum[n][x], unit), -kMiddle, bias_sum[n][x]);
+          sum_b = __fmaf_rn(__fmul_rn(__fmul_rn(w_sum[n][x], kSmall / 1024.f), unit), -kMiddle, bias_sum[n][x]);
         }
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) {
@@ -1111,7 +1110,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
             sum_b += __shfl_xor_sync(kAll, sum_b, d);
           }
         }
-        const float inv = !whole ? 1.f : none ? 0.f : __fdiv_rn(1.f, sum_l);
+        const float inv = !whole ? 1.f : none ? 0.f : __fdiv_rn(kResult, sum_l);
         scale_l[n][x] = sum_l;
         scale_o[n][x] = inv;
         add_o[n][x] = sum_b;
@@ -1135,10 +1134,10 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
         const int in_part = head_warp * S::kWarpHeads + h;
         if (g == 0) {
           if (!whole) {
-            part[in_part] = none ? -INFINITY : m[n][x] == -INFINITY ? -FLT_MAX : base[n][x];
+            part[in_part] = m[n][x] == -INFINITY && !none ? -FLT_MAX : m[n][x];
             part[S::kHeads + in_part] = scale_l[n][x];
           } else if (p.lse) {
-            p.lse[row] = none ? -INFINITY : __fmaf_rn(base[n][x] + kShift, kLn2, logf(__fmul_rn(scale_l[n][x], kUnshift)));
+            p.lse[row] = none ? -INFINITY : __fmaf_rn(base[n][x], kLn2, logf(scale_l[n][x]));
           }
         }
         uint16_t* const out = static_cast<uint16_t*>(p.out) + row * p.dim;
@@ -1147,8 +1146,8 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
         for (int t = 0; t < S::MT; ++t) {
           float a = o[n][t][x], b = o[n][t][2 + x];
           if constexpr (kQuantized) {
-            a = __fmaf_rn(__fmul_rn(a, 1.f / kCode), unit, add_o[n][x]);
-            b = __fmaf_rn(__fmul_rn(b, 1.f / kCode), unit, add_o[n][x]);
+            a = __fmaf_rn(__fmul_rn(a, kSmall / 1024.f / kCode), unit, add_o[n][x]);
+            b = __fmaf_rn(__fmul_rn(b, kSmall / 1024.f / kCode), unit, add_o[n][x]);
           }
           // 16-bit rows: columns g and g + 8 of a step of 16; quantized ones: two columns side by side
           const int column = BITS == 16 ? 16 * t + g : BITS == 8 ? 16 * t + 2 * g : 32 * (t / 2) + 4 * g + 2 * (t % 2);
@@ -1193,7 +1192,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     const float* const parts = reinterpret_cast<const float*>(smem);
     auto results_out = [&](int h, int column, float4 v, float top, float sum_l) {
       const bool none = top == -INFINITY;
-      const float inv = none ? 0.f : __fdiv_rn(1.f, sum_l);
+      const float inv = none ? 0.f : __fdiv_rn(kResult, sum_l);
       const int64_t row = ((int64_t)sm_request[0] * p.kv_heads + kv_head) * p.group + first_head + h;
       if (column < p.dim) {
         *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + (row * p.dim + column) * 2) =
@@ -1201,7 +1200,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
                        pack<BF16>(__fmul_rn(v.z, inv), __fmul_rn(v.w, inv)));
       }
       if (column == 0 && p.lse) {
-        p.lse[row] = none ? -INFINITY : __fmaf_rn(top + kShift, kLn2, logf(__fmul_rn(sum_l, kUnshift)));
+        p.lse[row] = none ? -INFINITY : __fmaf_rn(top, kLn2, logf(sum_l));
       }
     };
     const bool whole = block_begins && block_ends;
@@ -1435,7 +1434,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join(const PagedAtte
         top = all;
       }
       const int64_t row = ((int64_t)request * p.kv_heads + kv_head) * p.group + first_head + h;
-      const float inv = top == -INFINITY ? 0.f : __fdiv_rn(1.f, sum_l);  // (no row on a page of the cache: zeros)
+      const float inv = top == -INFINITY ? 0.f : __fdiv_rn(Weights<S, BF16>::kResult, sum_l);  // (no row on a page of the cache: zeros)
 #pragma unroll
       for (int j = 0; j < kCols; j += 2) {
         const int column = 32 * j + 2 * lane;
@@ -1445,7 +1444,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join(const PagedAtte
         }
       }
       if (lane == 0 && p.lse) {
-        p.lse[row] = __fmaf_rn(top == -INFINITY ? 0.f : top + Weights<S>::kShift, kLn2, logf(__fmul_rn(sum_l, Weights<S>::kUnshift)));
+        p.lse[row] = __fmaf_rn(top == -INFINITY ? 0.f : top, kLn2, logf(sum_l));
       }
     }
     if constexpr (TEAM > 1) {

@@ -261,3 +261,50 @@ def test_scores_that_rise_by_single_steps_far_from_zero(bits, kind):
             assert ((out >= 1 - 3 * 2.0 ** -8) & (out <= 2 + 6 * 2.0 ** -8)).all(), (power, step)
             top = 2.0 ** power + 255 * 4 * step
             assert ((lse - top).abs() <= 2.0 ** -16 * top).all(), (power, step)
+
+
+@pytest.mark.parametrize("page", [16, 8])
+@pytest.mark.parametrize("rows", [1, 50, 1500, 9000])
+@pytest.mark.parametrize("bits", [16, 8])
+def test_the_largest_values(bits, rows, page):
+    """Values near bf16's end: their mean is a number, though their sum is none."""
+    cache = paged.PagedKVCache.allocate(-(-rows // page), page, 1, 64, bit_rate=None if bits == 16 else bits, device=DEV)
+    lengths = torch.tensor([rows, max(1, rows // 2)], dtype=torch.int32, device=DEV)
+    q = torch.randn(2, 4, 64, device=DEV).bfloat16()
+    # the largest of all, by columns of one sign (8-bit rows: all of one sign, so that the row's range is a number), equal weights
+    v = torch.full((rows, 1, 64), torch.finfo(torch.bfloat16).max, device=DEV).bfloat16()
+    if bits == 16:
+        v[..., ::2] *= -1
+    tables = rows_of(cache, rows, torch.zeros_like(v), v).expand(2, -1).contiguous()
+    out = paged.paged_attention(cache, q, tables, lengths)
+    assert F.status_read(0)[0] and torch.equal(out, v[:1].expand(2, 4, 64))
+    # half of that, all signs, all weights
+    v = ((torch.rand(rows, 1, 64, device=DEV) - 0.5) * 2.0 ** 127).bfloat16()
+    tables = rows_of(cache, rows, torch.randn(rows, 1, 64, device=DEV).bfloat16(), v).expand(2, -1).contiguous()
+    out, lse = check_attention(cache, q, tables, lengths)
+    assert out.isfinite().all()
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_small_values(bits):
+    """Values of 1e-20 keep their bits."""
+    cache = paged.PagedKVCache.allocate(100, 16, 1, 64, bit_rate=None if bits == 16 else bits, device=DEV)
+    n = 1600
+    fill(cache)
+    scale = 2.0 ** -66
+    if bits == 16:
+        cache.v.mul_(scale)
+        big = cache.v.float() / scale
+    else:
+        at = cache.v[..., 64:]
+        at.copy_((at.contiguous().view(torch.float32) * scale).view(torch.uint8))
+    q = torch.randn(1, 4, 64, device=DEV).bfloat16()
+    tables = torch.arange(100, dtype=torch.int32, device=DEV)[None]
+    lengths = torch.tensor([n], dtype=torch.int32, device=DEV)
+    out = paged.paged_attention(cache, q, tables, lengths)
+    if bits == 16:
+        cache.v.copy_(big)
+    else:
+        at.copy_((at.contiguous().view(torch.float32) / scale).view(torch.uint8))
+    # (every step is by the same powers of two)
+    assert torch.equal(out.float() / scale, paged.paged_attention(cache, q, tables, lengths).float())
