@@ -325,7 +325,11 @@ static PyObject* rotary_append(PyObject* self, PyObject* const* args, Py_ssize_t
         return NULL;
       }
       for (Py_ssize_t i = 0; i < axes; ++i) {
-        r.section_end[i] = (int32_t)PyLong_AsLong(PyTuple_GET_ITEM(args[11], i));
+        const int64_t end = PyLong_AsLongLong(PyTuple_GET_ITEM(args[11], i));
+        if ((end == -1 && PyErr_Occurred()) || small("the sum of sections", end)) {
+          return NULL;
+        }
+        r.section_end[i] = (int32_t)end;
       }
       r.axes = (int32_t)axes;
       if (PyErr_Occurred() || look(args[8], "positions", 2, 0, &positions)) {

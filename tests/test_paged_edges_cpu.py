@@ -4,8 +4,9 @@ import re
 import subprocess
 
 import pytest
+import torch
 
-from fbgemm_b200 import _capi, build
+from fbgemm_b200 import _capi, build, paged
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -33,3 +34,16 @@ def test_copy_limit_refuses(wrong):
     lib = _capi.lib()
     assert lib.fbgemm_b200_set_copy_limit(wrong) == _capi.EINVAL and "nanoseconds" in _capi.last_error()
     assert lib.fbgemm_b200_set_copy_limit(10 ** 9) == 10 ** 9
+
+
+def append_with(sections):
+    x = torch.zeros(5, 2, 64).half()
+    cache = paged.PagedKVCache(torch.zeros(3, 4, 2, 64).half(), torch.zeros(3, 4, 2, 64).half())
+    return paged.rotary_append(cache, x, x, x, torch.zeros(5, dtype=torch.int64), torch.zeros(len(sections), 5, dtype=torch.int32),
+                               torch.zeros(9, 64), sections=sections)
+
+
+@pytest.mark.parametrize("sections", [(2 ** 32 + 32,), (16, 2 ** 32 + 16), (2 ** 31, 32), (2 ** 62, 2 ** 62), (2 ** 64, 32)])
+def test_sections_beyond_32_bits_are_refused(sections):
+    with pytest.raises((ValueError, OverflowError), match="sections|too (big|large)"):
+        append_with(sections)
