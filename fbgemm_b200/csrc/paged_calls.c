@@ -250,7 +250,7 @@ static PyObject* paged_slots(PyObject* self, PyObject* const* args, Py_ssize_t n
       block_table(args[3], lengths.size[0], &table, &row) ||
       vector(args[4], "free_pages", t_int32, "torch.int32", -1, &pages) ||
       vector(args[5], "num_free", t_int32, "torch.int32", 1, &num) || integers(args, 6, 2, size) || pointers(args, 8, 2, out) ||
-      integers(args, 10, 1, &slot) || handles(args, 11, 1, &stream) || on_device(&fresh, "new_tokens", lengths.device) ||
+      integers(args, 10, 1, &slot) || small("slot", slot) || handles(args, 11, 1, &stream) || on_device(&fresh, "new_tokens", lengths.device) ||
       on_device(&table, "block_tables", lengths.device) || on_device(&pages, "free_pages", lengths.device) ||
       on_device(&num, "num_free", lengths.device) || on_cuda(lengths.device)) {
     return NULL;
@@ -283,7 +283,7 @@ static PyObject* rotary_append(PyObject* self, PyObject* const* args, Py_ssize_t
       heads_of(args[5], "v", k.dtype, k.size[0], c->kv_heads, c->head_dim, 0, &v) ||
       heads_of(args[3], "q", k.dtype, k.size[0], -1, c->head_dim, 1, &q) ||
       vector(args[7], "slots", t_int64, "torch.int64", k.size[0], &slots) || integers(args, 10, 1, &interleaved) ||
-      integers(args, 12, 1, &slot) || handles(args, 13, 1, &stream)) {
+      integers(args, 12, 1, &slot) || small("slot", slot) || handles(args, 13, 1, &stream)) {
     return NULL;
   }
   q_out.p = NULL;
@@ -372,7 +372,7 @@ static PyObject* paged_attention(PyObject* self, PyObject* const* args, Py_ssize
       block_table(args[4], q.size[0], &table, &row) ||
       vector(args[5], "lengths", t_int32, "torch.int32", q.size[0], &lengths) || integers(args, 7, 1, &window) ||
       same_shape(args[8], "out", &q, &out) || pointers(args, 9, 2, more) || integers(args, 11, 1, &bytes) ||
-      integers(args, 12, 1, &slot) || handles(args, 13, 1, &stream) || on_device(&q, "q", device) ||
+      integers(args, 12, 1, &slot) || small("slot", slot) || handles(args, 13, 1, &stream) || on_device(&q, "q", device) ||
       on_device(&table, "block_tables", device) || on_device(&lengths, "lengths", device) || on_device(&out, "out", device) ||
       on_cuda(device)) {
     return NULL;

@@ -47,3 +47,17 @@ def append_with(sections):
 def test_sections_beyond_32_bits_are_refused(sections):
     with pytest.raises((ValueError, OverflowError), match="sections|too (big|large)"):
         append_with(sections)
+
+
+@pytest.mark.parametrize("slot", [2 ** 32, 2 ** 31, -2 ** 32, -1])
+def test_status_slots_beyond_32_bits_are_refused(slot):
+    i = dict(dtype=torch.int32)
+    x = torch.zeros(5, 2, 64).half()
+    cache = paged.PagedKVCache(torch.zeros(3, 4, 2, 64).half(), torch.zeros(3, 4, 2, 64).half())
+    with pytest.raises(ValueError, match="slot"):
+        paged.paged_slots(torch.zeros(2, **i), torch.ones(2, **i), torch.zeros(2, 3, **i), torch.zeros(8, **i), torch.ones(1, **i), 16, 4,
+                          slot=slot)
+    with pytest.raises(ValueError, match="slot"):
+        paged.rotary_append(cache, x, x, x, torch.zeros(5, dtype=torch.int64), slot=slot)
+    with pytest.raises(ValueError, match="slot"):
+        paged.paged_attention(cache, x, torch.zeros(5, 3, **i), torch.ones(5, **i), slot=slot)
