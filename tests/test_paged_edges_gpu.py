@@ -9,6 +9,7 @@ import torch
 import fbgemm_b200 as F
 from fbgemm_b200 import _capi, paged
 
+import test_paged_gpu as known
 from test_paged_gpu import DEV, TYPES, check_attention, fill, values
 
 pytestmark = pytest.mark.gpu
@@ -308,3 +309,112 @@ def test_small_values(bits):
         at.copy_((at.contiguous().view(torch.float32) / scale).view(torch.uint8))
     # (every step is by the same powers of two)
     assert torch.equal(out.float() / scale, paged.paged_attention(cache, q, tables, lengths).float())
+
+
+# ---- the form of rotary_append that many tokens take (a warp a token) --------
+
+MANY = [
+    # tokens, heads, kv_heads, dim, rot, sections, interleaved, bits, type, page, order, pitch
+    (2047, 4, 2, 64, 64, (8, 10, 14), False, 8, "bf16", 16, "heads", None),     # (the last size of the other form)
+    (2048, 7, 1, 256, 256, None, True, 16, "f16", 32, "pages last", None),
+    (2049, 4, 2, 64, 64, None, False, 16, "bf16", 16, "heads", None),
+    (2050, 10, 5, 80, 80, (10, 20, 10), True, 8, "bf16", 8, "tokens", 92),
+    (2051, 3, 1, 128, 128, (16, 24, 24), False, 8, "f16", 64, "tokens", None),
+    (2053, 6, 2, 64, 0, None, False, 4, "f16", 16, "heads", None),              # nothing is turned
+    (2055, 0, 2, 112, 112, None, False, 16, "bf16", 16, "heads", None),         # no queries
+    (3001, 1, 1, 32, 16, None, False, 4, "f16", 1, "tokens", 20),
+    (2501, 9, 3, 208, 96, (0, 40, 0, 8), True, 8, "f16", 16, "heads", 220),
+    (4097, 5, 3, 96, 48, None, True, 4, "bf16", 16, "heads", None),
+]
+
+
+@pytest.mark.parametrize("case", MANY, ids=lambda c: "-".join(str(x) for x in c))
+def test_append_of_many_tokens(oracle, case):
+    known.test_append(oracle, *case)
+
+
+def test_append_of_many_tokens_reports_what_is_outside():
+    n = 2051
+    cache = known.make_cache(140, 16, 2, 64, 8, torch.float16)
+    k = torch.randn(n, 2, 64, device=DEV).half()
+    before = cache.k.clone(), cache.v.clone()
+    table = known.angles(10, 64)
+    for token in (0, 1027, n - 1):
+        for value in (10, -1, 2 ** 31 - 1):
+            slots = torch.full((n,), -1, device=DEV)
+            slots[token] = 3
+            positions = torch.zeros(n, dtype=torch.int32, device=DEV)
+            positions[token] = value
+            q = paged.rotary_append(cache, k, k, k, slots, positions, table)
+            ok, info = F.status_read(0)
+            assert not ok and info == [_capi.STATUS_BAD_INDEX, token, 0, value]
+            assert torch.equal(q, k)                       # position 0 and the one outside: unturned
+        for value in (140 * 16, -2, 2 ** 62):
+            slots = torch.full((n,), -1, device=DEV)
+            slots[token] = value
+            paged.rotary_append(cache, k, k, k, slots, torch.zeros_like(positions), table)
+            ok, info = F.status_read(0)
+            assert not ok and info[:2] == [_capi.STATUS_BAD_PAGE, token]
+    assert torch.equal(cache.k, before[0]) and torch.equal(cache.v, before[1]) and F.status_read(0)[0]
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_append_of_many_tokens_in_place(bits):
+    n = 2051
+    made = [known.make_cache(140, 16, 2, 96, bits, torch.bfloat16) for _ in range(2)]
+    q, k, v = (torch.randn(n, heads, 96, device=DEV).bfloat16() for heads in (5, 2, 2))
+    slots = torch.randperm(140 * 16, device=DEV)[:n]
+    positions = torch.randint(0, 300, (n,), device=DEV, dtype=torch.int32)
+    want = paged.rotary_append(made[0], q, k, v, slots, positions, known.angles(300, 96))
+    assert paged.rotary_append(made[1], q, k, v, slots, positions, known.angles(300, 96), q_out=q) is q
+    assert torch.equal(q, want) and torch.equal(made[0].k.view(torch.uint8), made[1].k.view(torch.uint8))
+    assert torch.equal(made[0].v.view(torch.uint8), made[1].v.view(torch.uint8)) and F.status_read(0)[0]
+
+
+# ---- every row once ----------------------------------------------------------
+
+COUNTS = [
+    # lengths, heads, kv_heads, dim, bits, page, window
+    ([300_001, 5, 250_000, 0, 40_000], 8, 8, 64, 16, 16, 0),        # workers of either size
+    ([300_001, 5, 250_000, 0, 40_000], 8, 8, 64, 8, 64, 0),
+    ([300_001, 5, 250_000, 0, 40_000], 8, 8, 64, 4, 8, 0),
+    ([200_003, 90_000, 70], 34, 2, 128, 16, 32, 0),                 # two warps to a worker
+    ([100_001, 150_000], 20, 1, 256, 8, 32, 0),                     # and units of 16 rows
+    ([131_072], 32, 8, 128, 16, 16, 0),
+    ([260_000, 260_000], 8, 8, 64, 16, 64, 131_071),
+    ([4000] * 3, 8, 8, 128, 16, 16, 0),                             # clusters
+    ([100, 3000, 0, 777] * 40, 16, 4, 128, 4, 32, 0),               # items shared by neighbours
+]
+
+
+@pytest.mark.parametrize("lengths,heads,kv,dim,bits,page,window", COUNTS)
+def test_every_row_enters_once(lengths, heads, kv, dim, bits, page, window):
+    """Keys of 0: all weights are 1, and the sum of them is the number of rows.  Values are one of 64 columns' unit, by parts of the
+    request: a unit of 16 rows that is lost, or another's twice, is seen at any length."""
+    cache = paged.PagedKVCache.allocate(128, page, kv, dim, dtype=torch.float16, bit_rate=None if bits == 16 else bits, device=DEV)
+    one = 1.0 if bits == 16 else (2 ** bits - 1) / 2 ** bits         # scales of powers of two: no weight is rounded
+    v = torch.zeros(128 * page, kv, dim, device=DEV).half()
+    column = torch.arange(128, device=DEV).repeat_interleave(page) % 64
+    v[torch.arange(128 * page, device=DEV), :, column] = one
+    paged.rotary_append(cache, None, torch.zeros_like(v), v, torch.arange(128 * page, device=DEV))
+    width = -(-max(lengths) // page)
+    tables = torch.full((len(lengths), width), -1, dtype=torch.int32)
+    want = torch.zeros(len(lengths), 64, dtype=torch.float64)
+    rows = torch.tensor([min(n, window) if window else n for n in lengths])
+    for b, n in enumerate(lengths):
+        pages = -(-n // page)
+        part = torch.arange(pages) * 64 // max(pages, 1)
+        tables[b, :pages] = (part + 64 * torch.randint(0, 2, (pages,))).int()
+        t = torch.arange(n - int(rows[b]), n)
+        want[b] = torch.bincount(part[t // page], minlength=64).double()
+    q = torch.randn(len(lengths), heads, dim, device=DEV).half()
+    out, lse = paged.paged_attention(cache, q, tables.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), window=window,
+                                     return_lse=True)
+    assert F.status_read(0)[0]
+    some = rows > 0
+    # whole numbers below 2^24 are exact sums; a logarithm of up to 16 and its sum with 0 are rounded by 2^-21 each
+    assert ((lse.double().cpu()[some] - rows[some].double().log()[:, None]).abs() <= 2.0 ** -20).all()
+    got, want = out.double().cpu()[some], want[some] / rows[some, None] * one
+    # one rounding to fp16, and sums (of centred codes: of all rows) within 2^-20 of the whole
+    assert ((got[..., :64] - want[:, None]).abs() <= 2.0 ** -11 * want[:, None] + 2.0 ** -20).all()
+    assert (got[..., 64:].abs() <= 2.0 ** -20).all() and (out.cpu()[~some] == 0).all()
