@@ -16,6 +16,14 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (sm_100a)")
 
 
+@pytest.fixture(autouse=True)
+def seeded():
+    """What a test draws from torch's own generator is the same in every run."""
+    torch = sys.modules.get("torch")
+    if torch is not None:
+        torch.manual_seed(1234)
+
+
 @pytest.fixture(scope="session")
 def oracle():
     from oracle.checker import Oracle

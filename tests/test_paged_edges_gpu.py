@@ -15,11 +15,6 @@ from test_paged_gpu import DEV, TYPES, check_attention, fill, values
 pytestmark = pytest.mark.gpu
 
 
-@pytest.fixture(autouse=True)
-def seeded():
-    torch.manual_seed(1234)
-
-
 # ---- what is read ------------------------------------------------------------
 
 @pytest.mark.parametrize("dim,bits,pitch", [(64, 8, 80), (48, 8, 64), (128, 4, 80), (32, 4, 32), (96, 16, 208), (112, 8, 124), (160, 4, 88)])
