@@ -402,7 +402,8 @@ int fbgemm_b200_paged_attention(
   const PagedAttentionShape shape = shape_of(*cache, q_heads, dtype);
   DeviceGuard guard(ctx->device);
   const PagedAttentionPlan plan = plan_paged_attention(shape, sm_count());
-  if ((int64_t)batch * cache->kv_heads * plan.head_tiles > 0x7fffffffLL) {
+  const int64_t items = (int64_t)batch * cache->kv_heads * plan.head_tiles;
+  if (items > 0x7fffffffLL) {
     return refuse("paged_attention: 2^31 heads of all requests or more");
   }
   const int64_t most = (int64_t)width * cache->page_size;
@@ -445,9 +446,7 @@ int fbgemm_b200_paged_attention(
   p.aligned = rows_aligned(*cache);
   p.tall = cache->page_size >= 32;
   p.cluster = cluster;
-  // (no more units than that: the second workers' blocks would only come and go)
-  const int64_t span = span_most(*cache, width, window);
-  p.two = split && (int64_t)batch * cache->kv_heads * plan.head_tiles * (span / plan.unit + 1) >= kUnitsForTwo * plan.workers;
+  p.two = split && two_sizes(shape.bits, plan.tile_heads, items, items * (span_most(*cache, width, window) / plan.unit + 1), plan.workers);
   const cudaError_t e = launch_paged_attention(shape, plan, p, split, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? 0 : fail_cuda(e, "paged_attention launch");
 } catch (...) {

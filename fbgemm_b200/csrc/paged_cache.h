@@ -44,12 +44,9 @@ FBGEMM_B200_HD int32_t units_of(RowSpan s, int32_t unit) {
   return n > 0 ? n : 1;
 }
 
-// Who takes which units.  The first `workers` take `big` units each.  SMs are not equally fast (three quarters to one and
-// an eighth of the mean rate, by where they lie), so with enough to do the last quarter of the line is left to as many
-// workers again, `small` units each, whose blocks start where others have ended: over 32 requests of 16384 rows 320 us
-// instead of 332 (16-bit rows), 206 instead of 218 (8-bit).  Fewer units than kUnitsForTwo lose more by more parts and a second
-// start than they gain: at 35 a worker (64 requests of up to 8192 rows) nothing, at 37 (one of 131072) 107 us instead of 98, at
-// 17 (48 requests of one head of 256 columns) 52 instead of 41; the two above have 148.
+// Who takes which units.  The first `workers` take `big` units each.  SMs are not equally fast at bringing rows (three quarters to
+// one and an eighth of the mean rate, by where they lie), so where memory is what warps wait for (two_sizes) the last quarter of
+// the line is left to as many workers again, `small` units each, whose blocks start where others have ended.
 struct UnitSplit {
   int64_t big, small, workers;
   FBGEMM_B200_HD int64_t first(int64_t worker) const {
@@ -61,6 +58,16 @@ struct UnitSplit {
   FBGEMM_B200_HD int64_t units_of(int64_t worker) const { return worker < workers ? big : small; }
 };
 constexpr int64_t kUnitsForTwo = 40;  // units per worker from which on there are workers of either size
+// Whether a call may have workers of either size.  With them over without, 30, 42, 60 and 100 units a worker: 128 columns, 4 heads to a
+// cached one, 128 items 1.01 0.98 0.97 0.96 (16-bit rows), 0.99 0.96 0.96 0.98 (8-bit); 256 items of 64 or 96 columns 1.01 to 1.05,
+// 1.00 to 1.02, 0.97 to 0.99, 0.98 to 1.01; of 256 columns 1.03 to 1.08, 0.99 to 1.06, 0.99 to 1.02, 0.97 to 0.99; 32 requests of
+// 16384 8-bit rows (74 units) 0.98.  Few items are joined by parts: 64 items 1.03 1.00 0.98 0.96 and 1.00 0.98 0.98 0.98, 32 items
+// 1.07 1.02 1.00 1.00, 8 items 1.17 1.12 1.10 1.01.  Where instructions are what warps wait for, all SMs are as fast, and the second start
+// costs 10 to 20 us: 4-bit rows 1.13 to 1.30, 1.12 to 1.23, 1.10 to 1.17, 1.05 to 1.10 (1.03 still at 148 units), 16 heads of a warp and
+// 32 of two 1.09 to 1.25, 1.07 to 1.21, 1.03 to 1.16, 1.00 to 1.11.
+FBGEMM_B200_HD bool two_sizes(int32_t bits, int32_t tile_heads, int64_t items, int64_t most_units, int64_t workers) {
+  return bits != 4 && tile_heads <= 8 && items >= 64 && most_units >= kUnitsForTwo * workers;
+}
 FBGEMM_B200_HD UnitSplit split_units(int64_t total, int64_t workers, bool two) {
   UnitSplit s;
   s.workers = workers;

@@ -56,8 +56,19 @@ static void blocks() {
   }
 }
 
+// Workers of either size: where rows are waited for, with many items and long lines of units.
+static void sizes() {
+  for (int bits : {16, 8}) {
+    CHECK(two_sizes(bits, 8, 64, 40 * 1776, 1776) && two_sizes(bits, 8, 4096, 1000 * 1776, 1776));
+    CHECK(!two_sizes(bits, 8, 63, 1000 * 1776, 1776) && !two_sizes(bits, 8, 64, 40 * 1776 - 1, 1776));
+    CHECK(!two_sizes(bits, 16, 4096, 1000 * 1776, 1776) && !two_sizes(bits, 32, 4096, 1000 * 1776, 1776));
+  }
+  CHECK(!two_sizes(4, 8, 4096, 1000 * 1776, 1776));
+}
+
 int main() {
   pieces();
+  sizes();
   blocks();
   std::printf(failures ? "%d failures\n" : "ok\n", failures);
   return failures != 0;

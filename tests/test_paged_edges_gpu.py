@@ -3,6 +3,7 @@ last row, tables without a good page, numbers at the ends of their ranges, the
 forms that only large calls take."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -370,8 +371,13 @@ def test_append_of_many_tokens_in_place(bits):
 
 COUNTS = [
     # lengths, heads, kv_heads, dim, bits, page, window
-    ([300_001, 5, 250_000, 0, 40_000], 8, 8, 64, 16, 16, 0),        # workers of either size
+    ([300_001, 5, 250_000, 0, 40_000], 8, 8, 64, 16, 16, 0),
     ([300_001, 5, 250_000, 0, 40_000], 8, 8, 64, 8, 64, 0),
+    ([300_001, 5, 250_000, 0, 40_000], 32, 16, 64, 16, 16, 0),      # workers of either size
+    ([300_001, 5, 250_000, 0, 40_000], 16, 16, 64, 8, 64, 0),
+    ([9000, 30_011] * 20, 8, 4, 128, 8, 8, 0),
+    ([20_001, 9000] * 40, 8, 1, 256, 16, 32, 0),
+    ([300, 77] * 100, 4, 4, 64, 16, 16, 0),                         # (few units, although the table has room for more)
     ([300_001, 5, 250_000, 0, 40_000], 8, 8, 64, 4, 8, 0),
     ([200_003, 90_000, 70], 34, 2, 128, 16, 32, 0),                 # two warps to a worker
     ([100_001, 150_000], 20, 1, 256, 8, 32, 0),                     # and units of 16 rows
@@ -392,7 +398,7 @@ def test_every_row_enters_once(lengths, heads, kv, dim, bits, page, window):
     column = torch.arange(128, device=DEV).repeat_interleave(page) % 64
     v[torch.arange(128 * page, device=DEV), :, column] = one
     paged.rotary_append(cache, None, torch.zeros_like(v), v, torch.arange(128 * page, device=DEV))
-    width = -(-max(lengths) // page)
+    width = -(-max(max(lengths), 20_000) // page)
     tables = torch.full((len(lengths), width), -1, dtype=torch.int32)
     want = torch.zeros(len(lengths), 64, dtype=torch.float64)
     rows = torch.tensor([min(n, window) if window else n for n in lengths])
@@ -413,3 +419,16 @@ def test_every_row_enters_once(lengths, heads, kv, dim, bits, page, window):
     # one rounding to fp16, and sums (of centred codes: of all rows) within 2^-20 of the whole
     assert ((got[..., :64] - want[:, None]).abs() <= 2.0 ** -11 * want[:, None] + 2.0 ** -20).all()
     assert (got[..., 64:].abs() <= 2.0 ** -20).all() and (out.cpu()[~some] == 0).all()
+
+
+@pytest.mark.parametrize("bits,kind,page", [(16, "bf16", 16), (8, "f16", 64), (8, "bf16", 8)])
+def test_attention_of_many_long_items(bits, kind, page):
+    """Long lines of many items: a second set of workers takes the last quarter, and ends items that the first began."""
+    rng = np.random.default_rng(bits)
+    pages = 3000 // page
+    cache = known.make_cache(pages, page, 16, 64, bits, TYPES[kind])
+    fill(cache)
+    lengths = [200_001, 5, 150_000, 0, 40_000]
+    tables = torch.from_numpy(rng.integers(0, pages, (5, 200_001 // page + 1)).astype(np.int32)).to(DEV)
+    q = torch.randn(5, 32, 64, device=DEV).to(TYPES[kind])
+    check_attention(cache, q, tables, torch.tensor(lengths, dtype=torch.int32, device=DEV))
