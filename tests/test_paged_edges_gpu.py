@@ -432,3 +432,64 @@ def test_attention_of_many_long_items(bits, kind, page):
     tables = torch.from_numpy(rng.integers(0, pages, (5, 200_001 // page + 1)).astype(np.int32)).to(DEV)
     q = torch.randn(5, 32, 64, device=DEV).to(TYPES[kind])
     check_attention(cache, q, tables, torch.tensor(lengths, dtype=torch.int32, device=DEV))
+
+
+# ---- what may stand before a call in a graph ---------------------------------
+
+def test_captured_behind_copies_and_other_streams():
+    """In a graph behind a copy, a fill, a kernel of another stream and another call: the call waits for all of them."""
+    cache = paged.PagedKVCache.allocate(400, 16, 2, 64, device=DEV)
+    fill(cache)
+    tables = torch.randint(0, 400, (3, 200), device=DEV, dtype=torch.int32)
+    n = torch.tensor([3100, 40, 900], dtype=torch.int32, device=DEV)
+    source = torch.zeros(3, 4, 64, device=DEV).bfloat16()
+    q, lengths, other = torch.zeros_like(source), torch.zeros_like(n), torch.cuda.Stream()
+    big = torch.zeros(64 << 20, device=DEV)
+    width = [tables, tables[:, :64].contiguous()]      # shared by the chip; by clusters
+    outs = []
+
+    def step():
+        for t in width:
+            lengths.copy_(n)                              # a copy before it
+            q.copy_(source)
+            first = paged.paged_attention(cache, q, t, lengths.clamp(max=t.shape[1] * 16), return_lse=True)
+            lengths.zero_()                               # a fill before it
+            empty = paged.paged_attention(cache, q, t, lengths, return_lse=True)
+            other.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(other):
+                big.add_(1)                               # some 80 us, then what is read
+                lengths.copy_(n)
+                lengths.clamp_(max=t.shape[1] * 16)
+            torch.cuda.current_stream().wait_stream(other)
+            again = paged.paged_attention(cache, q, t, lengths, return_lse=True)
+            q.neg_()
+            third = paged.paged_attention(cache, q, t, lengths, return_lse=True)
+            fourth = paged.paged_attention(cache, third[0], t, lengths, return_lse=True)   # a call that reads a call's result
+            outs.append((first, empty, again, third, fourth))
+
+    source.normal_()
+    step()
+    torch.cuda.synchronize()
+    outs.clear()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    captured = list(outs)
+    for _ in range(3):
+        source.normal_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        got = [[(o.clone(), z.clone()) for o, z in x] for x in captured]
+        outs.clear()
+        for t in width:                                   # one call at a time
+            m = n.clamp(max=t.shape[1] * 16)
+            want = []
+            for x, lens in ((source, m), (source, torch.zeros_like(n)), (source, m), (-source, m)):
+                want.append(paged.paged_attention(cache, x.clone(), t, lens, return_lse=True))
+                torch.cuda.synchronize()
+            want.append(paged.paged_attention(cache, want[-1][0], t, m, return_lse=True))
+            torch.cuda.synchronize()
+            for (o, z), (o2, z2) in zip(got.pop(0), want):
+                assert torch.equal(o, o2) and torch.equal(z, z2)
+    assert F.status_read(0)[0]
