@@ -17,9 +17,11 @@ fbgemm_gpu/experimental/gen_ai/src/kv_cache; layouts and arithmetic are this
 library's own.
 
 All calls are asynchronous on torch's current stream of the tensors' device,
-allocate through torch only, and may be captured into a CUDA graph.  They are
-for serving: no result carries a gradient.  What they find wrong in the
-tensors' contents shows in status slot ``slot`` (``fbgemm_b200.status_read``).
+allocate through torch only, and may be captured into a CUDA graph (the first
+calls of a process too, once a ``PagedKVCache`` on the device has been made).
+They are for serving: no result carries a gradient.  What they find wrong in
+the tensors' contents shows in status slot ``slot``
+(``fbgemm_b200.status_read``).
 """
 from __future__ import annotations
 
@@ -85,6 +87,7 @@ class PagedKVCache:
         self._address = C.addressof(self._struct)
         self._workspace = {}   # (batch, query heads, type, width, window) -> bytes
         E._capi.check(E._capi.lib().fbgemm_b200_paged_cache_check(C.byref(self._struct)), "PagedKVCache")
+        _context(self._index)  # made here if this is the device's first: a capture does not let it allocate
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=torch.bfloat16,

@@ -2,6 +2,9 @@
 last row, tables without a good page, numbers at the ends of their ranges, the
 forms that only large calls take."""
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -14,6 +17,7 @@ import test_paged_gpu as known
 from test_paged_gpu import DEV, TYPES, check_attention, fill, values
 
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 # ---- what is read ------------------------------------------------------------
@@ -493,3 +497,29 @@ def test_captured_behind_copies_and_other_streams():
             for (o, z), (o2, z2) in zip(got.pop(0), want):
                 assert torch.equal(o, o2) and torch.equal(z, z2)
     assert F.status_read(0)[0]
+
+
+FIRST_CALLS = """
+import torch
+from fbgemm_b200 import paged
+cache = paged.PagedKVCache.allocate(40, 16, 2, 64, device="cuda:0")
+i = dict(dtype=torch.int32, device="cuda:0")
+q = torch.randn(2, 4, 64, device="cuda:0").bfloat16()
+tables, lengths, free, num_free = torch.arange(8, **i).view(2, 4), torch.tensor([60, 3], **i), torch.arange(8, 40, **i), torch.tensor([32], **i)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    s = paged.paged_slots(lengths, torch.ones_like(lengths), tables, free, num_free, 16, 4)
+    turned = paged.rotary_append(cache, q, q[:, :2], q[:, :2], s.slots[:2])
+    out = paged.paged_attention(cache, turned, tables, s.lengths)
+g.replay()
+torch.cuda.synchronize()
+want = paged.paged_attention(cache, turned, tables, s.lengths)
+assert s.slots.tolist() == [3 * 16 + 12, 4 * 16 + 3, -1, -1] and torch.equal(out, want) and want.abs().max() > 0
+print("captured")
+"""
+
+
+def test_the_first_calls_of_a_process_are_captured():
+    res = subprocess.run([sys.executable, "-c", FIRST_CALLS], capture_output=True, text=True, timeout=100, cwd=ROOT)
+    assert res.returncode == 0 and res.stdout == "captured\n", res.stderr
