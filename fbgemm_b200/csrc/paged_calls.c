@@ -58,8 +58,7 @@ static int arity(Py_ssize_t got, Py_ssize_t want) {
   return 0;
 }
 
-/* Runs CALL, which gives an int, without the interpreter's lock: a launch waits when the stream's queue is full, and lengths
- * mode takes the context's lock and may allocate. */
+/* Runs CALL, which gives an int, without the interpreter's lock: a launch waits when the stream's queue is full. */
 #define WITHOUT_LOCK(CALL)    \
   int rc;                     \
   Py_BEGIN_ALLOW_THREADS      \

@@ -159,7 +159,7 @@ def paged_slots(lengths: torch.Tensor, new_tokens: torch.Tensor, block_tables: t
     ``block_tables`` (int32 [batch, pages], in place; no other entry changes).
     The maps have ``capacity`` rows: the new rows, request after request, and
     padding behind them.  A last page that is not full is continued, so it must
-    not be shared with another request.
+    not be shared with another request.  1 to 16384 requests.
 
     All or nothing: if pages, table columns or capacity run out, no page and no
     slot is given out (``slots`` all -1, lengths and num_free as they were) and
@@ -238,7 +238,9 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, block_tables: torch.Te
     result; it does not overlap ``q``.
 
     Scores, sums and the output are fp32 until the output's one rounding; the
-    weights enter the sum over rows as 16-bit numbers.  A page outside the cache
+    weights enter the sum over rows as 16-bit numbers (bfloat16 beside a bfloat16
+    cache, float16 beside others; beside quantized rows times the row's scale,
+    each row off by up to 2**-36 of the widest row's range).  A page outside the cache
     is left out (status {7, request, row, page}; all of a request's pages: a
     request without rows); a length that is negative or
     beyond the table is brought within it (status {3, request, 0, length})."""

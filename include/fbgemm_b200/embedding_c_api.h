@@ -905,7 +905,7 @@ FBGEMM_B200_API int fbgemm_b200_paged_cache_check(const fbgemm_b200_paged_cache*
  * out: slots and requests are all -1, positions and offsets 0, lengths_out =
  * lengths, num_free_out = num_free, block_tables unchanged, and the record
  * {NO_PAGES, first request that does not fit, its new length, num_free} is in
- * status slot `slot`.  batch <= FBGEMM_B200_PAGED_MAX_BATCH, width * page_size
+ * status slot `slot`.  1 <= batch <= FBGEMM_B200_PAGED_MAX_BATCH, width * page_size
  * <= 2^31 - 256.  Inputs and outputs do not overlap.  One launch, nothing allocated.
  */
 #define FBGEMM_B200_PAGED_MAX_BATCH 16384
