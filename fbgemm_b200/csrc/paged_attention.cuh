@@ -27,11 +27,13 @@
 // set: 4-bit codes in the lowest 4 bits cost 6 bits of the sums, and results that were off by 1e-3.)
 //
 // One pass with a running maximum and sum per head in fp32 (in registers, per warp).  A tile's largest score is looked
-// for across lanes only if one exceeds the running maximum by more than 2^kSlack.  Weights are rounded to 16 bits for
-// the second product: bf16 beside bf16 rows; fp16 (2^10 times as large, so that weights down to 2^-24 of the largest
-// keep all 11 bits) otherwise, with the quantized rows' scales taken relative to the largest power of two seen so far.
-// A weight's rounding is at most half a step of the output's own type, and averages out over the rows; codes are weighed
-// about the middle of their range (sum w (c - 128) = sum w c - 128 sum w, with the rounded w), which keeps it there.
+// for across lanes only if one exceeds the running maximum by more than 2^kSlack.  A weight enters the second product as two
+// 16-bit numbers, itself rounded and what that leaves: bf16 beside bf16 rows, 16 bits together; fp16 otherwise (2^10 times as large, so
+// that weights down to 2^-13 of the largest keep 22 bits, down to 2^-24 eleven, down to 2^-34 some), with the quantized rows' scales taken
+// relative to the largest power of two seen so far.  (One number alone: errors against 64 bits of up to 1.55 times those of the output's own
+// rounding, 2.1e-3 for 1.7e-3 over 64 requests of up to 8192 bf16 rows.  The second one's products take 1 to 3 % of the time, 9 % over
+// 128 requests of 1000 4-bit rows.)  Beside 16-bit rows the first is rounded towards zero and the second is not 0 unless the weight is: so an
+// infinite value stays one (no inf - inf, no 0 inf).
 //
 // Work is split over the chip by paged_cache.h's rule: a worker is a warp (or the HW warps that share rows), and nothing
 // makes warps wait for one another, so that what a warp does between two items (its results out, the next queries in) is
@@ -41,9 +43,9 @@
 // all work on one item joins theirs first.  Short items are left to a block each, or to a cluster of two, four or eight that
 // joins its results through distributed shared memory: one launch.
 //
-// Measured over 32 requests of 16384 rows of 8 heads of 128 columns: 16-bit rows 318 to 323 us, 6.7 TB/s, what a plain copy
-// reaches.  8-bit rows 204 us, 0.85 of that rate, and 4-bit ones 141, 0.62: a tile is half or a quarter of the bytes and
-// no fewer instructions (about 700 of a warp for 32 4-bit rows, three warps a scheduler, one instruction in two cycles),
+// Measured over 32 requests of 16384 rows of 8 heads of 128 columns: 16-bit rows 320 to 325 us, 6.7 TB/s, what a plain copy
+// reaches.  8-bit rows 207 us, 0.84 of that rate, and 4-bit ones 153, 0.57: a tile is half or a quarter of the bytes and
+// no fewer instructions (about 750 of a warp for 32 4-bit rows, three warps a scheduler, one instruction in two cycles),
 // whose chain from the scores through the weights to the sums is what a tile takes.  Below some 100 us a fixed 15 us shows:
 // 4 until the first rows are there, the slowest SM's 10 behind the mean one, and the join.
 #pragma once
@@ -116,12 +118,16 @@ __device__ __forceinline__ float exp2_of(float x) {
   return r;
 }
 
-// a in the low half.
-template <bool BF16>
+// a in the low half; towards zero if DOWN.
+template <bool BF16, bool DOWN = false>
 __device__ __forceinline__ uint32_t pack(float a, float b) {
   uint32_t r;
-  if constexpr (BF16) {
+  if constexpr (BF16 && DOWN) {
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  } else if constexpr (BF16) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  } else if constexpr (DOWN) {
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
   } else {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
   }
@@ -281,7 +287,6 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   constexpr bool kQuantized = BITS != 16;
   constexpr bool kMmaBf16 = !kQuantized && BF16;
   constexpr float kWeight = Weights<S, BF16>::kWeight, kResult = Weights<S, BF16>::kResult;
-  constexpr float kMiddle = BITS == 8 ? 128.f : 8.f;
   constexpr float kCode = BITS == 4 ? 1.f / 1048576.f : 1.f / 16777216.f;  // what a code of 1 is to the products
   constexpr unsigned kFull = S::ROWS == 32 ? kAll : (1u << (S::ROWS & 31)) - 1;
   constexpr int kSlot = FAST ? S::SLOT_FAST : S::SLOT;
@@ -780,9 +785,9 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
 
     const bool any_far = kQuantized && BF16 && __any_sync(kAll, far != 0);
     float o[NT][S::MT][4];
-    // m: what weights are relative to, base = m, or 0 before the first; l: their sum over this lane's rows; of the rounded weights
-    // w_sum, of the weights times the rows' biases bias_sum
-    float m[NT][2], base[NT][2], l[NT][2], w_sum[NT][2], bias_sum[NT][2];
+    // m: what weights are relative to, base = m, or 0 before the first; l: their sum over this lane's rows, bias_sum: that of the
+    // weights times the rows' biases
+    float m[NT][2], base[NT][2], l[NT][2], bias_sum[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -793,7 +798,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
       for (int x = 0; x < 2; ++x) {
         m[n][x] = -INFINITY;
         base[n][x] = 0.f;
-        l[n][x] = w_sum[n][x] = bias_sum[n][x] = 0.f;
+        l[n][x] = bias_sum[n][x] = 0.f;
       }
     }
     // V's scales are taken relative to 2^(exponent - 127) = 2^10 / v_unit, and are below scale_limit, twice that.
@@ -1005,7 +1010,6 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
             const float f = __fmul_rn(fade, fade_scale);
             if constexpr (kQuantized) {
               bias_sum[n][x] = __fmul_rn(bias_sum[n][x], fade);
-              w_sum[n][x] = __fmul_rn(w_sum[n][x], f);
             }
 #pragma unroll
             for (int k = 0; k < S::MT; ++k) {
@@ -1016,13 +1020,13 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
         }
       }
       fill(S::SLOTS % 2 != 0);  // (into K's half, which has come, as that question has shown)
-      uint32_t wt[NT][SUB][2];
+      uint32_t wt[NT][SUB][2], rest[NT][SUB][2];
 #pragma unroll
       for (int s = 0; s < SUB; ++s) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float vs = kQuantized ? __fmul_rn(v_sb[s][r].x, v_unit) : 1.f;
-          const float vb = kQuantized ? __fmul_rn(__fmaf_rn(kMiddle, v_sb[s][r].x, v_sb[s][r].y), kSmall) : 0.f;
+          const float vb = kQuantized ? __fmul_rn(v_sb[s][r].y, kSmall) : 0.f;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             float e[2];
@@ -1037,13 +1041,14 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
                 e[x] = __fmul_rn(e[x], kWeight);
               }
             }
-            const uint32_t w = pack<kMmaBf16>(e[0], e[1]);
-            if constexpr (kQuantized) {
-              const float2 rounded = halves(w);
-              w_sum[n][0] += rounded.x;
-              w_sum[n][1] += rounded.y;
+            const uint32_t w = pack<kMmaBf16, !kQuantized>(e[0], e[1]);
+            const float2 held = kMmaBf16 ? make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)) : halves(w);
+            uint32_t left_out = pack<kMmaBf16>(e[0] - held.x, e[1] - held.y);
+            if constexpr (!kQuantized) {
+              left_out |= __vminu2(w, 0x00010001u);  // (the last bit, where the weight is not 0)
             }
             wt[n][s][r] = transposed(w);
+            rest[n][s][r] = transposed(left_out);
           }
         }
       }
@@ -1059,6 +1064,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               mma<kMmaBf16>(o[n][b / 2], r[0], r[1], r[2], r[3], wt[n][s][0], wt[n][s][1]);
+              mma<kMmaBf16>(o[n][b / 2], r[0], r[1], r[2], r[3], rest[n][s][0], rest[n][s][1]);
             }
           } else {
 #pragma unroll
@@ -1069,6 +1075,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                   mma<false>(o[n][b + h], a0, a1, a2, a3, wt[n][s][0], wt[n][s][1]);
+                  mma<false>(o[n][b + h], a0, a1, a2, a3, rest[n][s][0], rest[n][s][1]);
                 }
               } else {
 #pragma unroll
@@ -1078,6 +1085,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
 #pragma unroll
                   for (int n = 0; n < NT; ++n) {
                     mma<false>(o[n][2 * (b + h) + j], a0, a1, a2, a3, wt[n][s][0], wt[n][s][1]);
+                    mma<false>(o[n][2 * (b + h) + j], a0, a1, a2, a3, rest[n][s][0], rest[n][s][1]);
                   }
                 }
               }
@@ -1099,10 +1107,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        float sum_l = l[n][x], sum_b = 0.f;
-        if constexpr (kQuantized) {
-          sum_b = __fmaf_rn(__fmul_rn(__fmul_rn(w_sum[n][x], kSmall / 1024.f), unit), -kMiddle, bias_sum[n][x]);
-        }
+        float sum_l = l[n][x], sum_b = bias_sum[n][x];
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) {
           sum_l += __shfl_xor_sync(kAll, sum_l, d);

@@ -238,9 +238,10 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, block_tables: torch.Te
     result; it does not overlap ``q``.
 
     Scores, sums and the output are fp32 until the output's one rounding; the
-    weights enter the sum over rows as 16-bit numbers (bfloat16 beside a bfloat16
-    cache, float16 beside others; beside quantized rows times the row's scale,
-    each row off by up to 2**-36 of the widest row's range).  A page outside the cache
+    weights enter the sum over rows as two 16-bit numbers each (bfloat16 beside a
+    bfloat16 cache: 16 bits; float16 beside others: 22 bits; beside quantized rows
+    times the row's scale, each row off by up to 2**-35 of the widest row's
+    range).  A page outside the cache
     is left out (status {7, request, row, page}; all of a request's pages: a
     request without rows); a length that is negative or
     beyond the table is brought within it (status {3, request, 0, length})."""

@@ -523,3 +523,68 @@ print("captured")
 def test_the_first_calls_of_a_process_are_captured():
     res = subprocess.run([sys.executable, "-c", FIRST_CALLS], capture_output=True, text=True, timeout=100, cwd=ROOT)
     assert res.returncode == 0 and res.stdout == "captured\n", res.stderr
+
+
+# ---- one rounding ------------------------------------------------------------
+
+ROUNDED = [
+    # lengths, heads, kv_heads, dim, bits, type, page, window
+    ([1, 2, 5, 40], 8, 2, 64, 16, "bf16", 16, 0), ([1, 2, 5, 40], 8, 2, 64, 16, "f16", 16, 0),
+    ([1, 2, 5, 40], 8, 2, 64, 8, "f16", 8, 0), ([1, 2, 5, 40], 8, 2, 64, 4, "f16", 16, 0),
+    ([3000, 77, 900], 8, 2, 128, 16, "bf16", 16, 0), ([3000, 77, 900], 32, 2, 128, 16, "f16", 32, 500),
+    ([3000, 77, 900], 12, 1, 256, 16, "bf16", 32, 0), ([3000, 77, 900], 20, 1, 128, 16, "bf16", 4, 0),
+    ([3000, 77, 900], 8, 2, 128, 8, "f16", 32, 0), ([3000, 77, 900], 32, 2, 128, 8, "bf16", 16, 0),
+    ([3000, 77, 900], 12, 1, 256, 8, "f16", 64, 0), ([3000, 77, 900], 4, 1, 48, 8, "f16", 2, 0),
+    ([3000, 77, 900], 8, 2, 128, 4, "f16", 32, 0), ([3000, 77, 900], 32, 2, 128, 4, "bf16", 16, 0),
+    ([3000, 77, 900], 12, 1, 256, 4, "f16", 64, 300), ([3000, 77, 900], 4, 1, 96, 4, "f16", 8, 0),
+    ([100, 20, 300] * 60, 8, 4, 64, 8, "f16", 16, 0), ([100, 20, 300] * 60, 8, 4, 64, 16, "bf16", 16, 0),
+]
+
+
+@pytest.mark.parametrize("lengths,heads,kv,dim,bits,kind,page,window", ROUNDED)
+@pytest.mark.parametrize("sharp", [0.5, 4.0])
+def test_weights_are_as_good_as_their_sum(lengths, heads, kv, dim, bits, kind, page, window, sharp):
+    """The result is the formula's, rounded once to its type: what 16-bit weights would add on top is not there."""
+    dtype = TYPES[kind]
+    tables, pages = known.place(lengths, page, np.random.default_rng(1))
+    cache = paged.PagedKVCache.allocate(pages, page, kv, dim, dtype=dtype, bit_rate=None if bits == 16 else bits, device=DEV)
+    fill(cache)
+    q = (torch.randn(len(lengths), heads, dim, device=DEV) * sharp).to(dtype)
+    tables = torch.from_numpy(tables).to(DEV)
+    out = paged.paged_attention(cache, q, tables, torch.tensor(lengths, dtype=torch.int32, device=DEV), window=window)
+    assert F.status_read(0)[0]
+    off, once, n = 0.0, 0.0, 0
+    for b, length in list(enumerate(lengths))[:12]:
+        t = torch.arange(max(0, length - window) if window else 0, length, device=DEV)
+        where = tables[b, t // page].long()
+        k, v = (values(x[where, t % page], bits, dim)[0] for x in (cache.k, cache.v))
+        s = dim ** -0.5 * torch.einsum("kgd,tkd->kgt", q[b].double().view(kv, -1, dim), k)
+        o = torch.einsum("kgt,tkd->kgd", torch.softmax(s, -1), v).reshape(heads, dim)
+        off += float((out[b].double() - o).square().sum())
+        once += float((o.to(dtype).double() - o).square().sum())
+        n += o.numel()
+    # A rounding's error is even over half a step, which holds bf16's 2^-9 and fp16's 2^-12 of a value on average; what else there is (fp32
+    # sums, weights of 16 bits and more: 2^-14 beside bf16 rows, 2^-19 otherwise, of values below 5 and independent of it) adds less
+    # than a tenth of that to the root of the squares.
+    assert off ** 0.5 <= 1.1 * once ** 0.5 + 2.0 ** -20 * n ** 0.5, (off ** 0.5, once ** 0.5)
+
+
+@pytest.mark.parametrize("page", [16, 8])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("rows", [1, 40, 3000])
+def test_infinite_values(rows, kind, page):
+    """An infinity among 16-bit values is the result of its column, two of either sign a NaN, whatever the weights."""
+    dtype = TYPES[kind]
+    cache = paged.PagedKVCache.allocate(-(-rows // page), page, 1, 64, dtype=dtype, device=DEV)
+    v = torch.randn(rows, 1, 64, device=DEV).to(dtype)
+    v[rows // 2, 0, 3] = math.inf
+    v[rows - 1, 0, 17] = -math.inf
+    v[0, 0, 40], v[rows - 1, 0, 40] = -math.inf, math.inf
+    q = torch.randn(1, 8, 64, device=DEV).to(dtype)
+    for k in (torch.zeros_like(v), torch.randn(rows, 1, 64, device=DEV).to(dtype)):      # weights of powers of two, and others
+        tables = rows_of(cache, rows, k, v)
+        out = paged.paged_attention(cache, q, tables, torch.tensor([rows], dtype=torch.int32, device=DEV))[0]
+        assert (out[:, 3] == math.inf).all() and (out[:, 17] == -math.inf).all()
+        assert out[:, 40].isnan().all() if rows > 1 else (out[:, 40] == math.inf).all()
+        others = [c for c in range(64) if c not in (3, 17, 40)]
+        assert out[:, others].isfinite().all()
