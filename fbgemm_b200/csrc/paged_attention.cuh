@@ -27,13 +27,15 @@
 // set: 4-bit codes in the lowest 4 bits cost 6 bits of the sums, and results that were off by 1e-3.)
 //
 // One pass with a running maximum and sum per head in fp32 (in registers, per warp).  A tile's largest score is looked
-// for across lanes only if one exceeds the running maximum by more than 2^kSlack.  A weight enters the second product as two
-// 16-bit numbers, itself rounded and what that leaves: bf16 beside bf16 rows, 16 bits together; fp16 otherwise (2^10 times as large, so
-// that weights down to 2^-13 of the largest keep 22 bits, down to 2^-24 eleven, down to 2^-34 some), with the quantized rows' scales taken
-// relative to the largest power of two seen so far.  (One number alone: errors against 64 bits of up to 1.55 times those of the output's own
-// rounding, 2.1e-3 for 1.7e-3 over 64 requests of up to 8192 bf16 rows.  The second one's products take 1 to 3 % of the time, 9 % over
-// 128 requests of 1000 4-bit rows.)  Beside 16-bit rows the first is rounded towards zero and the second is not 0 unless the weight is: so an
-// infinite value stays one (no inf - inf, no 0 inf).
+// for across lanes only if one exceeds the running maximum by more than 2^kSlack.  Weights are rounded to 16 bits for the
+// second product: bf16 beside bf16 rows; fp16 otherwise (2^10 times as large, so that weights down to 2^-24 of the largest keep all 11
+// bits), with the quantized rows' scales taken relative to the largest power of two seen so far.  Where that rounding is as coarse as
+// the output's, what it leaves out enters as a second 16-bit number.  (Alone: errors against 64 bits of up to 1.55 times those of the
+// output's rounding, 2.1e-3 for 1.7e-3 over 64 requests of up to 8192 bf16 rows.  The second number's products take 1 to 3 % of the
+// time, 9 % over 128 requests of 1000 4-bit rows.)  Beside 16-bit rows the first is rounded towards zero, and the second is not 0 unless
+// the weight is: so an infinite value stays one (no inf - inf, no 0 inf).  Beside quantized rows and a bf16 output, eight times as coarse
+// as fp16 weights, codes are weighed about the middle of their range instead (sum w (c - 128) = sum w c - 128 sum w, with the rounded
+// w), which keeps the weights' roundings to the values' own size (8-bit rows, 32 requests of up to 16384: 130 us, 135 with two numbers).
 //
 // Work is split over the chip by paged_cache.h's rule: a worker is a warp (or the HW warps that share rows), and nothing
 // makes warps wait for one another, so that what a warp does between two items (its results out, the next queries in) is
@@ -44,7 +46,7 @@
 // joins its results through distributed shared memory: one launch.
 //
 // Measured over 32 requests of 16384 rows of 8 heads of 128 columns: 16-bit rows 320 to 325 us, 6.7 TB/s, what a plain copy
-// reaches.  8-bit rows 207 us, 0.84 of that rate, and 4-bit ones 153, 0.57: a tile is half or a quarter of the bytes and
+// reaches.  8-bit rows 204 us, 0.85 of that rate, and 4-bit ones 153, 0.57 (fp16, 141 bf16): a tile is half or a quarter of the bytes and
 // no fewer instructions (about 750 of a warp for 32 4-bit rows, three warps a scheduler, one instruction in two cycles),
 // whose chain from the scores through the weights to the sums is what a tile takes.  Below some 100 us a fixed 15 us shows:
 // 4 until the first rows are there, the slowest SM's 10 behind the mean one, and the join.
@@ -286,6 +288,9 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
   constexpr int BITS = S::BITS, NT = S::NT, SUB = S::SUB;
   constexpr bool kQuantized = BITS != 16;
   constexpr bool kMmaBf16 = !kQuantized && BF16;
+  constexpr bool kRest = !(kQuantized && BF16);   // weights enter with what their rounding leaves out
+  constexpr bool kCentred = kQuantized && !kRest;
+  constexpr float kMiddle = BITS == 8 ? 128.f : 8.f;
   constexpr float kWeight = Weights<S, BF16>::kWeight, kResult = Weights<S, BF16>::kResult;
   constexpr float kCode = BITS == 4 ? 1.f / 1048576.f : 1.f / 16777216.f;  // what a code of 1 is to the products
   constexpr unsigned kFull = S::ROWS == 32 ? kAll : (1u << (S::ROWS & 31)) - 1;
@@ -785,9 +790,9 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
 
     const bool any_far = kQuantized && BF16 && __any_sync(kAll, far != 0);
     float o[NT][S::MT][4];
-    // m: what weights are relative to, base = m, or 0 before the first; l: their sum over this lane's rows, bias_sum: that of the
-    // weights times the rows' biases
-    float m[NT][2], base[NT][2], l[NT][2], bias_sum[NT][2];
+    // m: what weights are relative to, base = m, or 0 before the first; l: their sum over this lane's rows; of the rounded weights
+    // w_sum (centred codes), of the weights times the rows' biases bias_sum
+    float m[NT][2], base[NT][2], l[NT][2], w_sum[NT][2], bias_sum[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -798,7 +803,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
       for (int x = 0; x < 2; ++x) {
         m[n][x] = -INFINITY;
         base[n][x] = 0.f;
-        l[n][x] = bias_sum[n][x] = 0.f;
+        l[n][x] = w_sum[n][x] = bias_sum[n][x] = 0.f;
       }
     }
     // V's scales are taken relative to 2^(exponent - 127) = 2^10 / v_unit, and are below scale_limit, twice that.
@@ -1010,6 +1015,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
             const float f = __fmul_rn(fade, fade_scale);
             if constexpr (kQuantized) {
               bias_sum[n][x] = __fmul_rn(bias_sum[n][x], fade);
+              w_sum[n][x] = __fmul_rn(w_sum[n][x], f);
             }
 #pragma unroll
             for (int k = 0; k < S::MT; ++k) {
@@ -1026,7 +1032,7 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float vs = kQuantized ? __fmul_rn(v_sb[s][r].x, v_unit) : 1.f;
-          const float vb = kQuantized ? __fmul_rn(v_sb[s][r].y, kSmall) : 0.f;
+          const float vb = __fmul_rn(kCentred ? __fmaf_rn(kMiddle, v_sb[s][r].x, v_sb[s][r].y) : v_sb[s][r].y, kSmall);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             float e[2];
@@ -1043,12 +1049,17 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
             }
             const uint32_t w = pack<kMmaBf16, !kQuantized>(e[0], e[1]);
             const float2 held = kMmaBf16 ? make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)) : halves(w);
-            uint32_t left_out = pack<kMmaBf16>(e[0] - held.x, e[1] - held.y);
-            if constexpr (!kQuantized) {
-              left_out |= __vminu2(w, 0x00010001u);  // (the last bit, where the weight is not 0)
-            }
             wt[n][s][r] = transposed(w);
-            rest[n][s][r] = transposed(left_out);
+            if constexpr (kRest) {
+              uint32_t left_out = pack<kMmaBf16>(e[0] - held.x, e[1] - held.y);
+              if constexpr (!kQuantized) {
+                left_out |= __vminu2(w, 0x00010001u);  // (the last bit, where the weight is not 0)
+              }
+              rest[n][s][r] = transposed(left_out);
+            } else {
+              w_sum[n][0] += held.x;
+              w_sum[n][1] += held.y;
+            }
           }
         }
       }
@@ -1075,7 +1086,9 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                   mma<false>(o[n][b + h], a0, a1, a2, a3, wt[n][s][0], wt[n][s][1]);
-                  mma<false>(o[n][b + h], a0, a1, a2, a3, rest[n][s][0], rest[n][s][1]);
+                  if constexpr (kRest) {
+                    mma<false>(o[n][b + h], a0, a1, a2, a3, rest[n][s][0], rest[n][s][1]);
+                  }
                 }
               } else {
 #pragma unroll
@@ -1085,7 +1098,9 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
 #pragma unroll
                   for (int n = 0; n < NT; ++n) {
                     mma<false>(o[n][2 * (b + h) + j], a0, a1, a2, a3, wt[n][s][0], wt[n][s][1]);
-                    mma<false>(o[n][2 * (b + h) + j], a0, a1, a2, a3, rest[n][s][0], rest[n][s][1]);
+                    if constexpr (kRest) {
+                      mma<false>(o[n][2 * (b + h) + j], a0, a1, a2, a3, rest[n][s][0], rest[n][s][1]);
+                    }
                   }
                 }
               }
@@ -1108,6 +1123,9 @@ paged_attention_kernel(const PagedAttentionParams p, const __grid_constant__ CUt
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         float sum_l = l[n][x], sum_b = bias_sum[n][x];
+        if constexpr (kCentred) {
+          sum_b = __fmaf_rn(__fmul_rn(__fmul_rn(w_sum[n][x], kSmall / 1024.f), unit), -kMiddle, sum_b);
+        }
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) {
           sum_l += __shfl_xor_sync(kAll, sum_l, d);

@@ -239,9 +239,9 @@ def paged_attention(cache: PagedKVCache, q: torch.Tensor, block_tables: torch.Te
 
     Scores, sums and the output are fp32 until the output's one rounding; the
     weights enter the sum over rows as two 16-bit numbers each (bfloat16 beside a
-    bfloat16 cache: 16 bits; float16 beside others: 22 bits; beside quantized rows
-    times the row's scale, each row off by up to 2**-35 of the widest row's
-    range).  A page outside the cache
+    bfloat16 cache: 16 bits; float16 beside others: 22 bits, beside quantized rows
+    with bfloat16 queries 11; beside quantized rows times the row's scale, each row
+    off by up to 2**-35 of the widest row's range).  A page outside the cache
     is left out (status {7, request, row, page}; all of a request's pages: a
     request without rows); a length that is negative or
     beyond the table is brought within it (status {3, request, 0, length})."""
