@@ -45,8 +45,8 @@
 // all work on one item joins theirs first.  Short items are left to a block each, or to a cluster of two, four or eight that
 // joins its results through distributed shared memory: one launch.
 //
-// Measured over 32 requests of 16384 rows of 8 heads of 128 columns: 16-bit rows 320 to 325 us, 6.7 TB/s, what a plain copy
-// reaches.  8-bit rows 204 us, 0.85 of that rate, and 4-bit ones 153, 0.57 (fp16, 141 bf16): a tile is half or a quarter of the bytes and
+// Measured over 32 requests of 16384 rows of 8 heads of 128 columns: 16-bit rows 323 to 326 us, 6.6 TB/s, what a plain copy
+// reaches.  8-bit rows 207 us, 0.84 of that rate, and 4-bit ones 141, 0.62 (beside fp16 queries 153): a tile is half or a quarter of the bytes and
 // no fewer instructions (about 750 of a warp for 32 4-bit rows, three warps a scheduler, one instruction in two cycles),
 // whose chain from the scores through the weights to the sums is what a tile takes.  Below some 100 us a fixed 15 us shows:
 // 4 until the first rows are there, the slowest SM's 10 behind the mean one, and the join.
