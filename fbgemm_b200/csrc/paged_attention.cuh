@@ -7,8 +7,8 @@
 // Bound by memory: a cached row is read once and used for the `group` query heads that share it, 2 operations per byte
 // and head.  That is too much for the fp32 units (8 heads on 4-bit rows: 200 TFLOP/s at the memory's rate) and little for
 // the tensor units.  The large tensor instructions read shared memory, where codes would have to be written back as numbers
-// first; the small ones take registers.  The rows are M and the heads N of m16n8k16: S^T = K Q^T takes 16 rows and 8 heads, O^T = V^T P^T 16 columns and 8 heads,
-// nothing is padded at 8 heads.  P^T is turned to the second product's layout by movmatrix.
+// first; the small ones take registers.  The rows are M and the heads N of m16n8k16: S^T = K Q^T takes 16 rows and 8 heads,
+// O^T = V^T P^T 16 columns and 8 heads, nothing is padded at 8 heads.  P^T is turned to the second product's layout by movmatrix.
 //
 // At 44 GB/s per SM and a microsecond of latency about 44 KB have to be on their way to every SM all the time.  Each
 // warp has a ring of half tiles (16 or 32 rows of K, or of V) in shared memory that it fills by asynchronous copies of
@@ -46,8 +46,8 @@
 // joins its results through distributed shared memory: one launch.
 //
 // Measured over 32 requests of 16384 rows of 8 heads of 128 columns: 16-bit rows 323 to 326 us, 6.6 TB/s, what a plain copy
-// reaches.  8-bit rows 207 us, 0.84 of that rate, and 4-bit ones 141, 0.62 (beside fp16 queries 153): a tile is half or a quarter of the bytes and
-// no fewer instructions (about 750 of a warp for 32 4-bit rows, three warps a scheduler, one instruction in two cycles),
+// reaches.  8-bit rows 207 us, 0.84 of that rate, and 4-bit ones 141, 0.62 (beside fp16 queries 153): a tile is half or a
+// quarter of the bytes and no fewer instructions (about 750 of a warp for 32 4-bit rows, three warps a scheduler, one instruction in two cycles),
 // whose chain from the scores through the weights to the sums is what a tile takes.  Below some 100 us a fixed 15 us shows:
 // 4 until the first rows are there, the slowest SM's 10 behind the mean one, and the join.
 #pragma once
